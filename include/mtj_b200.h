@@ -132,9 +132,10 @@ typedef struct mtj_stack_desc {
 } mtj_stack_desc;
 
 const char* mtj_last_error(void);
-/* ABI revision: 6 (2: mtj_config with the tuning fields, mtj_generate, mtj_start_batch / mtj_admit;
+/* ABI revision: 7 (2: mtj_config with the tuning fields, mtj_generate, mtj_start_batch / mtj_admit;
  * 3: top_k in mtj_sample_top_p / mtj_nucleus_filter, mtj_set_top_k; 4: layer-stack models, mtj_extend,
- * mtj_release; 5: more mixers and residual forms in mtj_stack_desc; 6: mtj_k_out_projection_pieces). */
+ * mtj_release; 5: more mixers and residual forms in mtj_stack_desc; 6: mtj_k_out_projection_pieces;
+ * 7: mtj_k_cache_attn, mtj_k_cache_evict, mtj_verify_drafts). */
 int32_t mtj_version(void);
 
 /* CausalTransformerShard.__init__ (transformer_shard.py:21-45): validates the
@@ -465,6 +466,111 @@ int32_t mtj_k_decode_attn_noalloc(const float* q_dev, const void* kpool_dev, con
                                   const int32_t* cur_dev, int32_t batch, int32_t heads, int32_t d_head,
                                   int32_t window, int32_t ring_pages, int32_t split_tokens,
                                   float* out_dev, int32_t ld_out, mtj_stream s);
+
+/* No counterpart in the reference, whose decode window forgets its oldest tokens and whose scan takes one token a step.
+ * Attention of new tokens over a cache of the layout of mtj_k_decode_attn, with grouped heads, a sliding window and a few
+ * first tokens that stay visible.  Sequence b holds lengths[b] slots, slot i in row i % 64 of page page_table[b][i / 64],
+ * its new_tokens[b] newest ones being those of this call: token t sits in slot p = lengths[b] - new_tokens[b] + t and sees
+ * slot j when j <= p and (j < sinks or p - j < window).
+ *     score_j = scale * q . k_j;   a_j = exp(score_j) / sum over the visible slots;   out = sum a_j v_j
+ * Query head h reads key head h / (heads / kv_heads).  With k_new_dev and v_new_dev the tokens' keys (rotated by the caller)
+ * and values are put into their slots first, rounded to bf16; without (both NULL) they are there already.
+ * Rows of q, k_new, v_new and out: [batch][tokens] with ld_* elements from one token to the next (multiples of 8), heads
+ * side by side within a row, type `dtype` (MTJ_BF16 or MTJ_F32); all pointers 16-byte aligned.  Rows t >= new_tokens[b] of
+ * out become zeros; those of k_new and v_new are not used.  Slots behind lengths[b] are never read into a result.
+ * weights_out_dev [batch][kv_heads][pages * 64] f32 (or NULL) receives for every slot j < lengths[b]
+ *     (j new ? 0 : weights_in_dev[j]) + sum of a_j over the call's tokens and the heads of the group,
+ * weights_in_dev NULL standing for zeros; both may be the same array.
+ * A sequence whose length is negative, below its new_tokens or beyond its pages is treated as empty, a page number outside
+ * [0, n_pages) as a page that nobody sees; either sets bit 1 of *status_dev (may be NULL), a bounded wait that runs out
+ * bit 0.  Queries of one call see the values of all its tokens multiplied by weight zero, so new values must be finite.
+ * d_head 64, 128 or 256; at most MTJ_CACHE_MAX_GROUP query heads per key head.  The scratch needs no initial contents.
+ * Calls that may overlap need scratch of their own. */
+#define MTJ_CACHE_MAX_GROUP 64
+typedef struct mtj_cache_attn_args {
+  void* kpool_dev;                  /* bf16 [n_pages][kv_heads][64][d_head]           */
+  void* vpool_dev;
+  const int32_t* page_table_dev;    /* [batch][pages]                                 */
+  const int32_t* lengths_dev;       /* [batch] slots in use, the new tokens included  */
+  const int32_t* new_tokens_dev;    /* [batch], NULL: `tokens` each                   */
+  uint32_t* status_dev;
+  const void* q_dev;
+  const void* k_new_dev;
+  const void* v_new_dev;
+  void* out_dev;
+  const float* weights_in_dev;
+  float* weights_out_dev;
+  int64_t ld_q, ld_k, ld_v, ld_out;
+  int32_t n_pages, batch, pages, heads, kv_heads, d_head;
+  int32_t tokens;                   /* rows per sequence, 1 <= tokens <= pages * 64   */
+  int32_t dtype;
+  int32_t window, sinks;            /* window >= 1, sinks >= 0                        */
+  float scale;                      /* > 0                                            */
+} mtj_cache_attn_args;
+int64_t mtj_k_cache_attn_scratch_bytes(const mtj_cache_attn_args* a);   /* -1: the arguments are refused */
+int32_t mtj_k_cache_attn(const mtj_cache_attn_args* a, void* scratch_dev, int64_t scratch_bytes, mtj_stream s);
+
+/* No counterpart in the reference.  Eviction from such a cache by accumulated attention weight: every key head of a
+ * sequence that holds more than `keep` slots keeps its first `first` slots, its last `last` slots and of the others the
+ * keep - first - last with the largest weights (the lower slot among equals), in the order of their slots.  The kept keys
+ * and values are copied to slots 0 .. keep - 1 of the sequence's spare pages, which its row of the new table names, with -1
+ * behind them.  Other sequences keep their pages.
+ *   kept_out [batch][kv_heads][keep]: the slots that were kept, -1 behind the last one;
+ *   weights_out [batch][kv_heads][pages * 64]: their weights, 0 behind the last one (may be weights_dev itself);
+ *   lengths_out [batch], page_table_out [batch][pages]: arrays other than the old ones.
+ * spare_pages [batch][(keep + 63) / 64] are pages that no sequence of the batch uses and that are named once; the old
+ * pages are the caller's again when the call has run.  A bad length or page number is treated as by mtj_k_cache_attn (rows
+ * of such a page are not copied). */
+typedef struct mtj_cache_evict_args {
+  void* kpool_dev;
+  void* vpool_dev;
+  const int32_t* page_table_dev;
+  const int32_t* lengths_dev;
+  const float* weights_dev;
+  const int32_t* spare_pages_dev;
+  int32_t* kept_out_dev;
+  int32_t* lengths_out_dev;
+  float* weights_out_dev;
+  int32_t* page_table_out_dev;
+  uint32_t* status_dev;
+  int32_t n_pages, batch, pages, kv_heads, d_head;
+  int32_t keep, first, last;        /* keep >= 1, first, last >= 0, first + last <= keep */
+} mtj_cache_evict_args;
+int32_t mtj_k_cache_evict(const mtj_cache_evict_args* a, mtj_stream s);
+
+/* No counterpart in the reference, whose scan samples every token on its own (transformer_shard.py:198-210).  Speculative
+ * decoding: which of the drafted tokens x_0 .. x_{n-1} of every sequence the target model takes, and the token behind
+ * them.  With p_k = softmax(target row k / temp), q_k = softmax(draft row k / temp), or q_k = 1 at x_k when
+ * draft_dev is NULL (tokens that were looked up), token k is taken while
+ *     accept[k] * q_k(x_k) < p_k(x_k);
+ * at the first k that is not, the next token comes from max(p_k - q_k, 0), behind all n from p_n, as arg max of
+ *     r_i / -log(noise_i)          (the lowest index among equals; r = p where the difference is zero everywhere),
+ * so that the tokens are distributed as samples of the target.  temp <= 0 (or NaN): p_k is 1 at the first largest entry of its row, a draft
+ * is taken when it is that entry, and accept, noise and the draft's logits are not used.
+ * target [batch][drafts + 1][vocab], draft [batch][drafts][vocab], type `dtype`, with ld_* elements from row to row and
+ * batch_* from sequence to sequence; -inf and the lowest value are shares of zero.  draft_tokens [batch][drafts] (outside
+ * [0, vocab): never taken); accept [batch][drafts], noise [batch][vocab] uniforms in [tiny, 1); counts [batch] drafted
+ * tokens of each sequence (NULL: drafts; clamped to [0, drafts]); temp_dev [batch], or NULL: `temp` for all.
+ * tokens_out [batch][drafts + 1]: the taken tokens, the next one, -1 behind it; accepted_out [batch]; logprobs_out
+ * [batch][drafts + 1] (or NULL): log p_k of every token that comes out, 0 behind the last. */
+typedef struct mtj_verify_args {
+  const void* target_dev;
+  const void* draft_dev;
+  const int32_t* draft_tokens_dev;
+  const float* accept_dev;
+  const float* noise_dev;
+  const int32_t* counts_dev;
+  const float* temp_dev;
+  int32_t* tokens_out_dev;
+  int32_t* accepted_out_dev;
+  float* logprobs_out_dev;
+  int64_t ld_target, batch_target, ld_draft, batch_draft;
+  int32_t batch, drafts, vocab;     /* drafts >= 0                                    */
+  int32_t dtype;
+  float temp;
+} mtj_verify_args;
+int64_t mtj_verify_scratch_bytes(const mtj_verify_args* a);             /* -1: the arguments are refused */
+int32_t mtj_verify_drafts(const mtj_verify_args* a, void* scratch_dev, int64_t scratch_bytes, mtj_stream s);
 
 #ifdef __cplusplus
 }

@@ -45,6 +45,31 @@ class MtjStackDesc(ctypes.Structure):
                 + [("act_f32", ctypes.c_int32), ("tc_min_rows", ctypes.c_int32)])
 
 
+class MtjCacheAttnArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "kpool", "vpool", "page_table", "lengths", "new_tokens", "status", "q", "k_new", "v_new", "out", "weights_in",
+        "weights_out")]
+        + [(n, ctypes.c_int64) for n in ("ld_q", "ld_k", "ld_v", "ld_out")]
+        + [(n, ctypes.c_int32) for n in (
+            "n_pages", "batch", "pages", "heads", "kv_heads", "d_head", "tokens", "dtype", "window", "sinks")]
+        + [("scale", ctypes.c_float)])
+
+
+class MtjCacheEvictArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "kpool", "vpool", "page_table", "lengths", "weights", "spare_pages", "kept_out", "lengths_out", "weights_out",
+        "page_table_out", "status")]
+        + [(n, ctypes.c_int32) for n in ("n_pages", "batch", "pages", "kv_heads", "d_head", "keep", "first", "last")])
+
+
+class MtjVerifyArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "target", "draft", "draft_tokens", "accept", "noise", "counts", "temp_per_row", "tokens_out", "accepted_out",
+        "logprobs_out")]
+        + [(n, ctypes.c_int64) for n in ("ld_target", "batch_target", "ld_draft", "batch_draft")]
+        + [(n, ctypes.c_int32) for n in ("batch", "drafts", "vocab", "dtype")] + [("temp", ctypes.c_float)])
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -99,6 +124,11 @@ def _load():
         "mtj_k_prefill_attn": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp]),
         "mtj_k_all_reduce_buffer_bytes": (i64, [vp, i32]),
         "mtj_k_all_reduce": (i32, [vp, ctypes.POINTER(vp), i32, i32, i32, i32, vp, vp, vp, i32, vp]),
+        "mtj_k_cache_attn_scratch_bytes": (i64, [ctypes.POINTER(MtjCacheAttnArgs)]),
+        "mtj_k_cache_attn": (i32, [ctypes.POINTER(MtjCacheAttnArgs), vp, i64, vp]),
+        "mtj_k_cache_evict": (i32, [ctypes.POINTER(MtjCacheEvictArgs), vp]),
+        "mtj_verify_scratch_bytes": (i64, [ctypes.POINTER(MtjVerifyArgs)]),
+        "mtj_verify_drafts": (i32, [ctypes.POINTER(MtjVerifyArgs), vp, i64, vp]),
         "mtj_k_decode_attn": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64, vp, i32, vp]),
     }
     partial = not LIB_PATH.endswith("libmtj_b200.so")

@@ -1,0 +1,160 @@
+"""Paged key / value caches in the caller's hands: attention of new tokens with a sliding window and first tokens that stay
+visible, and eviction by the attention weight that cached tokens have received.
+
+No counterpart in the reference, whose ``decode_once`` (layers.py:316-344) keeps the last ``seq - 1`` tokens of every sequence.
+A cache is tensors on one GPU: ``kpool`` and ``vpool`` bf16 ``[n_pages, kv_heads, 64, d_head]`` (the layout of the runtime's own
+caches; keys rotated by the caller), ``page_table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]``, which layers of one
+model can share.  Everything runs on the current stream of the tensors' GPU, allocates nothing but its results and its scratch,
+reads nothing back, and can be captured into a CUDA graph.  Nothing here records gradients.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._lib import MTJ_BF16, MTJ_F32, MtjCacheAttnArgs, MtjCacheEvictArgs, check, lib
+
+PAGE_TOKENS = 64
+_DTYPES = {torch.bfloat16: MTJ_BF16, torch.float32: MTJ_F32}
+
+
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _want(t, name, dtype, shape, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+
+
+def _pool_shape(kpool, vpool, page_table, lengths):
+    if not (isinstance(kpool, torch.Tensor) and kpool.is_cuda and kpool.dim() == 4 and kpool.shape[2] == PAGE_TOKENS):
+        raise ValueError(f"kpool must be a CUDA tensor [n_pages, kv_heads, {PAGE_TOKENS}, d_head]")
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError("page_table must be a tensor [batch, pages]")
+    shape, device, table = kpool.shape, kpool.device, page_table.shape
+    _want(kpool, "kpool", torch.bfloat16, shape, device)
+    _want(vpool, "vpool", torch.bfloat16, shape, device)
+    _want(page_table, "page_table", torch.int32, table, device)
+    _want(lengths, "lengths", torch.int32, table[:1], device)
+    return shape, table, device
+
+
+def _rows(t, name, heads, d_head, like):
+    """``t`` [batch, tokens, heads, d_head] with heads side by side in a row, rows at one stride and 16-byte aligned (a slice
+    of a fused projection is one); anything else is copied."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or \
+            t.shape[:2] != like.shape[:2] or t.shape[2] != heads or t.shape[3] != d_head:
+        raise ValueError(f"{name} must be a {like.dtype} tensor {[*like.shape[:2], heads, d_head]} on {like.device}")
+    s = t.stride()
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t, heads * d_head
+    ld = s[1] if t.shape[1] > 1 else s[0] if t.shape[0] > 1 else heads * d_head
+    if s[3] == 1 and (s[2] == d_head or heads == 1) and ld >= heads * d_head and not ld & 7 and not t.data_ptr() & 15 and \
+            (t.shape[0] == 1 or s[0] == ld * t.shape[1]):
+        return t, ld
+    return t.contiguous() if not t.is_contiguous() else t.clone(), heads * d_head
+
+
+def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window=None, sinks=0, scale=None, weights=None,
+                    weights_out=None, out=None, status=None):
+    """Appends the new tokens' keys and values to the cache and attends from them over it.
+
+    ``q`` [batch, tokens, heads, d_head] bf16 or float32; ``k``, ``v`` [batch, tokens, kv_heads, d_head] of the same type, or both
+    None when the cache holds them already.  ``lengths`` counts the slots in use with the new tokens; ``new`` int32 [batch] says
+    how many of the ``tokens`` rows of each sequence are new ones (default: all).  Token t of sequence b sits in slot
+    ``p = lengths[b] - new[b] + t`` and sees slot j when ``j <= p and (j < sinks or p - j < window)`` (``window`` None: all).
+    Scores are multiplied by ``scale`` (default ``d_head ** -0.5``).  Returns ``out`` like ``q``; rows from ``new[b]`` on are zeros.
+
+    ``weights`` float32 [batch, kv_heads, pages * 64]: the attention weight that each slot receives, summed over the tokens and
+    over the query heads that read its head, is added to it, slots of new tokens beginning at zero.  With ``weights_out`` the
+    sums go there and ``weights`` (may be None: zeros) stays as it is.
+
+    ``status`` int32 [1], if given, collects what the GPU found wrong: bit 1 a length or a page number outside the cache (that
+    sequence counts as empty, that page as unseen), bit 0 a wait that ran out."""
+    (n_pages, kv_heads, _, d_head), (batch, pages), device = _pool_shape(kpool, vpool, page_table, lengths)
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES or q.device != device or q.shape[0] != batch or \
+            q.shape[3] != d_head or q.shape[1] < 1 or q.shape[2] < 1:
+        raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
+    tokens, heads = q.shape[1:3]
+    if (k is None) != (v is None):
+        raise ValueError("k and v come together")
+    q, ld_q = _rows(q, "q", heads, d_head, q)
+    ld_k = ld_v = 0
+    if k is not None:
+        k, ld_k = _rows(k, "k", kv_heads, d_head, q)
+        v, ld_v = _rows(v, "v", kv_heads, d_head, q)
+    if new is not None:
+        _want(new, "new", torch.int32, lengths.shape, device)
+    if status is not None:
+        _want(status, "status", torch.int32, (1,), device)
+    if weights is not None or weights_out is not None:
+        if weights_out is None:
+            weights_out = weights
+        _want(weights_out, "weights_out", torch.float32, (batch, kv_heads, pages * PAGE_TOKENS), device)
+        if weights is not None and weights is not weights_out:
+            _want(weights, "weights", torch.float32, weights_out.shape, device)
+    if out is None:
+        out = torch.empty((batch, tokens, heads, d_head), dtype=q.dtype, device=device)
+        ld_out = heads * d_head
+    else:
+        given = out
+        out, ld_out = _rows(out, "out", heads, d_head, q)
+        if out is not given:
+            raise ValueError("out must have its heads side by side, rows at one stride and a 16-byte alignment")
+    a = MtjCacheAttnArgs(
+        kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), new.data_ptr() if new is not None else None,
+        status.data_ptr() if status is not None else None, q.data_ptr(), k.data_ptr() if k is not None else None,
+        v.data_ptr() if k is not None else None, out.data_ptr(), weights.data_ptr() if weights is not None else None,
+        weights_out.data_ptr() if weights_out is not None else None, ld_q, ld_k, ld_v, ld_out, n_pages, batch, pages, heads,
+        kv_heads, d_head, tokens, _DTYPES[q.dtype], pages * PAGE_TOKENS if window is None else min(int(window), 0x7fffffff),
+        min(int(sinks), 0x7fffffff), d_head ** -0.5 if scale is None else scale)
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            _run_attention(a, device, index)
+    else:
+        _run_attention(a, device, index)
+    return out
+
+
+def _run_attention(a, device, index):
+    ref = ctypes.byref(a)
+    nbytes = lib.mtj_k_cache_attn_scratch_bytes(ref)
+    if nbytes < 0:
+        raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    check(lib.mtj_k_cache_attn(ref, scratch.data_ptr(), nbytes, _stream(index)))
+
+
+def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, first=0, last=0, status=None):
+    """Cuts every sequence that holds more than ``keep`` slots down to ``keep``: each key head keeps the ``first`` first slots, the
+    ``last`` last ones and the heaviest by ``weights`` of the others (the lower slot among equals), in the order of their slots.
+
+    The kept keys and values are copied to ``spare_pages`` int32 [batch, ceil(keep / 64)], pages that no sequence uses, each
+    named once.  Returns ``(kept, lengths, weights, page_table)``, new tensors: the slots that were kept [batch, kv_heads, keep]
+    (-1 behind the last), and the cache as it is now.  The new table of a sequence that was cut names its spare pages, with -1
+    behind them where the caller puts pages for the tokens to come; its old pages are free again.  Sequences of ``keep`` slots
+    or fewer keep their pages and leave their spare ones unused."""
+    (n_pages, kv_heads, _, d_head), (batch, pages), device = _pool_shape(kpool, vpool, page_table, lengths)
+    keep, first, last = int(keep), int(first), int(last)
+    if keep < 1 or first < 0 or last < 0 or first + last > keep:
+        raise ValueError("keep must be positive and hold the first and the last slots")
+    _want(weights, "weights", torch.float32, (batch, kv_heads, pages * PAGE_TOKENS), device)
+    _want(spare_pages, "spare_pages", torch.int32, (batch, (keep + PAGE_TOKENS - 1) // PAGE_TOKENS), device)
+    if status is not None:
+        _want(status, "status", torch.int32, (1,), device)
+    kept = torch.empty((batch, kv_heads, keep), dtype=torch.int32, device=device)
+    lengths_out, weights_out, table_out = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(page_table)
+    a = MtjCacheEvictArgs(
+        kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), weights.data_ptr(), spare_pages.data_ptr(),
+        kept.data_ptr(), lengths_out.data_ptr(), weights_out.data_ptr(), table_out.data_ptr(),
+        status.data_ptr() if status is not None else None, n_pages, batch, pages, kv_heads, d_head, keep, first, last)
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            check(lib.mtj_k_cache_evict(ctypes.byref(a), _stream(index)))
+    else:
+        check(lib.mtj_k_cache_evict(ctypes.byref(a), _stream(index)))
+    return kept, lengths_out, weights_out, table_out

@@ -11,10 +11,12 @@ the kernel's own selection); the top-k branch of the reference filter
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 
-from ._lib import check, lib
+from ._lib import MTJ_BF16, MTJ_F32, MtjVerifyArgs, check, lib
 
 TINY = float(np.finfo(np.float32).tiny)
 
@@ -93,3 +95,80 @@ def nucleaus_filter(logits, top_p=0.9, top_k=None):
                                      rows, vocab, out.data_ptr(),
                                      torch.cuda.current_stream(dev).cuda_stream))
         return out
+
+
+_LOGIT_TYPES = {torch.float32: MTJ_F32, torch.bfloat16: MTJ_BF16}
+
+
+def _logit_rows(t, name, like, rows):
+    """``t`` [batch, rows, vocab] with unit stride inside a row; anything else is copied."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype != like.dtype or t.device != like.device or \
+            t.shape != (like.shape[0], rows, like.shape[2]):
+        raise ValueError(f"{name} must be a {like.dtype} tensor {[like.shape[0], rows, like.shape[2]]} on {like.device}")
+    s = t.stride()
+    if s[2] != 1 and t.shape[2] > 1 or s[1] < t.shape[2]:
+        t = t.contiguous()
+        s = t.stride()
+    return t, max(s[1], t.shape[2]), s[0]
+
+
+def _plain_rows(t, name, dtype, shape, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on {device}")
+    return t.contiguous()
+
+
+def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, count=None, temp=1.0):
+    """Speculative decoding: which drafted tokens the target model takes, and the token behind them.
+
+    The reference samples one token a step (transformer_shard.py:198-210); with drafts a step yields up to ``drafts + 1``, whose
+    distribution is that of the target's own samples.  ``target_logits`` [batch, drafts + 1, vocab] float32 or bf16, row k behind k
+    drafted tokens; ``draft_logits`` [batch, drafts, vocab] the logits that the drafts were sampled from at the same temperature, or
+    None for tokens that were looked up rather than sampled; ``draft_tokens`` int32 [batch, drafts]; ``accept`` [batch, drafts] and
+    ``noise`` [batch, vocab] float32 uniforms in [tiny, 1) (``draw_uniforms``); ``count`` int32 [batch] drafted tokens of each sequence
+    (default: all); ``temp`` a number or float32 [batch], 0: greedy, where a draft is taken if it is the first largest logit.
+    Logits filtered by ``nucleaus_filter`` make it nucleus sampling.
+
+    Draft k is taken while ``accept * q_k(x_k) < p_k(x_k)``.  The next token is sampled from ``max(p_k - q_k, 0)`` at the first that
+    is not, from ``p`` behind the last.  Returns device tensors, nothing is read back: tokens int32 [batch, drafts + 1] (the
+    taken ones, the next one, -1 behind it), the number taken int32 [batch], and log p_k of every token that comes out float32
+    [batch, drafts + 1] (0 behind the last)."""
+    if not isinstance(target_logits, torch.Tensor) or not target_logits.is_cuda or target_logits.dim() != 3 or \
+            target_logits.dtype not in _LOGIT_TYPES or min(target_logits.shape) < 1:
+        raise ValueError("target_logits must be a float32 or bfloat16 CUDA tensor [batch, drafts + 1, vocab]")
+    batch, rows, vocab = target_logits.shape
+    drafts, dev = rows - 1, target_logits.device
+    target, ld_target, batch_target = _logit_rows(target_logits, "target_logits", target_logits, rows)
+    draft, ld_draft, batch_draft = None, 0, 0
+    if draft_logits is not None:
+        draft, ld_draft, batch_draft = _logit_rows(draft_logits, "draft_logits", target, drafts)
+    tokens = _plain_rows(draft_tokens, "draft_tokens", torch.int32, (batch, drafts), dev)
+    accept = _plain_rows(accept, "accept", torch.float32, (batch, drafts), dev)
+    noise = _plain_rows(noise, "noise", torch.float32, (batch, vocab), dev)
+    if count is not None:
+        count = _plain_rows(count, "count", torch.int32, (batch,), dev)
+    temps = None
+    if isinstance(temp, torch.Tensor):
+        temps, temp = _plain_rows(temp, "temp", torch.float32, (batch,), dev), 1.0
+    out = torch.empty((batch, rows), dtype=torch.int32, device=dev)
+    taken = torch.empty((batch,), dtype=torch.int32, device=dev)
+    logprobs = torch.empty((batch, rows), dtype=torch.float32, device=dev)
+    a = MtjVerifyArgs(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else None, tokens.data_ptr(),
+                      accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else None,
+                      temps.data_ptr() if temps is not None else None, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
+                      ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev.index):
+            _run_verify(a, dev)
+    else:
+        _run_verify(a, dev)
+    return out, taken, logprobs
+
+
+def _run_verify(a, dev):
+    ref = ctypes.byref(a)
+    nbytes = lib.mtj_verify_scratch_bytes(ref)
+    if nbytes < 0:
+        raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    check(lib.mtj_verify_drafts(ref, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev.index)))

@@ -1,0 +1,309 @@
+"""mesh_transformer.cache.cache_attention against 64-bit attention over the same bf16 cache.
+
+Tolerance of an output row, from the arithmetic: its storage rounds by half a step of its type relative to the value; scores in 32 bits
+(sums of up to 256 products) and exponentials are off by under 2^-18 of the largest score (below 16 here) and the weights are multiplied
+as bf16 numbers on the prompt path, half a step each, which the sum over values bounds by 2^-8 of the sum of |a v| at worst; the few-token
+path keeps the weights to 2^-16."""
+import numpy as np
+import pytest
+import torch
+
+from cache_util import PAGE, Cache, host, rounding
+from oracle import cache_oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(c, q, lengths, fresh, window, sinks, scale):
+    kp, vp = host(c.kpool), host(c.vpool)
+    outs, received, spread = [], [], []
+    for b, (n, f) in enumerate(zip(lengths, fresh)):
+        keys, values = cache_oracle.slots_of(kp, c.table[b], n), cache_oracle.slots_of(vp, c.table[b], n)
+        o, r = cache_oracle.attention(host(q[b, :f]), keys, values, n, f, window, sinks, scale)
+        m, _ = cache_oracle.attention(host(q[b, :f]), keys, np.abs(values), n, f, window, sinks, scale)
+        outs.append(o)
+        received.append(r)
+        spread.append(m)
+    return outs, received, spread
+
+
+def _check(out, outs, spread, dtype, weight_rounding):
+    for b, o in enumerate(outs):
+        got = host(out[b, :len(o)])
+        assert np.isfinite(got).all(), b
+        room = rounding(dtype) * np.abs(o) + (weight_rounding + 2.0 ** -14) * spread[b]
+        assert (np.abs(got - o) <= room + 1e-30).all(), (b, np.abs(got - o).max(), (np.abs(got - o) / room).max())
+        assert float(out[b, len(o):].float().abs().sum()) == 0.0, b
+
+
+def _run(seed, batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks, dtype, append=True, weights=False, scale=None,
+         padded=0):
+    from mesh_transformer.cache import cache_attention
+    pages = max(1, (max(max(lengths), tokens) + PAGE - 1) // PAGE) + 1
+    c = Cache(seed, batch, pages, kv_heads, d_head, lengths)
+    q = c.rows(batch, tokens, heads, d_head, dtype, 1.5)
+    k, v = c.rows(batch, tokens, kv_heads, d_head, dtype), c.rows(batch, tokens, kv_heads, d_head, dtype)
+    if padded:                                            # slices of one fused row
+        fused = torch.full((batch, tokens, (heads + 2 * kv_heads) * d_head + padded), float("nan"), dtype=dtype, device="cuda")
+        fused[..., :heads * d_head] = q.flatten(2)
+        fused[..., heads * d_head:(heads + kv_heads) * d_head] = k.flatten(2)
+        fused[..., (heads + kv_heads) * d_head:(heads + 2 * kv_heads) * d_head] = v.flatten(2)
+        q = fused[..., :heads * d_head].unflatten(2, (heads, d_head))
+        k = fused[..., heads * d_head:(heads + kv_heads) * d_head].unflatten(2, (kv_heads, d_head))
+        v = fused[..., (heads + kv_heads) * d_head:(heads + 2 * kv_heads) * d_head].unflatten(2, (kv_heads, d_head))
+    before = [c.kpool.clone(), c.vpool.clone()]
+    want = [c.kpool.clone(), c.vpool.clone()]
+    if append:
+        for b, (n, f) in enumerate(zip(lengths, fresh)):
+            for t in range(f):
+                slot = n - f + t
+                for pool, rows in zip(want, (k, v)):
+                    pool[int(c.table[b, slot // PAGE]), :, slot % PAGE] = rows[b, t].to(torch.bfloat16)
+    new = torch.tensor(fresh, dtype=torch.int32, device="cuda")
+    status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+    w_in = w_out = None
+    if weights:
+        w_in = torch.rand((batch, kv_heads, pages * PAGE), device="cuda", generator=torch.Generator("cuda").manual_seed(seed))
+        w_out = torch.full_like(w_in, -7.0)
+    out = cache_attention(q, k if append else None, v if append else None, c.kpool, c.vpool, c.page_table, c.lengths_dev, new=new,
+                          window=window, sinks=sinks, scale=scale, weights=w_in, weights_out=w_out, status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for got, exp in zip((c.kpool, c.vpool), want if append else before):
+        assert torch.equal(got.view(torch.int16), exp.view(torch.int16)), "slots other than the new ones changed, or the new ones did not"
+    outs, received, spread = _reference(c, q, lengths, fresh, window or pages * PAGE, sinks, d_head ** -0.5 if scale is None else scale)
+    return c, out, outs, received, spread, (w_in, w_out)
+
+
+FEW = [
+    # batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks
+    (1, 4, 4, 64, 1, [1], [1], 1, 0),                                      # a token that sees itself
+    (1, 4, 4, 64, 1, [127], [1], None, 0),
+    (2, 16, 16, 256, 1, [300, 1], [1, 1], 128, 4),
+    (3, 8, 2, 128, 1, [65, 64, 63], [1, 1, 1], 64, 1),                     # page borders
+    (4, 8, 1, 128, 5, [700, 5, 130, 64], [5, 1, 3, 0], 100, 70),           # drafts, first tokens beyond a page, nothing new
+    (2, 40, 8, 64, 3, [200, 77], [3, 2], 7, 16),                           # odd group
+    (2, 6, 2, 256, 8, [513, 90], [8, 8], 33, 0),
+    (1, 64, 1, 64, 2, [1000], [2], 999, 2),                                # the largest group
+    (5, 3, 3, 128, 1, [0, 1, 2, 1500, 129], [0, 1, 1, 1, 1], None, 5),     # an empty sequence beside a long one
+    (1, 2, 2, 128, 1, [6000], [1], None, 0),                               # one long sequence, cut into many pieces
+    (1, 8, 8, 64, 1, [4100], [1], 70, 130),                                # first tokens and window far apart
+    (2, 4, 2, 64, 16, [40, 16], [16, 16], 3, 2),                           # more new tokens than the window holds
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", FEW)
+def test_few_tokens(cuda_device, case, dtype):
+    batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks = case
+    _, out, outs, _, spread, _ = _run(3, batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks, dtype)
+    _check(out, outs, spread, dtype, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", FEW)
+def test_received_weights(cuda_device, case, dtype):
+    """Every slot's weight to 2^-13 of itself (scores as above, so exponentials to 2^-14, and the same for the sum below them);
+    slots that nobody sees keep what they had, slots behind the sequence are not written."""
+    batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks = case
+    _, out, outs, received, spread, (w_in, w_out) = _run(5, batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks, dtype,
+                                                         weights=True)
+    _check(out, outs, spread, dtype, 2.0 ** -16)
+    w_in, w_out = w_in.double().cpu().numpy(), w_out.double().cpu().numpy()
+    for b, (n, f) in enumerate(zip(lengths, fresh)):
+        before = w_in[b, :, :n].copy()
+        before[:, n - f:] = 0
+        want = before + received[b]
+        assert (np.abs(w_out[b, :, :n] - want) <= 2.0 ** -13 * received[b] + 2.0 ** -22 * want).all()
+        assert (w_out[b, :, n:] == -7.0).all()
+
+
+def test_weights_in_place_and_from_nothing(cuda_device):
+    from mesh_transformer.cache import cache_attention
+    c = Cache(1, 2, 3, 2, 64, [150, 20])
+    q = c.rows(2, 1, 4, 64, torch.bfloat16)
+    a = torch.zeros((2, 2, 192), device="cuda")
+    cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, weights_out=a)
+    total = a.sum(-1).cpu().numpy()
+    assert np.abs(total - 2.0).max() <= 1e-4                     # two heads a group, shares of one each
+    b = torch.ones_like(a)
+    cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, weights=b)
+    for i, n in enumerate((150, 20)):
+        want = a[i, :, :n] + 1.0
+        want[:, n - 1] -= 1.0                                    # the new token's slot begins at zero
+        assert torch.allclose(b[i, :, :n], want, atol=1e-6)
+        assert (b[i, :, n:] == 1.0).all()
+
+
+PROMPT = [
+    (1, 2, 2, 256, 200, [200], [200], None, 0),
+    (2, 4, 2, 128, 333, [500, 333], [333, 100], 64, 4),                    # history, ragged
+    (1, 4, 4, 64, 129, [129], [129], 1, 0),                                # every token sees itself alone
+    (1, 5, 1, 64, 257, [900], [257], 130, 70),                             # first tokens beyond a page
+    (3, 2, 2, 128, 64, [64, 0, 1], [64, 0, 1], 10, 3),                     # an empty sequence
+    (1, 2, 1, 256, 300, [1000], [300], 300, 16),
+    (2, 3, 3, 64, 100, [640, 639], [100, 99], 65, 64),                     # last token at a page's end and before it
+    (1, 8, 8, 128, 700, [700], [700], 2000, 4),                            # a window that hides nothing
+]
+
+
+@pytest.mark.parametrize("padded", [0, 24])
+@pytest.mark.parametrize("case", PROMPT)
+def test_prompts(cuda_device, case, padded):
+    batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks = case
+    _, out, outs, _, spread, _ = _run(7, batch, heads, kv_heads, d_head, tokens, lengths, fresh, window, sinks, torch.bfloat16, padded=padded)
+    _check(out, outs, spread, torch.bfloat16, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("tokens,weights", [(90, False), (40, True)])
+def test_prompts_in_32_bits_and_with_weights(cuda_device, tokens, weights):
+    _, out, outs, received, spread, (w_in, w_out) = _run(9, 2, 4, 2, 128, tokens, [200, tokens], [tokens, tokens - 3], 50, 4, torch.float32,
+                                                         weights=weights)
+    _check(out, outs, spread, torch.float32, 2.0 ** -16)
+    if weights:
+        got = w_out[0, :, :200].double().cpu().numpy()
+        before = w_in[0, :, :200].double().cpu().numpy()
+        before[:, 200 - tokens:] = 0
+        assert (np.abs(got - before - received[0]) <= 2.0 ** -13 * received[0] + 2.0 ** -22 * (before + received[0])).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 150])
+def test_rows_that_are_in_the_cache_already(cuda_device, tokens):
+    _, out, outs, _, spread, _ = _run(11, 2, 4, 2, 64, tokens, [tokens + 60, tokens], [tokens, tokens], 40, 4, torch.bfloat16, append=False)
+    _check(out, outs, spread, torch.bfloat16, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_scale_and_one_key_that_outweighs_all(cuda_device, tokens):
+    """A score 60 above the others anywhere in the cache, the first and last slots of pages among its places."""
+    from mesh_transformer.cache import cache_attention
+    length = 400
+    for place in (0, 3, 63, 64, 200, 319, length - tokens):
+        c = Cache(13, 1, 7, 2, 128, [length])
+        q = c.rows(1, tokens, 2, 128, torch.bfloat16)
+        q[:] = q[:, :1]
+        row = q[0, 0].float()
+        c.kpool[int(c.table[0, place // PAGE]), :, place % PAGE] = (row * 60.0 / row.square().sum(-1, keepdim=True) / 0.5).to(torch.bfloat16)
+        out = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=250, sinks=4, scale=0.5)
+        for t in {0, tokens // 2, tokens - 1}:
+            p = length - tokens + t
+            keys, values = (cache_oracle.slots_of(host(x), c.table[0], p + 1) for x in (c.kpool, c.vpool))
+            o, _ = cache_oracle.attention(host(q[0, t:t + 1]), keys, values, p + 1, 1, 250, 4, 0.5)
+            m, _ = cache_oracle.attention(host(q[0, t:t + 1]), keys, np.abs(values), p + 1, 1, 250, 4, 0.5)
+            # a score of 60 in 32 bits: 60 * 2^-18
+            assert (np.abs(host(out[0, t]) - o[0]) <= 2.0 ** -9 * np.abs(o[0]) + (2.0 ** -8 + 60 * 2.0 ** -18) * m[0]).all(), (place, t)
+
+
+def test_a_page_shared_by_two_sequences(cuda_device):
+    """A common beginning is stored once."""
+    from mesh_transformer.cache import cache_attention
+    c = Cache(17, 2, 3, 2, 64, [130, 130])
+    c.table[1, 0] = c.table[0, 0]
+    c.page_table = torch.from_numpy(c.table).to("cuda")
+    q = c.rows(2, 1, 4, 64, torch.bfloat16)
+    out = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=100, sinks=4)
+    outs, _, spread = _reference(c, q, [130, 130], [1, 1], 100, 4, 0.125)
+    _check(out, outs, spread, torch.bfloat16, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+def test_bad_lengths_and_pages_are_reported_and_left_alone(cuda_device, tokens):
+    """A length beyond the pages, one below the new tokens, a negative one, and page numbers outside the pool: status bit 1, zeros or the
+    other pages' result, and nothing written."""
+    from mesh_transformer.cache import cache_attention
+    c = Cache(19, 4, 3, 2, 64, [150, 150, 150, 150])
+    q, k, v = (c.rows(4, tokens, h, 64, torch.bfloat16) for h in (4, 2, 2))
+    lengths = torch.tensor([193, tokens - 1, -5, 150], dtype=torch.int32, device="cuda")
+    before = c.kpool.clone()
+    status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+    out = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, lengths, window=100, sinks=4, status=status)
+    assert int(status) == 2
+    assert float(out[:3].float().abs().sum()) == 0.0
+    outs, _, spread = _reference(c, q, [150] * 4, [tokens] * 4, 100, 4, 0.125)
+    _check(out[3:], outs[3:], spread[3:], torch.bfloat16, 2.0 ** -8)
+    # the new tokens' pages do not exist: nothing is stored
+    table = c.page_table.clone()
+    table[:, 1:] = torch.tensor([[-1], [8 * 12], [2 ** 31 - 1], [-2 ** 31]], dtype=torch.int32, device="cuda")
+    status.zero_()
+    short = torch.full((4,), 64 + tokens, dtype=torch.int32, device="cuda")
+    cache_attention(q, k, v, c.kpool, c.vpool, table, short, window=100, sinks=4, status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 2
+    assert torch.equal(c.kpool.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 200])
+def test_captured_and_replayed_on_another_stream(cuda_device, tokens):
+    """The call is captured once and replayed with other lengths, queries and page tables in the same tensors."""
+    from mesh_transformer.cache import cache_attention
+    c = Cache(23, 2, 6, 2, 128, [300, 210])
+    q, k, v = (c.rows(2, tokens, h, 128, torch.bfloat16) for h in (4, 2, 2))
+    weights = torch.zeros((2, 2, 384), device="cuda") if tokens < 10 else None
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache_attention(q, k, v, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=90, sinks=4, weights_out=weights)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache_attention(q, k, v, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=90, sinks=4, weights_out=weights)
+    for lengths in ([300, 210], [280, 201]):
+        q.copy_(c.rows(2, tokens, 4, 128, torch.bfloat16))
+        c.lengths_dev.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got, got_w = out.clone(), None if weights is None else weights.clone()
+        again = cache_attention(q, k, v, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=90, sinks=4, weights_out=weights)
+        torch.cuda.synchronize()
+        assert torch.equal(got, again)
+        if weights is not None:
+            assert torch.equal(got_w, weights)
+        outs, _, spread = _reference(c, q, lengths, [tokens] * 2, 90, 4, 128 ** -0.5)
+        _check(got, outs, spread, torch.bfloat16, 2.0 ** -8)
+
+
+def test_two_calls_at_once(cuda_device):
+    """Two streams at work on caches of their own give what each gives alone."""
+    from mesh_transformer.cache import cache_attention
+    sets = []
+    for seed in (29, 31):
+        c = Cache(seed, 8, 20, 4, 128, [1200 - 9 * i for i in range(8)])
+        sets.append((c, c.rows(8, 1, 16, 128, torch.bfloat16), torch.zeros((8, 4, 1280), device="cuda")))
+    call = lambda c, q, w: cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, weights_out=w)
+    alone = [(call(*s), s[2].clone()) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        outs = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                outs.append(call(*s))
+        torch.cuda.synchronize()
+        for (want, w), got, s in zip(alone, outs, sets):
+            assert torch.equal(want, got) and torch.equal(w, s[2])
+
+
+def test_same_bits_every_time(cuda_device):
+    from mesh_transformer.cache import cache_attention
+    for tokens in (1, 5, 300):
+        c = Cache(37, 3, 30, 2, 128, [1900, 900, 350])
+        q = c.rows(3, tokens, 16, 128, torch.bfloat16)
+        first = None
+        for _ in range(10):
+            w = torch.zeros((3, 2, 1920), device="cuda") if tokens < 10 else None
+            out = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=800, sinks=4, weights_out=w)
+            if first is None:
+                first = out, w
+            assert torch.equal(first[0], out) and (w is None or torch.equal(first[1], w))
+
+
+def test_output_of_the_callers_own_with_wide_rows(cuda_device):
+    from mesh_transformer.cache import cache_attention
+    for tokens in (1, 80):
+        c = Cache(41, 2, 4, 2, 64, [200, 100])
+        q = c.rows(2, tokens, 4, 64, torch.bfloat16)
+        wide = torch.full((2, tokens, 4 * 64 + 40), 5.0, dtype=torch.bfloat16, device="cuda")
+        out = wide[..., :256].unflatten(2, (4, 64))
+        assert cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=50, out=out) is not None
+        want = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=50)
+        assert torch.equal(wide[..., :256].reshape(want.shape), want) and (wide[..., 256:] == 5.0).all()
