@@ -3,8 +3,7 @@
 
 #include <string>
 
-#include "mtj_cache.cuh"
-#include "mtj_kernels.h"
+#include "mtj_cache_kernels.h"
 
 namespace mtj {
 namespace {
@@ -13,9 +12,7 @@ constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 
 __device__ __forceinline__ float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load_value(const float* p) { return *p; }
 __device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
 
 // The new tokens' keys and values into their slots: one block a token and sequence.
 template <typename T>
@@ -101,48 +98,6 @@ __global__ void __launch_bounds__(kRowThreads) cache_row_kernel(const mtj_cache_
   if (lse && threadIdx.x == 0) lse[row * a.heads + h] = make_float2(M, L);
 }
 
-// weights_out: one warp a slot and key head
-template <typename T, int DH>
-__global__ void __launch_bounds__(256) cache_weights_kernel(const mtj_cache_attn_args a, const float2* lse) {
-  constexpr int EPL = DH / 32;
-  const int lane = threadIdx.x & 31;
-  const size_t slots = static_cast<size_t>(a.pages) * kPageTokens;
-  const size_t unit = static_cast<size_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (unit >= slots * a.kv_heads * a.batch) return;
-  const int j = static_cast<int>(unit % slots), kvh = static_cast<int>(unit / slots % a.kv_heads), b = static_cast<int>(unit / slots / a.kv_heads);
-  const CacheSeq s = cache_seq(a.lengths_dev, a.new_tokens_dev, b, a.tokens, a.pages);
-  if (j >= s.length) return;
-  const int group = a.heads / a.kv_heads;
-  float sum = 0.f;
-  const int page = a.page_table_dev[static_cast<size_t>(b) * a.pages + j / kPageTokens];
-  if (cache_page_ok(page, a.n_pages)) {
-    float k[EPL];
-#pragma unroll
-    for (int e = 0; e < EPL; ++e)
-      k[e] = load_value(static_cast<const __nv_bfloat16*>(a.kpool_dev) +
-                        ((static_cast<size_t>(page) * a.kv_heads + kvh) * kPageTokens + j % kPageTokens) * DH + e * 32 + lane);
-    for (int t = 0; t < s.fresh; ++t) {
-      const int p = s.length - s.fresh + t;
-      if (j > p || (j >= a.sinks && p - j >= a.window)) continue;
-      for (int g = 0; g < group; ++g) {
-        const size_t row = static_cast<size_t>(b) * a.tokens + t;
-        float d = 0.f;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          d = fmaf(load_value(static_cast<const T*>(a.q_dev) + row * a.ld_q + (kvh * group + g) * DH + e * 32 + lane) * a.scale, k[e], d);
-        d = warp_sum(d);
-        const float2 ml = lse[row * a.heads + kvh * group + g];
-        sum += __expf(d - ml.x) / ml.y;
-      }
-    }
-  }
-  if (lane == 0) {
-    const size_t at = (static_cast<size_t>(b) * a.kv_heads + kvh) * slots + j;
-    const float before = a.weights_in_dev && j < s.length - s.fresh ? a.weights_in_dev[at] : 0.f;
-    a.weights_out_dev[at] = before + sum;
-  }
-}
-
 int32_t check_args(const mtj_cache_attn_args* a, std::string* err) {
   auto bad = [&](const char* what) {
     *err = what;
@@ -178,22 +133,19 @@ int32_t check_args(const mtj_cache_attn_args* a, std::string* err) {
   const int64_t most = 0x7fffffff, rows = static_cast<int64_t>(a->batch) * a->tokens;
   if (rows > most || rows * a->heads > most) return bad("batch * tokens * heads is too large");
   if (static_cast<int64_t>(a->batch) * a->kv_heads > most / kPageTokens / a->pages) return bad("batch * kv_heads * slots is too large");
+  if (static_cast<int64_t>(a->n_pages) * a->kv_heads > most / kPageTokens) return bad("n_pages * kv_heads is too large");
   return MTJ_OK;
 }
 
-int64_t lse_bytes(const mtj_cache_attn_args& a) {
-  return a.weights_out_dev ? static_cast<int64_t>(a.batch) * a.tokens * a.heads * sizeof(float2) : 0;
+// Few rows per key head, queries in 32 bits and calls that add up weights go tile by tile over the cache; other prompts row by row.
+bool takes_few(const mtj_cache_attn_args& a) {
+  return a.dtype == MTJ_F32 || a.weights_out_dev || a.tokens * static_cast<int64_t>(a.heads / a.kv_heads) <= 64;
 }
 
-template <typename T, int DH>
-cudaError_t run(const mtj_cache_attn_args& a, char* scratch, cudaStream_t s) {
-  float2* lse = a.weights_out_dev ? reinterpret_cast<float2*>(scratch) : nullptr;
-  if (a.k_new_dev) cache_append_kernel<T><<<a.batch * a.tokens, 256, 0, s>>>(a);
-  cache_row_kernel<T, DH><<<a.batch * a.tokens * a.heads, kRowThreads, 0, s>>>(a, lse);
-  if (lse) {
-    const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.pages * kPageTokens;
-    cache_weights_kernel<T, DH><<<static_cast<unsigned>((units + 7) / 8), 256, 0, s>>>(a, lse);
-  }
+template <int DH>
+cudaError_t run_prompt(const mtj_cache_attn_args& a, cudaStream_t s) {
+  if (a.k_new_dev) cache_append_kernel<__nv_bfloat16><<<a.batch * a.tokens, 256, 0, s>>>(a);
+  cache_row_kernel<__nv_bfloat16, DH><<<a.batch * a.tokens * a.heads, kRowThreads, 0, s>>>(a, nullptr);
   return cudaGetLastError();
 }
 
@@ -211,22 +163,23 @@ int64_t mtj_k_cache_attn_scratch_bytes(const mtj_cache_attn_args* a) {
     mtj_set_error(rc, err.c_str());
     return -1;
   }
-  return 256 + mtj::lse_bytes(*a);
+  return mtj::takes_few(*a) ? mtj::plan_cache_few(*a).total : 256;
 }
 
 int32_t mtj_k_cache_attn(const mtj_cache_attn_args* a, void* scratch, int64_t scratch_bytes, mtj_stream s) {
   std::string err;
   const int32_t rc = mtj::check_args(a, &err);
   if (rc) return mtj_set_error(rc, err.c_str());
-  if (!scratch || scratch_bytes < 256 + mtj::lse_bytes(*a) || (reinterpret_cast<uintptr_t>(scratch) & 255))
+  const bool few = mtj::takes_few(*a);
+  mtj::CacheFewPlan p = {};
+  if (few) p = mtj::plan_cache_few(*a);
+  else p.total = 256;
+  if (!scratch || scratch_bytes < p.total || (reinterpret_cast<uintptr_t>(scratch) & 255))
     return mtj_set_error(MTJ_ERR_INVALID, "scratch too small or not 256-byte aligned");
   const cudaStream_t st = static_cast<cudaStream_t>(s);
-  char* w = static_cast<char*>(scratch);
-  const bool f32 = a->dtype == MTJ_F32;
-  cudaError_t e;
-  if (a->d_head == 64) e = f32 ? mtj::run<float, 64>(*a, w, st) : mtj::run<__nv_bfloat16, 64>(*a, w, st);
-  else if (a->d_head == 128) e = f32 ? mtj::run<float, 128>(*a, w, st) : mtj::run<__nv_bfloat16, 128>(*a, w, st);
-  else e = f32 ? mtj::run<float, 256>(*a, w, st) : mtj::run<__nv_bfloat16, 256>(*a, w, st);
+  const cudaError_t e = few ? mtj::run_cache_few(*a, p, static_cast<char*>(scratch), st)
+                        : a->d_head == 64 ? mtj::run_prompt<64>(*a, st)
+                        : a->d_head == 128 ? mtj::run_prompt<128>(*a, st) : mtj::run_prompt<256>(*a, st);
   if (e != cudaSuccess) return mtj_set_error(MTJ_ERR_CUDA, cudaGetErrorString(e));
   return MTJ_OK;
 }

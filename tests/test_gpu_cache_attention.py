@@ -307,3 +307,30 @@ def test_output_of_the_callers_own_with_wide_rows(cuda_device):
         assert cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=50, out=out) is not None
         want = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=50)
         assert torch.equal(wide[..., :256].reshape(want.shape), want) and (wide[..., 256:] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,d_head,tokens", [(8, 8, 64, 1), (16, 4, 64, 5), (16, 4, 128, 1), (24, 4, 128, 4), (6, 6, 256, 1), (16, 2, 256, 2)])
+def test_many_long_sequences(cuda_device, heads, kv_heads, d_head, tokens, dtype):
+    """More tiles than blocks: a block works on parts of several sequences, and rings go round many times."""
+    from mesh_transformer.cache import cache_attention
+    lengths = [6000 - 331 * i for i in range(17)]
+    window, sinks, group = 4000, 4, heads // kv_heads
+    c = Cache(43, 17, 94, kv_heads, d_head, lengths)
+    q, k, v = (c.rows(17, tokens, h, d_head, dtype) for h in (heads, kv_heads, kv_heads))
+    w = torch.zeros((17, kv_heads, 94 * 64), device="cuda")
+    for _ in range(3):
+        out = cache_attention(q, k, v, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=window, sinks=sinks, weights_out=w)
+    for b, n in enumerate(lengths):
+        table = c.page_table[b].long()
+        keys, values = (x[table].transpose(0, 1).reshape(kv_heads, -1, d_head)[:, :n].double() for x in (c.kpool, c.vpool))
+        p = torch.arange(n - tokens, n, device="cuda")[:, None]
+        j = torch.arange(n, device="cuda")[None]
+        hidden = (j > p) | ((j >= sinks) & (p - j >= window))
+        qb = q[b].double().reshape(tokens, kv_heads, group, d_head).permute(1, 2, 0, 3)
+        share = torch.softmax((torch.einsum("hgtd,hjd->hgtj", qb, keys) * d_head ** -0.5).masked_fill(hidden, float("-inf")), -1)
+        want = torch.einsum("hgtj,hjd->thgd", share, values).reshape(tokens, heads, d_head)
+        spread = torch.einsum("hgtj,hjd->thgd", share, values.abs()).reshape(tokens, heads, d_head)
+        assert ((out[b].double() - want).abs() <= rounding(dtype) * want.abs() + 2.0 ** -13 * spread).all(), b
+        received = share.sum((1, 2))
+        assert ((w[b, :, :n].double() - received).abs() <= 2.0 ** -13 * received).all(), b
