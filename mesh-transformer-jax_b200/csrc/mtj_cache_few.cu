@@ -36,18 +36,23 @@ constexpr int kFewThreads = 32 * kWorkers + 32;
 constexpr uint32_t kTileBytes = 16384;               // keys and values
 constexpr int kJoinThreads = 256;
 constexpr float kGrowth = 8.f;                       // weights stay below 2^8
-constexpr int kWeightSlots = 2048;                   // slots of one key head that a block of the second kernel adds weights to
+constexpr int kWeightSlots = 1024;                   // slots of one key head that a block of the second kernel adds weights to
+
+// n tiles of rows that a warp takes: its accumulators are DH / 4 registers each
+constexpr int few_n_tiles(int dh, int nt) { return dh == 256 ? 1 : dh == 128 && nt > 2 ? 2 : nt; }
+// times 16 keys that a warp works on side by side
+constexpr int few_sub(int dh, int nt) { return dh == 256 || few_n_tiles(dh, nt) == 4 ? 1 : 2; }
 
 template <int DH, int NT, typename T>
 struct FewCfg {
   static constexpr int kKeys = 4096 / DH;            // of a tile: 16, 32, 64
-  // n tiles of rows that a warp takes (its accumulators are DH / 4 registers each), warps beside each other on the same keys
-  static constexpr int kNt = DH == 256 ? 1 : DH == 128 && NT > 2 ? 2 : NT, kRowWarps = NT / kNt;
-  static constexpr int kKeyWarps = kKeys / 16;
+  static constexpr int kNt = few_n_tiles(DH, NT), kRowWarps = NT / kNt;      // warps beside each other on the same keys
+  static constexpr int kSub = few_sub(DH, NT);
+  static constexpr int kKeyWarps = kKeys / (16 * kSub);
   static constexpr int kTeam = kKeyWarps * kRowWarps;      // warps that share a tile
   static constexpr int kTeams = kWorkers / kTeam;
   static constexpr int kParts = kWorkers / kRowWarps;      // warps with results for one row
-  static constexpr int kChains = kNt == 4 ? 1 : 2;         // of sums for a score
+  static constexpr int kChains = kSub * kNt >= 4 ? 1 : 2;  // of sums for a score
   static constexpr int kRows = 8 * NT;
   static constexpr int kQTerms = sizeof(T) == 2 ? 1 : 3, kPTerms = sizeof(T) == 2 ? 2 : 3;
   // 32-bit queries: the product adds 16 terms at a time, what it adds them to is rounded towards zero, so the sums over steps and
@@ -63,6 +68,7 @@ struct FewCfg {
   // parity that a team waits for is also that of the phase before the one another team still waits for
   static constexpr int kStages = static_cast<int>(kRoom / kTileBytes < 6 ? kRoom / kTileBytes : 6) / kTeams * kTeams;
   static constexpr uint32_t kSmem = 1024 + kStages * kTileBytes + kQBytes + kOBytes;
+  static_assert(kTeams * kTeam == kWorkers && kParts >= 2, "all warps work");
   static_assert(kStages >= 4 && kStages % kTeams == 0, "a ring");
 };
 
@@ -157,10 +163,18 @@ __device__ __forceinline__ int2 few_held(const CacheFewArgs& a, int b, bool repo
   return make_int2(s.length - s.fresh + min(s.fresh, a.t0) + fresh, fresh);
 }
 
+// Where units are few beside the blocks (aligned), no piece reaches over a unit's end: changing units costs a block about as much as
+// two rounds of tiles (16 units of 129 tiles: 16 against 10.5 us).  With the pieces this wide they are at most as many as the blocks.
+__device__ __forceinline__ int piece_width(const CacheFewArgs& a, int total, int units) {
+  const int w = max(a.least, (total + kPieces - units - 1) / (kPieces - units));
+  return (w + a.teams - 1) / a.teams * a.teams;
+}
+__device__ __forceinline__ int pieces_in(int tiles, int width) { return max(1, (tiles + width - 1) / width); }
+
 // The line of tiles: prefix[b] tiles lie before sequence b, its units one after the other.  Called by all threads of a block.
 static_assert(kFewBatch <= 2 * kFewThreads, "two sequences a thread");
 template <int KEYS>
-__device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* held, int* prefix, int* scan) {
+__device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* held, int* prefix, int* first, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = 2 * tid;
   int n0 = 0, n1 = 0;
   if (b < a.c.batch) {
@@ -179,13 +193,41 @@ __device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* 
   }
   if (lane == 31) scan[warp] = x;
   __syncthreads();
-  int before = x - n0 - n1;
-  for (int w = 0; w < warp; ++w) before += scan[w];
+  int before = x - n0 - n1, total = 0;
+  for (int w = 0; w < kFewThreads / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
   if (b <= a.c.batch) prefix[b] = before;
   if (b + 1 <= a.c.batch) prefix[b + 1] = before + n0;
-  if (blockIdx.x == 0) {                   // for the second kernel
-    if (b <= a.c.batch) a.prefix[b] = before;
-    if (b + 1 <= a.c.batch) a.prefix[b + 1] = before + n0;
+  int* second = a.prefix;                  // for the second kernel
+  if (blockIdx.x == 0) {
+    if (b <= a.c.batch) second[b] = before;
+    if (b + 1 <= a.c.batch) second[b + 1] = before + n0;
+  }
+  if (a.aligned) {
+    // pieces of sequence b: first[b] before it, its units' after one another
+    const int width = piece_width(a, total, a.c.batch * units);
+    n0 = b < a.c.batch ? pieces_in(n0 / units, width) * units : 0;
+    n1 = b + 1 < a.c.batch ? pieces_in(n1 / units, width) * units : 0;
+    x = n0 + n1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    before = x - n0 - n1;
+    for (int w = 0; w < warp; ++w) before += scan[w];
+    if (b <= a.c.batch) first[b] = before;
+    if (b + 1 <= a.c.batch) first[b + 1] = before + n0;
+    if (blockIdx.x == 0) {
+      second += kFewBatch + 1;
+      if (b <= a.c.batch) second[b] = before;
+      if (b + 1 <= a.c.batch) second[b + 1] = before + n0;
+    }
   }
   __syncthreads();
 }
@@ -215,7 +257,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
   __shared__ int tile_slot[kStages];                 // first slot of the tile in this stage, -1: its page does not exist
   __shared__ int tile_page[kStages];
   __shared__ int scan[kFewThreads / 32];
-  __shared__ int prefix[kFewBatch + 1];
+  __shared__ int prefix[kFewBatch + 1], first_piece[kFewBatch + 1];
   __shared__ int2 held[kFewBatch];
   __shared__ float sm_m[C::kParts][kRows], sm_l[C::kParts][kRows];
   const uint32_t raw = smem_u32(few_raw), ring = (raw + 1023) & ~1023u;
@@ -237,11 +279,32 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
     mbar_fence_init();
   }
   pdl_launch_dependents();                           // the second kernel waits for this one's end
-  lay_out<kKeys>(a, units, held, prefix, scan);
+  lay_out<kKeys>(a, units, held, prefix, first_piece, scan);
   const int64_t total = prefix[a.c.batch];
-  const int pieces = pieces_of(total, gridDim.x);
-  if (static_cast<int>(blockIdx.x) >= pieces) return;
-  const int begin = piece_begin(total, pieces, blockIdx.x), end = piece_begin(total, pieces, blockIdx.x + 1);
+  int begin, end;
+  if (a.aligned) {
+    if (static_cast<int>(blockIdx.x) >= first_piece[a.c.batch]) return;
+    const int b = sequence_of(first_piece, a.c.batch, blockIdx.x);
+    const FewSeq s = few_seq<kKeys>(a, held[b]);
+    const int n = (first_piece[b + 1] - first_piece[b]) / units, rest = blockIdx.x - first_piece[b], unit = rest / n, k = rest - unit * n;
+    begin = prefix[b] + unit * s.tiles + s.tiles * k / n;
+    end = prefix[b] + unit * s.tiles + s.tiles * (k + 1) / n;
+    if (s.tiles == 0) {                              // rows that see nothing
+      const int kvh = unit / row_tiles, row0 = unit % row_tiles * kRows;
+      const float zero[8] = {};
+      for (int i = tid; i < min(kRows, rows - row0) * (DH / 8); i += kFewThreads) {
+        const int r = row0 + i / (DH / 8), t = r / group;
+        store8(static_cast<T*>(a.c.out_dev) + (static_cast<size_t>(b) * a.c.tokens + a.t0 + t) * a.c.ld_out +
+                   (kvh * group + r - t * group) * DH + i % (DH / 8) * 8, zero, 0.f);
+      }
+      return;
+    }
+  } else {
+    const int pieces = pieces_of(total, gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= pieces) return;
+    begin = piece_begin(total, pieces, blockIdx.x);
+    end = piece_begin(total, pieces, blockIdx.x + 1);
+  }
 
   if (warp == kWorkers) {
     // ---- producer ----
@@ -298,12 +361,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
   }
 
   // ---- workers ----
-  const int team = warp / C::kTeam, key0 = (warp % C::kKeyWarps) * 16;   // this warp's 16 keys of its team's tiles
+  const int team = warp / C::kTeam, key0 = (warp % C::kKeyWarps) * (16 * C::kSub);   // this warp's keys of its team's tiles
   const int nt0 = C::kRowWarps == 1 ? 0 : warp / C::kKeyWarps % C::kRowWarps * C::kNt;     // and its rows' first n tile
   const int part_id = team * C::kKeyWarps + warp % C::kKeyWarps;
   const int g = lane >> 2, c = lane & 3;                                 // fragment coordinates
   constexpr int kNt = C::kNt;
-  constexpr int kBlock = kNt == 1 ? 4 : 2;           // steps whose products are issued side by side
+  constexpr int kSub = C::kSub;
+  constexpr int kBlock = kNt * kSub == 1 ? 4 : 2;    // steps whose products are issued side by side
   constexpr bool kQInRegisters = C::kQTerms * kNt * kSteps <= 16;
   uint2 qr[kQInRegisters ? C::kQTerms * kNt * kSteps : 1];
   bool arrived = true;
@@ -386,10 +450,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
       if (tile_slot[st] >= 0) {
         const uint32_t sk = ring + st * kTileBytes, sv = sk + kTileBytes / 2;
         // slots of new tokens and slots behind the sequence
-        if (slot0 + 16 > first) {
+        if (slot0 + 16 * kSub > first) {
           unsigned char* pk = ring_ptr + st * kTileBytes;
           const size_t page = static_cast<size_t>(tile_page[st]) * a.c.kv_heads + kvh;
-          for (int v = lane; v < 16 * (DH / 8); v += 32) {
+          for (int v = lane; v < 16 * kSub * (DH / 8); v += 32) {
             const int r = v / (DH / 8), piece = v % (DH / 8), j = slot0 + r, t = j - first;
             const uint32_t at = piece_at<kKeys>(key0 + r, piece);
             if (j >= s.length) {
@@ -412,24 +476,30 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
           __syncwarp();
         }
         // S^T
-        float sc[C::kChains][kNt][4];
+        float sc[C::kChains][kSub][kNt][4];
 #pragma unroll
-        for (int nt = 0; nt < kNt; ++nt)
+        for (int ch = 0; ch < C::kChains; ++ch)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[0][nt][e] = sc[C::kChains - 1][nt][e] = 0.f;
-        const int krow = key0 + (lane & 15);
-#pragma unroll
-        for (int k0 = 0; k0 < kSteps; k0 += kBlock) {
-          uint32_t ka[kBlock][4];
-          float part[kBlock][kNt][4];
-#pragma unroll
-          for (int u = 0; u < kBlock; ++u) {
-            ldsm4(ka[u], sk + piece_at<kKeys>(krow, (k0 + u) * 2 + (lane >> 4)));
+          for (int sb = 0; sb < kSub; ++sb)
 #pragma unroll
             for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) part[u][nt][e] = 0.f;
-          }
+              for (int e = 0; e < 4; ++e) sc[ch][sb][nt][e] = 0.f;
+        const int krow = key0 + (lane & 15);
+#pragma unroll
+        for (int k0 = 0; k0 < kSteps; k0 += kBlock) {
+          uint32_t ka[kBlock][kSub][4];
+          float part[kBlock][kSub][kNt][4];
+#pragma unroll
+          for (int u = 0; u < kBlock; ++u)
+#pragma unroll
+            for (int sb = 0; sb < kSub; ++sb) {
+              ldsm4(ka[u][sb], sk + piece_at<kKeys>(krow + 16 * sb, (k0 + u) * 2 + (lane >> 4)));
+#pragma unroll
+              for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[u][sb][nt][e] = 0.f;
+            }
 #pragma unroll
           for (int q = 0; q < C::kQTerms; ++q) {
             const int term = C::kQTerms - 1 - q;                         // smallest first
@@ -440,47 +510,56 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
                 uint2 bq;
                 if constexpr (kQInRegisters) bq = qr[(term * kNt + nt) * kSteps + k0 + u];
                 else bq = q_frag[((term * NT + nt0 + nt) * kSteps + k0 + u) * 32 + lane];
-                mma16(C::kExactSums ? part[u][nt] : sc[u % C::kChains][nt], ka[u], bq.x, bq.y);
+#pragma unroll
+                for (int sb = 0; sb < kSub; ++sb)
+                  mma16(C::kExactSums ? part[u][sb][nt] : sc[u % C::kChains][sb][nt], ka[u][sb], bq.x, bq.y);
               }
           }
           if constexpr (C::kExactSums) {
 #pragma unroll
             for (int u = 0; u < kBlock; ++u)
 #pragma unroll
-              for (int nt = 0; nt < kNt; ++nt)
+              for (int sb = 0; sb < kSub; ++sb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[u % C::kChains][nt][e] += part[u][nt][e];
+                for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) sc[u % C::kChains][sb][nt][e] += part[u][sb][nt][e];
           }
         }
         // weights
-        const int last = slot0 + 15;
+        const int last = slot0 + 16 * kSub - 1;
         const bool whole = last <= first && (last < a.c.sinks || s.length - 1 - slot0 < a.c.window);     // every row sees every key
-        float v[kNt][4];
+        float v[kSub][kNt][4];
         bool grow = false;
 #pragma unroll
-        for (int nt = 0; nt < kNt; ++nt) {
+        for (int sb = 0; sb < kSub; ++sb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[nt][e] = (C::kChains == 1 ? sc[0][nt][e] : sc[0][nt][e] + sc[C::kChains - 1][nt][e]) * a.scale_log2;
-            const int j = slot0 + g + (e >> 1) * 8, p = place[nt][e & 1];
-            if (whole ? p < 0 : (j > p || (j >= a.c.sinks && p - j >= a.c.window))) v[nt][e] = -INFINITY;
-            grow |= v[nt][e] > m[nt][e & 1] + kGrowth;
-          }
-          if (a.scores) {
-            // [tile of the line][key][row]
-            const size_t at = (static_cast<size_t>(x + i) * kKeys + key0 + g) * a.score_rows;
-            const int r = (nt0 + nt) * 8 + 2 * c;
-            if (a.score_rows == 1) {
-              if (r == 0) {
-                a.scores[at] = v[nt][0];
-                a.scores[at + 8] = v[nt][2];
+          for (int nt = 0; nt < kNt; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float y = sc[0][sb][nt][e];
+              if (C::kChains == 2) y += sc[C::kChains - 1][sb][nt][e];
+              y *= a.scale_log2;
+              const int j = slot0 + sb * 16 + g + (e >> 1) * 8, p = place[nt][e & 1];
+              if (whole ? p < 0 : (j > p || (j >= a.c.sinks && p - j >= a.c.window))) y = -INFINITY;
+              grow |= y > m[nt][e & 1] + kGrowth;
+              v[sb][nt][e] = y;
+            }
+            if (a.scores) {
+              // [tile of the line][key][row]
+              const size_t at = (static_cast<size_t>(x + i) * kKeys + key0 + sb * 16 + g) * a.score_rows;
+              const int r = (nt0 + nt) * 8 + 2 * c;
+              if (a.score_rows == 1) {
+                if (r == 0) {
+                  a.scores[at] = v[sb][nt][0];
+                  a.scores[at + 8] = v[sb][nt][2];
+                }
+              } else if (r < a.score_rows) {
+                *reinterpret_cast<float2*>(a.scores + at + r) = make_float2(v[sb][nt][0], v[sb][nt][1]);
+                *reinterpret_cast<float2*>(a.scores + at + 8 * a.score_rows + r) = make_float2(v[sb][nt][2], v[sb][nt][3]);
               }
-            } else if (r < a.score_rows) {
-              *reinterpret_cast<float2*>(a.scores + at + r) = make_float2(v[nt][0], v[nt][1]);
-              *reinterpret_cast<float2*>(a.scores + at + 8 * a.score_rows + r) = make_float2(v[nt][2], v[nt][3]);
             }
           }
-        }
         // the maxima that weights refer to move when a score exceeds one by more than kGrowth
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -488,10 +567,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
             float corr[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(v[nt][e], v[nt][e + 2]);
+              float top = m[nt][e];
+#pragma unroll
+              for (int sb = 0; sb < kSub; ++sb) top = fmaxf(top, fmaxf(v[sb][nt][e], v[sb][nt][e + 2]));
 #pragma unroll
               for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
-              top = fmaxf(top, m[nt][e]);
               corr[e] = m[nt][e] == top ? 1.f : exp2_fast(m[nt][e] - top);
               m[nt][e] = top;
               l[nt][e] *= corr[e];
@@ -502,52 +582,59 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
               for (int e = 0; e < 4; ++e) o[d][nt][e] *= corr[e & 1];
           }
         }
-        uint32_t pb[C::kPTerms][kNt][2];
+        uint32_t pb[C::kPTerms][kSub][kNt][2];
 #pragma unroll
-        for (int nt = 0; nt < kNt; ++nt) {
+        for (int sb = 0; sb < kSub; ++sb)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-            v[nt][e] = exp2_fast(v[nt][e] - base);
-            v[nt][e + 2] = exp2_fast(v[nt][e + 2] - base);
-            l[nt][e] += v[nt][e] + v[nt][e + 2];
+          for (int nt = 0; nt < kNt; ++nt) {
+            float* y = v[sb][nt];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+              y[e] = exp2_fast(y[e] - base);
+              y[e + 2] = exp2_fast(y[e + 2] - base);
+              l[nt][e] += y[e] + y[e + 2];
+            }
+            uint32_t lo[C::kPTerms], hi[C::kPTerms];
+            split2<C::kPTerms>(y[0], y[1], lo);
+            split2<C::kPTerms>(y[2], y[3], hi);
+#pragma unroll
+            for (int p = 0; p < C::kPTerms; ++p) {
+              pb[p][sb][nt][0] = transposed(lo[p]);
+              pb[p][sb][nt][1] = transposed(hi[p]);
+            }
           }
-          uint32_t lo[C::kPTerms], hi[C::kPTerms];
-          split2<C::kPTerms>(v[nt][0], v[nt][1], lo);
-          split2<C::kPTerms>(v[nt][2], v[nt][3], hi);
-#pragma unroll
-          for (int p = 0; p < C::kPTerms; ++p) {
-            pb[p][nt][0] = transposed(lo[p]);
-            pb[p][nt][1] = transposed(hi[p]);
-          }
-        }
         // O^T
         const int vrow = key0 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
         for (int d0 = 0; d0 < kSteps; d0 += kBlock) {
-          uint32_t va[kBlock][4];
-          float part[kBlock][kNt][4];
 #pragma unroll
-          for (int u = 0; u < kBlock; ++u) {
-            ldsm4_trans(va[u], sv + piece_at<kKeys>(vrow, (d0 + u) * 2 + ((lane >> 3) & 1)));
+          for (int sb = 0; sb < kSub; ++sb) {
+            uint32_t va[kBlock][4];
+            float part[kBlock][kNt][4];
 #pragma unroll
-            for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) part[u][nt][e] = 0.f;
-          }
-#pragma unroll
-          for (int p = C::kPTerms - 1; p >= 0; --p)
-#pragma unroll
-            for (int u = 0; u < kBlock; ++u)
-#pragma unroll
-              for (int nt = 0; nt < kNt; ++nt) mma16(C::kExactSums ? part[u][nt] : o[d0 + u][nt], va[u], pb[p][nt][0], pb[p][nt][1]);
-          if constexpr (C::kExactSums) {
-#pragma unroll
-            for (int u = 0; u < kBlock; ++u)
+            for (int u = 0; u < kBlock; ++u) {
+              ldsm4_trans(va[u], sv + piece_at<kKeys>(vrow + 16 * sb, (d0 + u) * 2 + ((lane >> 3) & 1)));
 #pragma unroll
               for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[d0 + u][nt][e] += part[u][nt][e];
+                for (int e = 0; e < 4; ++e) part[u][nt][e] = 0.f;
+            }
+#pragma unroll
+            for (int p = C::kPTerms - 1; p >= 0; --p)
+#pragma unroll
+              for (int u = 0; u < kBlock; ++u)
+#pragma unroll
+                for (int nt = 0; nt < kNt; ++nt)
+                  mma16(C::kExactSums ? part[u][nt] : o[d0 + u][nt], va[u], pb[p][sb][nt][0], pb[p][sb][nt][1]);
+            if constexpr (C::kExactSums) {
+#pragma unroll
+              for (int u = 0; u < kBlock; ++u)
+#pragma unroll
+                for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[d0 + u][nt][e] += part[u][nt][e];
+            }
           }
         }
       }
@@ -636,7 +723,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
 // Second kernel: blocks [0, join_blocks) one a (sequence, unit, row) join the parts of units that several blocks worked on, and
 // write the zeros of rows that nobody worked on; the others add the attention weights of kWeightSlots slots of one key head.
 template <int DH, typename T>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const CacheFewArgs a, int tile_rows, int most, int join_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const CacheFewArgs a, int tile_rows, int most, int join_blocks) {
   constexpr int kKeys = 4096 / DH;
   constexpr int kLanes = DH / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 sm_o[kGroups][kLanes];
@@ -653,7 +740,18 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const CacheFew
   pdl_wait();
   pdl_launch_dependents();
   const int64_t total = a.prefix[a.c.batch];
-  const int begin = a.prefix[b], pieces = pieces_of(total, most);
+  const int begin = a.prefix[b], pieces = a.aligned ? a.prefix[kFewBatch + 1 + b] : pieces_of(total, most);
+  const int each = a.aligned ? (a.prefix[kFewBatch + 1 + b + 1] - pieces) / units : 0;
+  // the blocks that worked on a unit: the first one and how many
+  auto blocks_of = [&](int unit, int* n) {
+    if (a.aligned) {
+      *n = each;
+      return pieces + unit * each;
+    }
+    const int u0 = begin + unit * s.tiles, fb = piece_of(total, pieces, u0);
+    *n = piece_of(total, pieces, u0 + s.tiles - 1) - fb + 1;
+    return fb;
+  };
 
   // part k of the unit that lies at [u0, u1) in the line: the end of the first block's piece, then the beginnings of the next ones'
   if (joins) {
@@ -665,8 +763,8 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const CacheFew
       return;
     }
     const int unit = kvh * row_tiles + row / tile_rows, r = row % tile_rows;
-    const int u0 = begin + unit * s.tiles, u1 = u0 + s.tiles;
-    const int fb = piece_of(total, pieces, u0), lb = piece_of(total, pieces, u1 - 1), n = lb - fb + 1;
+    int n;
+    const int fb = blocks_of(unit, &n);
     if (n == 1) return;                                                  // one block had it all
     auto part_of = [&](int k) { return (static_cast<size_t>(fb + k) * 2 + (k == 0 ? 1 : 0)) * tile_rows + r; };
     float top = -INFINITY;
@@ -735,7 +833,8 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const CacheFew
     for (int rt = 0; rt < row_tiles; ++rt) {
       const int unit = kvh * row_tiles + rt;
       const int u0 = begin + unit * s.tiles;
-      const int fb = piece_of(total, pieces, u0), n = piece_of(total, pieces, u0 + s.tiles - 1) - fb + 1;
+      int n;
+      const int fb = blocks_of(unit, &n);
       __syncthreads();
       for (int r = warp; r < tile_rows; r += kJoinThreads / 32) {
         float top = -INFINITY, l = 0.f;
@@ -812,9 +911,10 @@ cudaError_t launch(const CacheFewArgs& a, const CUtensorMap& mk, const CUtensorM
   e = launch_pdl(cache_few_kernel<DH, NT, T>, dim3(pieces), dim3(kFewThreads), C::kSmem, s, false, mk, mv, a);
   if (e != cudaSuccess) return e;
   const int rows = a.tokens * (a.c.heads / a.c.kv_heads);
-  const int join = a.c.batch * a.c.kv_heads * rows;
+  const int join = a.whole ? 0 : a.c.batch * a.c.kv_heads * rows;
   const int slots = a.c.pages * kPageTokens;
   const int weigh = a.c.weights_out_dev ? a.c.batch * a.c.kv_heads * ((slots + kWeightSlots - 1) / kWeightSlots) : 0;
+  if (join + weigh == 0) return cudaSuccess;
   return launch_pdl(cache_join_kernel<DH, T>, dim3(join + weigh), dim3(kJoinThreads), 0, s, true, a, C::kRows, pieces, join);
 }
 
@@ -843,14 +943,21 @@ CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c) {
   p.batch = std::min(c.batch, kFewBatch);
   const int64_t units = static_cast<int64_t>(p.batch) * c.kv_heads * ((rows + p.tile_rows - 1) / p.tile_rows);
   const int64_t tiles = units * most_tiles(c, p.tokens);
-  p.pieces = static_cast<int>(std::min<int64_t>(kPieces, tiles));
+  p.aligned = units <= kPieces / 2;
+  const int nt = p.tile_rows / 8;
+  p.teams = kWorkers / (4096 / c.d_head / (16 * few_sub(c.d_head, nt)) * (nt / few_n_tiles(c.d_head, nt)));      // as FewCfg has them
+  // up to four rounds of tiles the second kernel costs more than it gives
+  p.whole = p.aligned && most_tiles(c, p.tokens) <= 4 * p.teams;
+  p.least = p.whole ? 4 * p.teams : p.teams;
+  p.pieces = static_cast<int>(p.aligned ? std::min<int64_t>(kPieces, units * ((most_tiles(c, p.tokens) + p.least - 1) / p.least))
+                                        : std::min<int64_t>(kPieces, tiles));
   p.score_rows = rows == 1 ? 1 : std::min(p.tile_rows, (rows + 1) / 2 * 2);
   auto take = [&](int64_t bytes) {
     const int64_t at = p.total;
     p.total += (bytes + 255) / 256 * 256;
     return at;
   };
-  p.prefix_off = take((kFewBatch + 1) * 4);
+  p.prefix_off = take(2 * (kFewBatch + 1) * 4);
   p.ml_off = take(static_cast<int64_t>(p.pieces) * 2 * p.tile_rows * 8);
   p.o_off = take(static_cast<int64_t>(p.pieces) * 2 * p.tile_rows * c.d_head * 4);
   p.lse_off = take(c.weights_out_dev ? units * p.tile_rows * 8 : 0);
@@ -896,6 +1003,10 @@ cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, c
       }
       a.scale_log2 = c.scale * 1.4426950408889634f;
       a.score_rows = p.score_rows;
+      a.aligned = p.aligned;
+      a.whole = p.whole;
+      a.least = p.least;
+      a.teams = p.teams;
       a.prefix = reinterpret_cast<int32_t*>(scratch + p.prefix_off);
       a.part_ml = reinterpret_cast<float2*>(scratch + p.ml_off);
       a.part_o = reinterpret_cast<float*>(scratch + p.o_off);

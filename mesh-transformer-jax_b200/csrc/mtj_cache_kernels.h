@@ -12,14 +12,16 @@ struct CacheFewArgs {
   int t0, tokens;                          // the launch's tokens of the call's
   float scale_log2;                        // score scale times log2(e)
   int score_rows;                          // rows of a key's scores
-  int32_t* prefix;                         // [batch + 1] tiles before each sequence
+  int aligned, whole;                      // pieces end where units do; every unit is one piece
+  int least, teams;                        // tiles of a piece at least, and the multiple that it is of
+  int32_t* prefix;                         // [2][kFewBatch + 1] tiles, and pieces, before each sequence
   float2* part_ml;                         // [pieces][2][tile rows]: maximum (base 2), sum
   float* part_o;                           // [pieces][2][tile rows][d_head]
   float2* lse;                             // [units][tile rows] of units that one block had, with weights
   float* scores;                           // [tiles][keys][score_rows] (base 2), with weights
 };
 struct CacheFewPlan {
-  int tokens, batch, tile_rows, pieces, score_rows;
+  int tokens, batch, tile_rows, pieces, score_rows, aligned, whole, least, teams;
   int64_t line, prefix_off, ml_off, o_off, lse_off, scores_off, total;
 };
 CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c);
