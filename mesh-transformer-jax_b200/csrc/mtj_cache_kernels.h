@@ -1,4 +1,4 @@
-// Launchers behind mtj_k_cache_attn: few new tokens (mtj_cache_few.cu) and prompts.
+// Launchers behind mtj_k_cache_attn: few new tokens (mtj_cache_few.cu) and prompts (mtj_cache_prompt.cu).
 #pragma once
 #include "mtj_cache.cuh"
 #include "mtj_kernels.h"
@@ -26,6 +26,8 @@ struct CacheFewPlan {
 };
 CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c);
 cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, char* scratch, cudaStream_t s);
+// Prompts, bf16 without weights (mtj_cache_prompt.cu); no scratch.
+cudaError_t run_cache_prompt(const mtj_cache_attn_args& a, cudaStream_t s);
 
 // eight numbers of a row as bf16, rounded where they are not
 __device__ __forceinline__ uint4 load8_bf16(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
