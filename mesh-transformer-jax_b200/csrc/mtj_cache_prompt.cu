@@ -28,6 +28,8 @@ constexpr int kKeysB = 128;                // keys of a block: two pages
 constexpr int kSoftThreads = 256;
 constexpr int kPromptThreads = kSoftThreads + 64;      // and the warps of TMA and of the products
 constexpr int kBlockNotes = 8;
+constexpr int kPolyOf = 4;                 // of this many pairs of weights one is worked out on the multiply-add units
+constexpr float kExp0 = 0.99992806f, kExp1 = 0.69326097f, kExp2 = 0.24261114f, kExp3 = 0.05517167f;
 
 template <int DH>
 struct PromptCfg {
@@ -54,24 +56,35 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit_to(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The warp of the products runs as one, with the same values in all lanes, and one lane issues: descriptors then come from uniform
+// registers.  (In a branch of one lane, every product cost 90 cycles of moves: 720 for the eight of P V whatever their size.)
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x;
+}
+__device__ __forceinline__ void commit_to(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(bar), "r"(leader)
+      : "memory");
 }
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
 // shared-memory matrix descriptor, 128-byte swizzle; lbo / sbo in bytes
@@ -83,6 +96,72 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two numbers in a register pair
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpair(uint64_t d, float* lo, float* hi) {
+  uint32_t x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(d));
+  *lo = __uint_as_float(x);
+  *hi = __uint_as_float(y);
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of a pair on the multiply-add units, for x in [-126, 9]: x = n + f with |f| <= 1/2 by adding and taking away 1.5 * 2^23, a
+// polynomial of degree 3 in f (fitted to the relative error, 8e-5 at most: a twentieth of the rounding to bf16 that follows),
+// n added to its exponent
+__device__ __forceinline__ void exp2_pair(uint64_t x, float* y0, float* y1) {
+  const uint64_t magic = pair_of(12582912.f, 12582912.f);
+  const uint64_t n = add_pair(x, magic);
+  const uint64_t f = add_pair(x, fma_pair(n, pair_of(-1.f, -1.f), magic));
+  uint64_t p = fma_pair(pair_of(kExp3, kExp3), f, pair_of(kExp2, kExp2));
+  p = fma_pair(p, f, pair_of(kExp1, kExp1));
+  p = fma_pair(p, f, pair_of(kExp0, kExp0));
+  float p0, p1, n0, n1;
+  unpair(p, &p0, &p1);
+  unpair(n, &n0, &n1);
+  *y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  *y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
+// bits 0 .. n - 1
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// 32 columns of this warp's lanes, on their way until tmem_wait()
+__device__ __forceinline__ void tmem_fetch32(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// nothing that uses r comes before this place
+__device__ __forceinline__ void pin32(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* r) {
   asm volatile(
@@ -252,49 +331,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     }
   } else if (warp == 9) {
     // ---- products ----
-    if (lane == 0 && nb > 0) {
+    if (nb > 0) {
+      const uint32_t leader = elected();
+      auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
       constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kRowsT >> 4) << 24);
       constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kRowsT >> 4) << 24);
       auto issue_s = [&](int u) {
         const int j = u / kTiles, t = u % kTiles, st = j % C::kKSlots;
-        if (t == 0 && !mbar_wait(k_full + 8 * st, (j / C::kKSlots) & 1)) return false;
+        if (t == 0 && !wait(k_full + 8 * st, (j / C::kKSlots) & 1)) return false;
         fence_after();
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
           const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
           const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (kKeysB * 128), 16, 1024);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ss(tmem + C::kColS + (u & 1) * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) mma_ss(tmem + C::kColS + (u & 1) * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
         }
-        commit_to(s_full + 8 * (u & 1));
-        if (t == kTiles - 1) commit_to(k_empty + 8 * st);
+        commit_to(s_full + 8 * (u & 1), leader);
+        if (t == kTiles - 1) commit_to(k_empty + 8 * st, leader);
         return true;
       };
       auto issue_pv = [&](int u) {
         const int j = u / kTiles, t = u % kTiles;
-        if (!mbar_wait(p_full + 8 * (u & 1), (u >> 1) & 1)) return false;
+        if (!wait(p_full + 8 * (u & 1), (u >> 1) & 1)) return false;
 #pragma unroll
         for (int i = 0; i < 2 / C::kVPages; ++i) {
           const int n = j * (2 / C::kVPages) + i, st = n % C::kVSlots;
-          if (t == 0 && !mbar_wait(v_full + 8 * st, (n / C::kVSlots) & 1)) return false;
+          if (t == 0 && !wait(v_full + 8 * st, (n / C::kVSlots) & 1)) return false;
           fence_after();
           const uint64_t vd = smem_desc(sV + st * C::kVBytes, C::kVPages * kPageTokens * 128, 1024);
           const uint32_t pa = tmem + C::kColS + (u & 1) * kKeysB + i * (kPageTokens / 2);
 #pragma unroll
           for (int k = 0; k < C::kVPages * 4; ++k)
-            mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | i | k) ? 1u : 0u);
-          if (t == kTiles - 1) commit_to(v_empty + 8 * st);
+            mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | i | k) ? 1u : 0u, leader);
+          if (t == kTiles - 1) commit_to(v_empty + 8 * st, leader);
         }
-        commit_to(o_done + 8 * (u & 1));
+        commit_to(o_done + 8 * (u & 1), leader);
         return true;
       };
-      bool ok = mbar_wait(q_full, 0) && issue_s(0);
+      bool ok = wait(q_full, 0) && issue_s(0);
       if (ok && units > 1) ok = issue_s(1);
       for (int u = 0; ok && u < units; ++u) {
         ok = issue_pv(u);
         if (ok && u + 2 < units) ok = issue_s(u + 2);
       }
-      if (!ok) atomicOr(&failed, 1u);
+      if (!ok && leader) atomicOr(&failed, 1u);
     }
   } else {
     // ---- weights ----
@@ -317,7 +398,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
       uint32_t x[kKeysThread];
 #pragma unroll
-      for (int i = 0; i < kKeysThread; i += 32) tmem_load32(at_s + i, x + i);
+      for (int i = 0; i < kKeysThread; i += 32) tmem_fetch32(at_s + i, x + i);
+      tmem_wait();
+#pragma unroll
+      for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
       // V's rows that hold nothing: zeroed before anybody's weights are announced
       if (note != (kPageTokens | kPageTokens << 8)) {
 #pragma unroll
@@ -339,24 +423,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       const bool whole = note == (kPageTokens | kPageTokens << 8) && key + kKeysThread - 1 <= warp_first &&
                          (key + kKeysThread - 1 < a.sinks || warp_last - key < a.window) && warp_last >= warp_first;
       if (!whole) {
+        // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
         const int hi = p - key, lo = p - a.window + 1 - key, sk = a.sinks - key;
-        const int v0 = note & 255, v1 = note >> 8;
 #pragma unroll
-        for (int i = 0; i < kKeysThread; ++i) {
-          const int within = part * kKeysThread + i;
-          const bool there = within < kPageTokens ? within < v0 : within - kPageTokens < v1;
-          if (!(there && i <= hi && (i >= lo || i < sk))) x[i] = 0xff800000u;
+        for (int w = 0; w < kKeysThread / 32; ++w) {
+          const int within = part * kKeysThread + 32 * w;
+          const int held = (within < kPageTokens ? note & 255 : note >> 8) - within % kPageTokens;
+          const uint32_t see = low_bits(min(hi + 1, held + 32 * w) - 32 * w) & (~low_bits(lo - 32 * w) | low_bits(sk - 32 * w));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(see >> i & 1u)) x[32 * w + i] = 0xff800000u;
         }
       }
-      float top0 = -INFINITY, top1 = -INFINITY, top2 = -INFINITY, top3 = -INFINITY;
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kKeysThread; i += 4) {
-        top0 = fmaxf(top0, __uint_as_float(x[i]));
-        top1 = fmaxf(top1, __uint_as_float(x[i + 1]));
-        top2 = fmaxf(top2, __uint_as_float(x[i + 2]));
-        top3 = fmaxf(top3, __uint_as_float(x[i + 3]));
-      }
-      float top = fmaxf(fmaxf(top0, top1), fmaxf(top2, top3)) * scale_log2;      // scale > 0
+      for (int i = 0; i < kKeysThread; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale_log2;      // scale > 0
       if constexpr (kTiles == 1) {
         part_max[part][r] = top;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
@@ -367,15 +451,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top;
       const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
       const float neg = m_new == -INFINITY ? 0.f : -m_new;
-      float sum0 = 0.f, sum1 = 0.f;
+      const uint64_t scale2 = pair_of(scale_log2, scale_log2), neg2 = pair_of(neg, neg);
+      uint64_t sums[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < kKeysThread; i += 2) {
-        const float y0 = exp2_ftz(fmaf(__uint_as_float(x[i]), scale_log2, neg));
-        const float y1 = exp2_ftz(fmaf(__uint_as_float(x[i + 1]), scale_log2, neg));
-        sum0 += y0;
-        sum1 += y1;
+        const uint64_t e2 = fma_pair(pair_of(x[i], x[i + 1]), scale2, neg2);
+        float y0, y1;
+        if (kPolyOf > 0 && (i / 2) % kPolyOf == kPolyOf - 1) {
+          float e0, e1;
+          unpair(e2, &e0, &e1);
+          exp2_pair(pair_of(fmaxf(e0, -126.f), fmaxf(e1, -126.f)), &y0, &y1);
+        } else {
+          unpair(e2, &y0, &y1);
+          y0 = exp2_ftz(y0);
+          y1 = exp2_ftz(y1);
+        }
+        sums[(i / 2) & 1] = add_pair(sums[(i / 2) & 1], pair_of(y0, y1));
         x[i / 2] = pack_bf16x2(y0, y1);
       }
+      float sum0, sum1;
+      unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
       l = fmaf(l, corr, sum0 + sum1);
       if (__any_sync(0xffffffffu, corr != 1.0f)) {
         // O changes scale: the tile's products so far must have landed
