@@ -43,7 +43,7 @@ int32_t check_args(const mtj_cache_attn_args* a, std::string* err) {
   const int64_t most = 0x7fffffff, rows = static_cast<int64_t>(a->batch) * a->tokens;
   if (rows > most || rows * a->heads > most) return bad("batch * tokens * heads is too large");
   if (static_cast<int64_t>(a->batch) * a->kv_heads > most / kPageTokens / a->pages) return bad("batch * kv_heads * slots is too large");
-  if (a->batch > 65535 && a->dtype == MTJ_BF16) return bad("at most 65535 sequences");
+  if (!cache_prompt_fits(*a)) return bad("more than 2^20 new tokens a sequence");
   if (static_cast<int64_t>(a->n_pages) * a->kv_heads > most / kPageTokens) return bad("n_pages * kv_heads is too large");
   return MTJ_OK;
 }
@@ -68,7 +68,7 @@ int64_t mtj_k_cache_attn_scratch_bytes(const mtj_cache_attn_args* a) {
     mtj_set_error(rc, err.c_str());
     return -1;
   }
-  return mtj::takes_few(*a) ? mtj::plan_cache_few(*a).total : 256;
+  return mtj::takes_few(*a) ? mtj::plan_cache_few(*a).total : mtj::cache_prompt_scratch(*a);
 }
 
 int32_t mtj_k_cache_attn(const mtj_cache_attn_args* a, void* scratch, int64_t scratch_bytes, mtj_stream s) {
@@ -78,12 +78,12 @@ int32_t mtj_k_cache_attn(const mtj_cache_attn_args* a, void* scratch, int64_t sc
   const bool few = mtj::takes_few(*a);
   mtj::CacheFewPlan p = {};
   if (few) p = mtj::plan_cache_few(*a);
-  else p.total = 256;
+  else p.total = mtj::cache_prompt_scratch(*a);
   if (!scratch || scratch_bytes < p.total || (reinterpret_cast<uintptr_t>(scratch) & 255))
     return mtj_set_error(MTJ_ERR_INVALID, "scratch too small or not 256-byte aligned");
   const cudaStream_t st = static_cast<cudaStream_t>(s);
   const cudaError_t e = few ? mtj::run_cache_few(*a, p, static_cast<char*>(scratch), st)
-                            : mtj::run_cache_prompt(*a, st);
+                            : mtj::run_cache_prompt(*a, static_cast<char*>(scratch), st);
   if (e != cudaSuccess) return mtj_set_error(MTJ_ERR_CUDA, cudaGetErrorString(e));
   return MTJ_OK;
 }

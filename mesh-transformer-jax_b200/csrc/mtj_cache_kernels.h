@@ -26,8 +26,10 @@ struct CacheFewPlan {
 };
 CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c);
 cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, char* scratch, cudaStream_t s);
-// Prompts, bf16 without weights (mtj_cache_prompt.cu); no scratch.
-cudaError_t run_cache_prompt(const mtj_cache_attn_args& a, cudaStream_t s);
+// Prompts, bf16 without weights (mtj_cache_prompt.cu).
+int64_t cache_prompt_scratch(const mtj_cache_attn_args& c);
+bool cache_prompt_fits(const mtj_cache_attn_args& c);      // the new tokens of a sequence, into a launch's plan
+cudaError_t run_cache_prompt(const mtj_cache_attn_args& c, char* scratch, cudaStream_t s);
 
 // eight numbers of a row as bf16, rounded where they are not
 __device__ __forceinline__ uint4 load8_bf16(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }

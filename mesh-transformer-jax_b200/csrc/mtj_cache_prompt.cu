@@ -11,12 +11,23 @@
 // weights of a unit, the tensor cores have the other unit's products.  The bound for d_head 128 is shared by the tensor cores (1024
 // cycles a unit) and the exponentials (16 a cycle: 1024).
 //
+// A job is a sequence, a head (pair) and the tokens of a block.  148 blocks, one an SM, take whole jobs, longest first, in turns that
+// go forth and back; where that would leave SMs idle for longer than a join takes, the line of all jobs' key blocks is cut into equal
+// pieces instead, and where jobs are few, every job into pieces of its own (at least kLeastBlocks).  cache_begin_kernel plans that; jobs in
+// several pieces are joined by cache_part_kernel from their parts' (maximum, sum, weighted values).
+//
+// The new tokens' keys and values are read where the caller has them: key blocks are those of the cached slots, the last one filled up,
+// then 128 new tokens each.  Two warps of every block store them to their slots meanwhile (16 x 256, 2047 tokens: 67 MB, 16 us when a
+// kernel before did it).
+//
 // Scores, maxima, sums and O are 32-bit; P is rounded to bf16, half a step on average as large as the rounding of the output (a second
 // term would be half as many products again).  O is rescaled when a row's maximum has grown by more than 2^8.  The rows of V
 // behind the sequence, or of a page that does not exist, are zeroed in shared memory before they meet their zero weights.
 // Every wait is bounded.
 #include <cuda.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "mtj_cache_kernels.h"
 
@@ -26,8 +37,15 @@ namespace {
 constexpr int kRowsT = 128;                // rows of a tile
 constexpr int kKeysB = 128;                // keys of a block: two pages
 constexpr int kSoftThreads = 256;
-constexpr int kPromptThreads = kSoftThreads + 64;      // and the warps of TMA and of the products
+constexpr int kCopyThreads = 64;
+constexpr int kPromptThreads = kSoftThreads + 64 + kCopyThreads;      // and the warps of TMA and of the products
 constexpr int kBlockNotes = 8;
+constexpr int kPieces = 148;               // one block on each of a B200's SMs
+constexpr int kLeastBlocks = 4;            // of a piece that a job is cut into: the join costs about as much as three
+constexpr int kMostEntries = 8192;         // (sequence, token range) pairs of a launch
+constexpr int kJoinCost = 8;               // what cutting and joining costs, in key blocks of every piece
+constexpr int kPlanHead = 8, kPlanList = kPlanHead + kPieces * 8;      // places in the plan
+constexpr int kSizeBins = 1024;
 constexpr int kPolyOf = 4;                 // of this many pairs of weights one is worked out on the multiply-add units
 constexpr float kExp0 = 0.99992806f, kExp1 = 0.69326097f, kExp2 = 0.24261114f, kExp3 = 0.05517167f;
 
@@ -36,10 +54,11 @@ struct PromptCfg {
   static constexpr int kTiles = DH == 256 ? 1 : 2;
   static constexpr int kKeysThread = kTiles == 2 ? 128 : 64;
   static constexpr int kChunks = DH / 64;              // 64-column parts of a row
+  static constexpr int kHalves = kTiles;               // in which a thread announces its weights
   static constexpr uint32_t kQBytes = kTiles * kRowsT * DH * 2;
   static constexpr uint32_t kKBytes = kKeysB * DH * 2;
   // d_head 256: one block of keys, and values by the page
-  static constexpr int kKSlots = DH == 256 ? 1 : DH == 128 ? 2 : 4, kVSlots = DH == 256 ? 3 : DH == 128 ? 3 : 4;
+  static constexpr int kKSlots = DH == 256 ? 1 : DH == 128 ? 2 : 4, kVSlots = DH == 256 ? 3 : DH == 128 ? 2 : 4;
   static constexpr int kVPages = DH == 256 ? 1 : 2;    // of a slot
   static constexpr uint32_t kVBytes = kVPages * kPageTokens * DH * 2;
   static constexpr uint32_t kSmem = kQBytes + kKSlots * kKBytes + kVSlots * kVBytes;
@@ -176,6 +195,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* r) {
       : "r"(at)
       : "memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -196,36 +225,261 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
       : "memory");
 }
 
-// The new tokens' keys and values into their slots: a warp a (token, sequence) and key head, 16 bytes a lane.
-__global__ void __launch_bounds__(256) cache_append_kernel(const mtj_cache_attn_args a) {
-  pdl_launch_dependents();
-  const int vecs = a.kv_heads * (a.d_head / 8);
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = i / vecs;
-  if (row >= static_cast<int64_t>(a.batch) * a.tokens) return;
-  const int piece = static_cast<int>(i - row * vecs), t = static_cast<int>(row % a.tokens), b = static_cast<int>(row / a.tokens);
-  const CacheSeq s = cache_seq(a.lengths_dev, a.new_tokens_dev, b, a.tokens, a.pages);
-  if (t >= s.fresh) return;
-  const int slot = s.length - s.fresh + t;
-  const int page = a.page_table_dev[static_cast<size_t>(b) * a.pages + slot / kPageTokens];
-  if (!cache_page_ok(page, a.n_pages)) return;         // reported by the attention, which reads the same table
-  const int h = piece / (a.d_head / 8), e = piece % (a.d_head / 8);
-  const size_t at = ((static_cast<size_t>(page) * a.kv_heads + h) * kPageTokens + slot % kPageTokens) * (a.d_head / 8) + e;
-  static_cast<uint4*>(a.kpool_dev)[at] = load8_bf16(static_cast<const __nv_bfloat16*>(a.k_new_dev) + row * a.ld_k + piece * 8);
-  static_cast<uint4*>(a.vpool_dev)[at] = load8_bf16(static_cast<const __nv_bfloat16*>(a.v_new_dev) + row * a.ld_v + piece * 8);
+struct PromptArgs {
+  mtj_cache_attn_args c;                   // pointers from the launch's first sequence on
+  float scale_log2;
+  int by_heads, span;                      // a job's tiles are two heads; tokens of a job
+  int head_jobs, token_jobs;               // jobs of a token range, token ranges of a sequence
+  int* plan;                               // whole jobs or not, jobs | [kPieces][8]: sequence, head job, token job, first key
+                                           // block, key blocks | entries by size
+  float2* part_ml;                         // [kPieces][2][tiles * 128]
+  float* part_o;                           // [kPieces][2][tiles * 128][d_head]
+};
+
+// The key blocks of a job: those with first tokens, then those of the window.  Places of keys: cached slots, up to a multiple of
+// kKeysB, then the call's tokens (where it brings their keys).
+struct JobKeys {
+  int t_first, t_end;                      // its tokens
+  int fresh, first;                        // new tokens, slot of the first of them
+  int cached, tail;                        // slots that are read from pages; the first place of the call's tokens
+  int low_block, sink_blocks, blocks;
+  __device__ __forceinline__ int place(int j) const { return (j < sink_blocks ? j : low_block + j - sink_blocks) * kKeysB; }
+  __device__ __forceinline__ int slot_of(int place) const { return place < tail ? place : place - tail + cached; }
+  __device__ __forceinline__ int place_of(int slot) const { return slot < cached ? slot : slot - cached + tail; }
+};
+__device__ __forceinline__ JobKeys job_keys(const PromptArgs& a, const CacheSeq& s, int token_job) {
+  JobKeys k;
+  k.fresh = s.fresh;
+  k.first = s.length - s.fresh;
+  k.cached = a.c.k_new_dev ? k.first : s.length;
+  k.tail = (k.cached + kKeysB - 1) / kKeysB * kKeysB;
+  k.t_first = token_job * a.span;
+  k.t_end = min(s.fresh, k.t_first + a.span);
+  const int low = cache_window_low(k.first + k.t_first, a.c.window), sinks = min(a.c.sinks, low);
+  k.low_block = k.place_of(low) / kKeysB;
+  k.sink_blocks = sinks > 0 ? min(k.place_of(sinks - 1) / kKeysB + 1, k.low_block) : 0;
+  k.blocks = k.t_end > k.t_first ? k.sink_blocks + k.place_of(k.first + k.t_end - 1) / kKeysB - k.low_block + 1 : 0;
+  return k;
+}
+__device__ __forceinline__ CacheSeq prompt_seq(const PromptArgs& a, int b) {
+  return cache_seq(a.c.lengths_dev, a.c.new_tokens_dev, b, a.c.tokens, a.c.pages);
 }
 
-// by_heads: a block's two tiles are heads 2i and 2i + 1 at the same tokens, otherwise 256 tokens of one head
+// Block 0 plans; the others put zeros into the rows of the output that no token has, a warp a row.
+constexpr int kBeginThreads = 256, kZeroRows = 64;
+__device__ __forceinline__ int begin_scan(int v, int* sums, int* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  int before = x - v, total = 0;
+  for (int w = 0; w < kBeginThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  *all = total;
+  return before;
+}
+__global__ void __launch_bounds__(kBeginThreads) cache_begin_kernel(const PromptArgs a) {
+  pdl_launch_dependents();
+  const mtj_cache_attn_args& c = a.c;
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    const int64_t rows = static_cast<int64_t>(c.batch) * c.tokens, r0 = static_cast<int64_t>(blockIdx.x - 1) * kZeroRows;
+    for (int64_t row = r0 + (tid >> 5); row < min(rows, r0 + kZeroRows); row += kBeginThreads / 32) {
+      const int b = static_cast<int>(row / c.tokens), t = static_cast<int>(row - static_cast<int64_t>(b) * c.tokens);
+      if (t < prompt_seq(a, b).fresh) continue;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(c.out_dev) + row * c.ld_out);
+      for (int v = tid & 31; v < c.heads * (c.d_head / 8); v += 32) out[v] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  // before[e]: key blocks, later pieces, of a head job before entry e = (sequence, token job)
+  __shared__ int before[kMostEntries + 1], sums[kBeginThreads / 32], bins[kSizeBins], s_most;
+  const int entries = c.batch * a.token_jobs, per = (entries + kBeginThreads - 1) / kBeginThreads;
+  const int e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
+  int mine = 0, jobs = 0, most = 0, total, all_jobs;
+  if (tid == 0) s_most = 0;
+  for (int e = e0; e < e1; ++e) {
+    const int b = e / a.token_jobs;
+    const CacheSeq s = prompt_seq(a, b);
+    if (s.bad && e == b * a.token_jobs && c.status_dev) atomicOr(c.status_dev, kDevErrBadIndex);
+    const int n = job_keys(a, s, e - b * a.token_jobs).blocks;
+    before[e] = n;
+    mine += n;
+    jobs += n > 0;
+    most = max(most, n);
+  }
+  int x = begin_scan(mine, sums, &total);
+  begin_scan(jobs, sums, &all_jobs);
+  atomicMax(&s_most, most);
+  __syncthreads();
+  most = s_most;
+  const int64_t line = static_cast<int64_t>(total) * a.head_jobs;
+  const int64_t job_count = static_cast<int64_t>(all_jobs) * a.head_jobs;
+  const int64_t turns = (job_count + kPieces - 1) / kPieces;
+  const bool whole = job_count == 0 || max(static_cast<int64_t>(most), turns * line / job_count) <= line / kPieces + kJoinCost;
+  const bool cut_jobs = !whole && job_count <= kPieces / 2;
+  if (tid == 0) {
+    a.plan[0] = whole ? 1 : 0;
+    a.plan[1] = static_cast<int>(job_count);
+  }
+  if (whole) {
+    // entries by size, the largest first; the order among equals is of no consequence
+    for (int i = tid; i < kSizeBins; i += kBeginThreads) bins[i] = 0;
+    __syncthreads();
+    for (int e = e0; e < e1; ++e)
+      if (before[e] > 0) atomicAdd(&bins[kSizeBins - min(before[e], kSizeBins)], 1);
+    __syncthreads();
+    constexpr int kBinsEach = kSizeBins / kBeginThreads;
+    int n = 0, counts[kBinsEach];
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) n += counts[i] = bins[tid * kBinsEach + i];
+    x = begin_scan(n, sums, &total);
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) {
+      bins[tid * kBinsEach + i] = x;
+      x += counts[i];
+    }
+    __syncthreads();
+    for (int e = e0; e < e1; ++e)
+      if (before[e] > 0) a.plan[kPlanList + atomicAdd(&bins[kSizeBins - min(before[e], kSizeBins)], 1)] = e;
+    if (tid < kPieces) a.plan[kPlanHead + tid * 8 + 4] = 0;
+    return;
+  }
+  // with pieces this wide they are at most kPieces
+  const int width = cut_jobs ? max(kLeastBlocks, static_cast<int>((line + kPieces - job_count - 1) / (kPieces - job_count))) : 0;
+  if (cut_jobs) {
+    mine = 0;
+    for (int e = e0; e < e1; ++e) mine += before[e] = (before[e] + width - 1) / width;
+    x = begin_scan(mine, sums, &total);
+  }
+  for (int e = e0; e < e1; ++e) {
+    const int n = before[e];
+    before[e] = x;
+    x += n;
+  }
+  if (tid == 0) before[entries] = total;
+  __syncthreads();
+  const int64_t pieces_line = cut_jobs ? static_cast<int64_t>(total) * a.head_jobs : line;
+  if (tid < kPieces) {
+    const int64_t used = min(pieces_line, static_cast<int64_t>(kPieces));      // no piece before the last one is empty
+    const int64_t at = cut_jobs || tid >= used ? tid : line * tid / used;
+    int n = tid >= used ? 0 : cut_jobs ? 1 : static_cast<int>(line * (tid + 1) / used - at);
+    int b = 0, head_job = 0, token_job = 0, j = 0;
+    if (n > 0) {
+      int lo = 0, hi = c.batch - 1;                      // the last sequence that begins at or before this place
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (static_cast<int64_t>(before[mid * a.token_jobs]) * a.head_jobs <= at) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+      const int base = before[b * a.token_jobs], of_head = before[(b + 1) * a.token_jobs] - base;
+      const int64_t rest = at - static_cast<int64_t>(base) * a.head_jobs;
+      head_job = static_cast<int>(rest / of_head);
+      const int within = static_cast<int>(rest - static_cast<int64_t>(head_job) * of_head);
+      lo = 0;
+      hi = a.token_jobs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[b * a.token_jobs + mid] - base <= within) lo = mid;
+        else hi = mid - 1;
+      }
+      token_job = lo;
+      j = within - (before[b * a.token_jobs + token_job] - base);
+      if (cut_jobs) {
+        const int blocks = job_keys(a, prompt_seq(a, b), token_job).blocks, parts = (blocks + width - 1) / width, k = j;
+        j = blocks * k / parts;
+        n = blocks * (k + 1) / parts - j;
+      }
+    }
+    int* p = a.plan + kPlanHead + tid * 8;
+    p[0] = b;
+    p[1] = head_job;
+    p[2] = token_job;
+    p[3] = j;
+    p[4] = n;
+  }
+}
+
+// A block's way through its jobs; every role of a block goes it on its own.
+struct Walk {
+  int b, head_job, token_job, j, left, turn, jobs;
+  JobKeys k;
+  int n;                                   // key blocks of the current job that belong to the block
+  __device__ __forceinline__ bool begin(const PromptArgs& a) {
+    turn = a.plan[0] ? 0 : -1;
+    jobs = a.plan[1];
+    if (turn >= 0) return take(a);
+    const int* p = a.plan + kPlanHead + blockIdx.x * 8;
+    b = p[0];
+    head_job = p[1];
+    token_job = p[2];
+    j = p[3];
+    left = p[4];
+    if (left > 0) enter(a);
+    return left > 0;
+  }
+  // whole jobs: turn by turn, every other turn from the last block to the first
+  __device__ __forceinline__ bool take(const PromptArgs& a) {
+    const int64_t at = static_cast<int64_t>(turn) * kPieces + (turn & 1 ? kPieces - 1 - blockIdx.x : blockIdx.x);
+    if (at >= jobs) return false;
+    const int e = a.plan[kPlanList + at / a.head_jobs];
+    b = e / a.token_jobs;
+    token_job = e - b * a.token_jobs;
+    head_job = static_cast<int>(at % a.head_jobs);
+    j = 0;
+    left = 0x7fffffff;
+    enter(a);
+    return true;
+  }
+  __device__ __forceinline__ void enter(const PromptArgs& a) {
+    k = job_keys(a, prompt_seq(a, b), token_job);
+    n = min(left, k.blocks - j);
+  }
+  __device__ __forceinline__ bool next(const PromptArgs& a) {
+    if (turn >= 0) {
+      ++turn;
+      return take(a);
+    }
+    left -= n;
+    if (left <= 0) return false;
+    j = 0;
+    ++token_job;
+    for (;;) {
+      if (token_job < a.token_jobs) {
+        enter(a);
+        if (k.blocks > 0) return true;
+      }
+      token_job = 0;                       // a sequence's token jobs without tokens are its last ones
+      if (++head_job == a.head_jobs) {
+        head_job = 0;
+        if (++b >= a.c.batch) return false;      // cannot happen: the pieces end with the line
+      }
+      enter(a);
+      if (k.blocks > 0) return true;
+    }
+  }
+  __device__ __forceinline__ bool whole() const { return j == 0 && n == k.blocks; }
+};
+
 template <int DH>
 __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v,
-                                                                      const mtj_cache_attn_args a, float scale_log2, int by_heads,
-                                                                      int token_tiles) {
+                                                                      const __grid_constant__ CUtensorMap map_k_new,
+                                                                      const __grid_constant__ CUtensorMap map_v_new, const PromptArgs a) {
   using C = PromptCfg<DH>;
-  constexpr int kTiles = C::kTiles, kKeysThread = C::kKeysThread;
+  constexpr int kTiles = C::kTiles, kKeysThread = C::kKeysThread, kHalves = C::kHalves;
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
-  __shared__ __align__(8) uint64_t bars[1 + 2 * C::kKSlots + 2 * C::kVSlots + 6];
+  __shared__ __align__(8) uint64_t bars[2 + 2 * C::kKSlots + 2 * C::kVSlots + 10];
   __shared__ uint32_t tmem_slot, failed;
   __shared__ int notes[kBlockNotes];                   // valid rows of a key block's pages: first | second << 8
   __shared__ float part_max[2][kRowsT];                // d_head 256: of the two threads of a row
@@ -233,11 +487,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   const uint32_t sQ = base, sK = base + C::kQBytes, sV = sK + C::kKSlots * C::kKBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = k_full + 8 * C::kKSlots, v_full = k_empty + 8 * C::kKSlots,
-                 v_empty = v_full + 8 * C::kVSlots, s_full = v_empty + 8 * C::kVSlots, p_full = s_full + 16, o_done = p_full + 16;
+  const uint32_t q_full = bar0, q_empty = bar0 + 8, k_full = bar0 + 16, k_empty = k_full + 8 * C::kKSlots, v_full = k_empty + 8 * C::kKSlots,
+                 v_empty = v_full + 8 * C::kVSlots, s_full = v_empty + 8 * C::kVSlots, p_full = s_full + 16, p_half = p_full + 16,
+                 o_done = p_half + 16, o_free = o_done + 16;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 1 + 2 * C::kKSlots + 2 * C::kVSlots + 6; ++i) mbar_init(bar0 + 8u * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(p_full + 8u * i, kTiles == 2 ? 128 : 256);
+    for (int i = 0; i < 2 + 2 * C::kKSlots + 2 * C::kVSlots + 10; ++i) mbar_init(bar0 + 8u * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(p_full + 8u * i, kSoftThreads / kTiles);
+      mbar_init(p_half + 8u * i, kSoftThreads / kTiles);
+      mbar_init(o_free + 8u * i, kSoftThreads / kTiles);
+    }
     mbar_fence_init();
     failed = 0;
   }
@@ -249,284 +508,371 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
-
-  // what this block has: sequence b, the tiles' first head and token; later tokens, which see more, first
-  const int b = blockIdx.z, group = a.heads / a.kv_heads;
-  const int tile0 = (token_tiles - 1 - static_cast<int>(blockIdx.y)) * (kTiles == 2 && !by_heads ? 2 : 1);
-  const int head0 = blockIdx.x * (by_heads ? 2 : 1), kvh = head0 / group;
-  const CacheSeq s = cache_seq(a.lengths_dev, a.new_tokens_dev, b, a.tokens, a.pages);
-  if (s.bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && a.status_dev) atomicOr(a.status_dev, kDevErrBadIndex);
-  const int t_first = tile0 * kRowsT, t_end = min(s.fresh, t_first + (kTiles == 2 && !by_heads ? 2 : 1) * kRowsT);
-  const int p_first = s.length - s.fresh + t_first, p_last = s.length - s.fresh + t_end - 1;
-  const int low = cache_window_low(p_first, a.window);
-  const int low_block = low / kKeysB, sink_blocks = min((min(a.sinks, low) + kKeysB - 1) / kKeysB, low_block);
-  const int nb = t_end > t_first ? sink_blocks + p_last / kKeysB - low_block + 1 : 0;
-  const int units = nb * kTiles;
-  auto first_key = [&](int j) { return (j < sink_blocks ? j : low_block + j - sink_blocks) * kKeysB; };
   pdl_wait();
+  pdl_launch_dependents();                             // behind the allocation of tensor memory
+  const int group = a.c.heads / a.c.kv_heads;
 
+  if (warp >= 8) {
+    // registers: 8 warps of 200 and 4 of 88 are 62464 of the 64512 that the block is launched with
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    Walk w;
+    const bool work = w.begin(a);
   if (warp == 8) {
     // ---- TMA ----
-    if (lane == 0 && nb > 0) {
-      asm volatile("fence.proxy.async;" ::: "memory");     // the slots' newest rows were stored by the kernel before
-      mbar_expect_tx(q_full, C::kQBytes);
+    if (lane == 0 && work) {
+      int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
+      bool ok = true;
+      do {
+        const int head0 = w.head_job * (a.by_heads ? 2 : 1), kvh = head0 / group;
+        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1);
+        if (!ok) break;
+        mbar_expect_tx(q_full, C::kQBytes);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int c = 0; c < C::kChunks; ++c)
-          tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (by_heads ? t : 0)) * DH + c * 64,
-                  b * a.tokens + t_first + (by_heads ? 0 : t * kRowsT), q_full);
-      const int32_t* table = a.page_table_dev + static_cast<size_t>(b) * a.pages;
-      int page[2], valid[2];
-      auto look_up = [&](int j) {
-        const int key = first_key(j);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = key / kPageTokens + h;
-          valid[h] = min(kPageTokens, max(0, s.length - at * kPageTokens));
-          page[h] = valid[h] > 0 ? table[at] : 0;
-          if (!cache_page_ok(page[h], a.n_pages)) {
-            valid[h] = page[h] = 0;
-            if (a.status_dev) atomicOr(a.status_dev, kDevErrBadIndex);
-          }
-        }
-      };
-      auto load_k = [&](int j) {
-        const int st = j % C::kKSlots;
-        if (j >= C::kKSlots && !mbar_wait(k_empty + 8 * st, (j / C::kKSlots - 1) & 1)) return false;
-        look_up(j);
-        notes[j % kBlockNotes] = valid[0] | valid[1] << 8;
-        // a page without valid rows is not read: page 0 stands in, nobody sees its scores
-        mbar_expect_tx(k_full + 8 * st, C::kKBytes);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
-            tma_box(sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), &map_k, c * 64,
-                    (page[h] * a.kv_heads + kvh) * kPageTokens, k_full + 8 * st);
-        return true;
-      };
-      auto load_v = [&](int j) {
-        look_up(j);
-        for (int i = 0; i < 2 / C::kVPages; ++i) {
-          const int n = j * (2 / C::kVPages) + i, st = n % C::kVSlots;
-          if (n >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (n / C::kVSlots - 1) & 1)) return false;
-          mbar_expect_tx(v_full + 8 * st, C::kVBytes);
+            tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t : 0)) * DH + c * 64,
+                    w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : t * kRowsT), q_full);
+        const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
+        // a key block's pages, or its rows of new tokens: the row and column where the 64 begin, and how many hold something
+        int row[2], valid[2];
+        bool cached = true;
+        auto look_up = [&](int j) {
+          const int place = w.k.place(w.j + j);
+          cached = place < w.k.tail;
 #pragma unroll
-          for (int h = 0; h < C::kVPages; ++h)
+          for (int h = 0; h < 2; ++h) {
+            if (!cached) {
+              const int t = place - w.k.tail + h * kPageTokens;
+              valid[h] = min(kPageTokens, max(0, w.k.fresh - t));
+              row[h] = w.b * a.c.tokens + t;
+              continue;
+            }
+            const int at = place / kPageTokens + h;
+            valid[h] = min(kPageTokens, max(0, w.k.cached - at * kPageTokens));
+            int page = valid[h] > 0 ? table[at] : 0;
+            if (!cache_page_ok(page, a.c.n_pages)) {
+              // not read: page 0 stands in, nobody sees its scores
+              valid[h] = page = 0;
+              if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+            }
+            row[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
+          }
+        };
+        auto load_k = [&](int j) {
+          const int st = kc % C::kKSlots;
+          if (kc >= C::kKSlots && !mbar_wait(k_empty + 8 * st, (kc / C::kKSlots - 1) & 1)) return false;
+          look_up(j);
+          notes[kc % kBlockNotes] = valid[0] | valid[1] << 8;
+          mbar_expect_tx(k_full + 8 * st, C::kKBytes);
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
-              tma_box(sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128), &map_v, c * 64,
-                      (page[C::kVPages == 2 ? h : i] * a.kv_heads + kvh) * kPageTokens, v_full + 8 * st);
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c) {
+              const uint32_t dst = sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128);
+              if (cached) tma_box(dst, &map_k, c * 64, row[h], k_full + 8 * st);
+              else tma_box(dst, &map_k_new, kvh * DH + c * 64, row[h], k_full + 8 * st);
+            }
+          ++kc;
+          return true;
+        };
+        auto load_v = [&](int j) {
+          look_up(j);
+          for (int i = 0; i < 2 / C::kVPages; ++i, ++vc) {
+            const int st = vc % C::kVSlots;
+            if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
+            mbar_expect_tx(v_full + 8 * st, C::kVBytes);
+#pragma unroll
+            for (int h = 0; h < C::kVPages; ++h)
+#pragma unroll
+              for (int c = 0; c < C::kChunks; ++c) {
+                const uint32_t dst = sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128);
+                const int at = row[C::kVPages == 2 ? h : i];
+                if (cached) tma_box(dst, &map_v, c * 64, at, v_full + 8 * st);
+                else tma_box(dst, &map_v_new, kvh * DH + c * 64, at, v_full + 8 * st);
+              }
+          }
+          return true;
+        };
+        // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...
+        ok = load_k(0);
+        for (int j = 0; ok && j < w.n; ++j) {
+          if (j + 1 < w.n) ok = load_k(j + 1);
+          if (ok) ok = load_v(j);
         }
-        return true;
-      };
-      // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...
-      bool ok = load_k(0);
-      for (int j = 0; ok && j < nb; ++j) {
-        if (j + 1 < nb) ok = load_k(j + 1);
-        if (ok) ok = load_v(j);
-      }
+        ++seg;
+      } while (ok && w.next(a));
       if (!ok) atomicOr(&failed, 1u);
     }
   } else if (warp == 9) {
     // ---- products ----
-    if (nb > 0) {
+    if (work) {
       const uint32_t leader = elected();
       auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
       constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kRowsT >> 4) << 24);
       constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kRowsT >> 4) << 24);
-      auto issue_s = [&](int u) {
-        const int j = u / kTiles, t = u % kTiles, st = j % C::kKSlots;
-        if (t == 0 && !wait(k_full + 8 * st, (j / C::kKSlots) & 1)) return false;
-        fence_after();
-#pragma unroll
-        for (int c = 0; c < C::kChunks; ++c) {
-          const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
-          const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (kKeysB * 128), 16, 1024);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ss(tmem + C::kColS + (u & 1) * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
-        }
-        commit_to(s_full + 8 * (u & 1), leader);
-        if (t == kTiles - 1) commit_to(k_empty + 8 * st, leader);
-        return true;
-      };
-      auto issue_pv = [&](int u) {
-        const int j = u / kTiles, t = u % kTiles;
-        if (!wait(p_full + 8 * (u & 1), (u >> 1) & 1)) return false;
-#pragma unroll
-        for (int i = 0; i < 2 / C::kVPages; ++i) {
-          const int n = j * (2 / C::kVPages) + i, st = n % C::kVSlots;
-          if (t == 0 && !wait(v_full + 8 * st, (n / C::kVSlots) & 1)) return false;
+      int k0 = 0, v0 = 0, u0 = 0, seg = 0;                 // key blocks, value slots, units and jobs before the current job
+      bool ok = true;
+      do {
+        // the same in all lanes, and known to be: what hangs on it stays in uniform registers
+        const int blocks = __reduce_max_sync(0xffffffffu, w.n), units = blocks * kTiles;
+        auto issue_s = [&](int u) {
+          const int j = k0 + u / kTiles, t = u % kTiles, st = j % C::kKSlots, buf = (u0 + u) & 1;
+          if (t == 0 && !wait(k_full + 8 * st, (j / C::kKSlots) & 1)) return false;
           fence_after();
-          const uint64_t vd = smem_desc(sV + st * C::kVBytes, C::kVPages * kPageTokens * 128, 1024);
-          const uint32_t pa = tmem + C::kColS + (u & 1) * kKeysB + i * (kPageTokens / 2);
 #pragma unroll
-          for (int k = 0; k < C::kVPages * 4; ++k)
-            mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | i | k) ? 1u : 0u, leader);
-          if (t == kTiles - 1) commit_to(v_empty + 8 * st, leader);
+          for (int c = 0; c < C::kChunks; ++c) {
+            const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
+            const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (kKeysB * 128), 16, 1024);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_ss(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+          }
+          commit_to(s_full + 8 * buf, leader);
+          if (t == kTiles - 1) commit_to(k_empty + 8 * st, leader);
+          if (u == units - 1) commit_to(q_empty, leader);
+          return true;
+        };
+        auto issue_pv = [&](int u) {
+          const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1;
+          const uint32_t parity = ((u0 + u) >> 1) & 1;
+          // the accumulator's last job has been read
+          if (seg > 0 && u < kTiles && !wait(o_free + 8 * t, (seg - 1) & 1)) return false;
+          if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                    // by the page: the second half of the weights comes later
+            if (C::kHalves == 2 && h == 1 && !wait(p_full + 8 * buf, parity)) return false;
+            const int n = v0 + (C::kVPages == 2 ? j : 2 * j + h), st = n % C::kVSlots;
+            if (t == 0 && (C::kVPages == 1 || h == 0) && !wait(v_full + 8 * st, (n / C::kVSlots) & 1)) return false;
+            fence_after();
+            const uint64_t vd = smem_desc(sV + st * C::kVBytes, C::kVPages * kPageTokens * 128, 1024);
+            const uint32_t pa = tmem + C::kColS + buf * kKeysB + h * (kPageTokens / 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>(((C::kVPages == 2 ? h * 4 + k : k) * 2048) >> 4), kIdO,
+                     (j | h | k) ? 1u : 0u, leader);
+            if (t == kTiles - 1 && (C::kVPages == 1 || h == 1)) commit_to(v_empty + 8 * st, leader);
+          }
+          commit_to(o_done + 8 * buf, leader);
+          return true;
+        };
+        ok = wait(q_full, seg & 1) && issue_s(0);
+        if (ok && units > 1) ok = issue_s(1);
+        for (int u = 0; ok && u < units; ++u) {
+          ok = issue_pv(u);
+          if (ok && u + 2 < units) ok = issue_s(u + 2);
         }
-        commit_to(o_done + 8 * (u & 1), leader);
-        return true;
-      };
-      bool ok = wait(q_full, 0) && issue_s(0);
-      if (ok && units > 1) ok = issue_s(1);
-      for (int u = 0; ok && u < units; ++u) {
-        ok = issue_pv(u);
-        if (ok && u + 2 < units) ok = issue_s(u + 2);
-      }
+        k0 += blocks;
+        v0 += blocks * (2 / C::kVPages);
+        u0 += units;
+        ++seg;
+      } while (__any_sync(0xffffffffu, ok && w.next(a)));
       if (!ok && leader) atomicOr(&failed, 1u);
     }
+  } else if (warp >= 10) {
+    // ---- the new rows into their slots, this block's share ----
+    // a warp a token, so that what it has to work out for one is little beside the softmax warps' arithmetic on the same schedulers
+    if (a.c.k_new_dev) {
+      const int vecs = a.c.kv_heads * (DH / 8), stride = a.c.kv_heads * kPageTokens * (DH / 8);
+      const int rows = a.c.batch * a.c.tokens;
+      for (int row = blockIdx.x * (kCopyThreads / 32) + warp - 10; row < rows; row += kPieces * (kCopyThreads / 32)) {
+        const int b = row / a.c.tokens, t = row - b * a.c.tokens;
+        const CacheSeq s = prompt_seq(a, b);
+        if (t >= s.fresh) continue;
+        const int slot = s.length - s.fresh + t, page = a.c.page_table_dev[static_cast<size_t>(b) * a.c.pages + slot / kPageTokens];
+        if (!cache_page_ok(page, a.c.n_pages)) {
+          if (lane == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+          continue;
+        }
+        const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.c.k_new_dev) + static_cast<size_t>(row) * a.c.ld_k;
+        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v_new_dev) + static_cast<size_t>(row) * a.c.ld_v;
+        const size_t at = static_cast<size_t>(page) * stride + slot % kPageTokens * (DH / 8);
+        constexpr int kFlight = 4;
+        for (int i = lane; i < vecs; i += 32 * kFlight) {
+          uint4 xk[kFlight], xv[kFlight];
+#pragma unroll
+          for (int f = 0; f < kFlight; ++f)
+            if (i + 32 * f < vecs) {
+              xk[f] = load8_bf16(k + (i + 32 * f) * 8);
+              xv[f] = load8_bf16(v + (i + 32 * f) * 8);
+            }
+#pragma unroll
+          for (int f = 0; f < kFlight; ++f)
+            if (i + 32 * f < vecs) {
+              const int e = i + 32 * f;
+              const size_t to = at + static_cast<size_t>(e / (DH / 8)) * (kPageTokens * (DH / 8)) + e % (DH / 8);
+              static_cast<uint4*>(a.c.kpool_dev)[to] = xk[f];
+              static_cast<uint4*>(a.c.vpool_dev)[to] = xv[f];
+            }
+        }
+      }
+    }
+  }
   } else {
     // ---- weights ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    Walk w;
+    if (w.begin(a)) {
     const int wg = warp >> 2, quad = warp & 3;
     const int tile = kTiles == 2 ? wg : 0, part = kTiles == 2 ? 0 : wg;      // of the keys of a block
     const int r = quad * 32 + lane;                        // row of the tile = lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const int head = head0 + (by_heads ? tile : 0), t0 = t_first + (by_heads ? 0 : tile * kRowsT);
-    const int t = t0 + r;
-    const int p = t < s.fresh ? s.length - s.fresh + t : -1;
-    const int warp_first = s.length - s.fresh + t0 + quad * 32;      // slots of the warp's rows: warp_first .. + 31
-    float m_ref = -INFINITY, l = 0.f;
+    int block = 0;                                         // key blocks so far
     bool ok = true;
-    for (int j = 0; j < nb; ++j) {
-      const int u = kTiles == 2 ? 2 * j + wg : j;
-      if (ok) ok = mbar_wait(s_full + 8 * (u & 1), (u >> 1) & 1);
-      fence_after();
-      const int key = first_key(j) + part * kKeysThread;
-      const int note = notes[j % kBlockNotes];
-      const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
-      uint32_t x[kKeysThread];
+    do {
+      const int head = w.head_job * (a.by_heads ? 2 : 1) + (a.by_heads ? tile : 0);
+      const int t0 = w.k.t_first + (a.by_heads ? 0 : tile * kRowsT), t = t0 + r;
+      const int p = t < w.k.fresh ? w.k.first + t : -1;
+      const int p_last = w.k.first + w.k.t_end - 1;
+      const int warp_first = w.k.first + t0 + quad * 32;   // slots of the warp's rows: warp_first .. + 31
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < w.n; ++j, ++block) {
+        const int u = kTiles == 2 ? 2 * block + wg : block;
+        if (ok) ok = mbar_wait(s_full + 8 * (u & 1), (u >> 1) & 1);
+        fence_after();
+        const int key = w.k.slot_of(w.k.place(w.j + j)) + part * kKeysThread;      // slot of this thread's first key
+        const int note = notes[block % kBlockNotes];
+        const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
+        uint32_t x[kKeysThread];
 #pragma unroll
-      for (int i = 0; i < kKeysThread; i += 32) tmem_fetch32(at_s + i, x + i);
-      tmem_wait();
+        for (int i = 0; i < kKeysThread; i += 32) tmem_fetch32(at_s + i, x + i);
+        tmem_wait();
 #pragma unroll
-      for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
-      // V's rows that hold nothing: zeroed before anybody's weights are announced
-      if (note != (kPageTokens | kPageTokens << 8)) {
+        for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
+        constexpr int kFullNote = kPageTokens | kPageTokens << 8;
+        // V's rows that hold nothing: zeroed before anybody's weights are announced
+        if (note != kFullNote) {
 #pragma unroll
-        for (int i = 0; i < 2 / C::kVPages; ++i) {
-          const int n = j * (2 / C::kVPages) + i, st = n % C::kVSlots;
-          if (ok) ok = mbar_wait(v_full + 8 * st, (n / C::kVSlots) & 1);
-          if (tile == 0) {
-            // [64-column part][page][64 rows][128 bytes]
-            for (int e = threadIdx.x; e < static_cast<int>(C::kVBytes / 16); e += kTiles == 2 ? 128 : 256) {
-              const int row = e / 8 % kPageTokens, h = C::kVPages == 2 ? e / 8 / kPageTokens % 2 : i;
-              if (row >= ((note >> (8 * h)) & 255))
-                *reinterpret_cast<uint4*>(prompt_smem + (sV - base) + st * C::kVBytes + e * 16) = make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 2 / C::kVPages; ++i) {
+            const int n = block * (2 / C::kVPages) + i, st = n % C::kVSlots;
+            if (ok) ok = mbar_wait(v_full + 8 * st, (n / C::kVSlots) & 1);
+            if (tile == 0) {
+              // [64-column part][page][64 rows][128 bytes]
+              for (int e = threadIdx.x; e < static_cast<int>(C::kVBytes / 16); e += kSoftThreads / kTiles) {
+                const int row = e / 8 % kPageTokens, h = C::kVPages == 2 ? e / 8 / kPageTokens % 2 : i;
+                if (row >= ((note >> (8 * h)) & 255))
+                  *reinterpret_cast<uint4*>(prompt_smem + (sV - base) + st * C::kVBytes + e * 16) = make_uint4(0, 0, 0, 0);
+              }
             }
           }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      const int warp_last = min(warp_first + 31, p_last);
-      const bool whole = note == (kPageTokens | kPageTokens << 8) && key + kKeysThread - 1 <= warp_first &&
-                         (key + kKeysThread - 1 < a.sinks || warp_last - key < a.window) && warp_last >= warp_first;
-      if (!whole) {
-        // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
-        const int hi = p - key, lo = p - a.window + 1 - key, sk = a.sinks - key;
+        const int warp_last = min(warp_first + 31, p_last);
+        const bool all_seen = note == kFullNote && key + kKeysThread - 1 <= warp_first &&
+                              (key + kKeysThread - 1 < a.c.sinks || warp_last - key < a.c.window) && warp_last >= warp_first;
+        if (!all_seen) {
+          // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
+          const int hi = p - key, lo = p - a.c.window + 1 - key, sk = a.c.sinks - key;
 #pragma unroll
-        for (int w = 0; w < kKeysThread / 32; ++w) {
-          const int within = part * kKeysThread + 32 * w;
-          const int held = (within < kPageTokens ? note & 255 : note >> 8) - within % kPageTokens;
-          const uint32_t see = low_bits(min(hi + 1, held + 32 * w) - 32 * w) & (~low_bits(lo - 32 * w) | low_bits(sk - 32 * w));
+          for (int i = 0; i < kKeysThread / 32; ++i) {
+            const int within = part * kKeysThread + 32 * i;
+            const int held = (within < kPageTokens ? note & 255 : note >> 8) - within % kPageTokens;
+            const uint32_t see = low_bits(min(hi + 1, held + 32 * i) - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i));
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(see >> i & 1u)) x[32 * w + i] = 0xff800000u;
+            for (int e = 0; e < 32; ++e)
+              if (!(see >> e & 1u)) x[32 * i + e] = 0xff800000u;
+          }
         }
-      }
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kKeysThread; i += 8)
+        for (int i = 0; i < kKeysThread; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale_log2;      // scale > 0
-      if constexpr (kTiles == 1) {
-        part_max[part][r] = top;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        top = fmaxf(top, part_max[part ^ 1][r]);
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-      }
-      float m_new = m_ref;
-      if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top;
-      const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
-      const float neg = m_new == -INFINITY ? 0.f : -m_new;
-      const uint64_t scale2 = pair_of(scale_log2, scale_log2), neg2 = pair_of(neg, neg);
-      uint64_t sums[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < kKeysThread; i += 2) {
-        const uint64_t e2 = fma_pair(pair_of(x[i], x[i + 1]), scale2, neg2);
-        float y0, y1;
-        if (kPolyOf > 0 && (i / 2) % kPolyOf == kPolyOf - 1) {
-          float e0, e1;
-          unpair(e2, &e0, &e1);
-          exp2_pair(pair_of(fmaxf(e0, -126.f), fmaxf(e1, -126.f)), &y0, &y1);
-        } else {
-          unpair(e2, &y0, &y1);
-          y0 = exp2_ftz(y0);
-          y1 = exp2_ftz(y1);
+          for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;      // scale > 0
+        if constexpr (kTiles == 1) {
+          part_max[part][r] = top;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+          top = fmaxf(top, part_max[part ^ 1][r]);
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
         }
-        sums[(i / 2) & 1] = add_pair(sums[(i / 2) & 1], pair_of(y0, y1));
-        x[i / 2] = pack_bf16x2(y0, y1);
-      }
-      float sum0, sum1;
-      unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
-      l = fmaf(l, corr, sum0 + sum1);
-      if (__any_sync(0xffffffffu, corr != 1.0f)) {
-        // O changes scale: the tile's products so far must have landed
-        const int before = u - kTiles;
-        if (ok) ok = mbar_wait(o_done + 8 * (before & 1), (before >> 1) & 1);
-        fence_after();
+        float m_new = m_ref;
+        if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top;
+        const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+          // O changes scale: the tile's products so far must have landed
+          const int before = u - kTiles;
+          if (ok) ok = mbar_wait(o_done + 8 * (before & 1), (before >> 1) & 1);
+          fence_after();
 #pragma unroll 1
-        for (int c0 = 0; c0 < DH / (3 - kTiles); c0 += 32) {
-          const uint32_t at = tmem + lanes + C::kColO + tile * DH + part * (DH / 2) + c0;
-          uint32_t o[32];
-          tmem_load32(at, o);
+          for (int c0 = 0; c0 < DH / (3 - kTiles); c0 += 16) {
+            const uint32_t at = tmem + lanes + C::kColO + tile * DH + part * (DH / 2) + c0;
+            uint32_t o[16];
+            tmem_load16(at, o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-          tmem_store32(at, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_store16(at, o);
+          }
         }
-      }
+        const float neg = m_new == -INFINITY ? 0.f : -m_new;
+        const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
+        const uint32_t at_p = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * (kKeysThread / 2);
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < kKeysThread / 2; i += 32)
-        tmem_store32(tmem + lanes + C::kColS + (u & 1) * kKeysB + part * (kKeysThread / 2) + i, x + i);
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      fence_before();
-      arrive_at(p_full + 8 * (u & 1));
-      m_ref = m_new;
-    }
-    if (nb > 0) {
-      const int u = kTiles == 2 ? 2 * (nb - 1) + wg : nb - 1;
+        for (int half = 0; half < kHalves; ++half) {
+#pragma unroll
+          for (int i = half * (kKeysThread / kHalves); i < (half + 1) * (kKeysThread / kHalves); i += 2) {
+            const uint64_t e2 = fma_pair(pair_of(x[i], x[i + 1]), scale2, neg2);
+            float y0, y1;
+            if (kPolyOf > 0 && (i / 2) % kPolyOf == kPolyOf - 1) {
+              float e0, e1;
+              unpair(e2, &e0, &e1);
+              exp2_pair(pair_of(fmaxf(e0, -126.f), fmaxf(e1, -126.f)), &y0, &y1);
+            } else {
+              unpair(e2, &y0, &y1);
+              y0 = exp2_ftz(y0);
+              y1 = exp2_ftz(y1);
+            }
+            sums[(i / 2) & 1] = add_pair(sums[(i / 2) & 1], pair_of(y0, y1));
+            x[i / 2] = pack_bf16x2(y0, y1);
+          }
+#pragma unroll
+          for (int i = half * (kKeysThread / kHalves / 2); i < (half + 1) * (kKeysThread / kHalves / 2); i += 32) tmem_store32(at_p + i, x + i);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          fence_before();
+          arrive_at((half < kHalves - 1 ? p_half : p_full) + 8 * (u & 1));
+        }
+        float sum0, sum1;
+        unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
+        l = fmaf(l, corr, sum0 + sum1);
+        m_ref = m_new;
+      }
+      // the job's result, or the piece's part of it
+      const int u = kTiles == 2 ? 2 * (block - 1) + wg : block - 1;
       if (ok) ok = mbar_wait(o_done + 8 * (u & 1), (u >> 1) & 1);
-      if (!ok) atomicOr(&failed, 1u);
-    }
-    fence_after();
-    if constexpr (kTiles == 1) {
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-      part_max[part][r] = l;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-      l = part_max[0][r] + part_max[1][r];
-    }
-    const float inv = nb > 0 && l > 0.f ? 1.0f / l : 0.f;
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out_dev) + (static_cast<size_t>(b) * a.tokens + min(t, a.tokens - 1)) * a.ld_out + head * DH;
-#pragma unroll 1
-    for (int c0 = part * (DH / 2); c0 < (kTiles == 2 ? DH : (part + 1) * (DH / 2)); c0 += 32) {
-      uint32_t o[32];
-      if (nb > 0) {
-        tmem_load32(tmem + lanes + C::kColO + tile * DH + c0, o);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      fence_after();
+      if constexpr (kTiles == 1) {
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+        part_max[part][r] = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+        l = part_max[0][r] + part_max[1][r];
       }
-      if (t < a.tokens) {
+      const bool whole = w.whole();
+      const float inv = l > 0.f ? 1.0f / l : 0.f;
+      const size_t part_row = (static_cast<size_t>(blockIdx.x) * 2 + (w.j == 0 ? 1 : 0)) * (kTiles * kRowsT) + tile * kRowsT + r;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(w.b) * a.c.tokens + min(t, a.c.tokens - 1)) * a.c.ld_out + head * DH;
+#pragma unroll 1
+      for (int c0 = part * (DH / 2); c0 < (kTiles == 2 ? DH : (part + 1) * (DH / 2)); c0 += 32) {
+        uint32_t o[32];
+        tmem_load32(tmem + lanes + C::kColO + tile * DH + c0, o);
+        if (whole && p >= 0) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          float v[8];
+          for (int i = 0; i < 32; i += 8) {
+            float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = p < 0 ? 0.f : __uint_as_float(o[i + e]);
-          store8(out + c0 + i, v, inv);
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[i + e]);
+            store8(out + c0 + i, v, inv);
+          }
+        } else if (!whole) {
+          float4* dst = reinterpret_cast<float4*>(a.part_o + part_row * DH + c0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
         }
       }
+      if (!whole && part == 0) a.part_ml[part_row] = make_float2(m_ref, l);
+      fence_before();
+      arrive_at(o_free + 8 * tile);
+    } while (w.next(a));
+    if (!ok) atomicOr(&failed, 1u);
     }
   }
   fence_before();
@@ -535,37 +881,136 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
   }
-  if (threadIdx.x == 0 && failed && a.status_dev) atomicOr(a.status_dev, kDevErrTimeout);
+  if (threadIdx.x == 0 && failed && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
+}
+
+// Joins jobs that lie in several pieces.  blockIdx.y is a piece that begins inside a job, the first such of the job; a block has 8 rows,
+// a warp a row.
+constexpr int kPartRows = 8;
+template <int DH>
+__global__ void __launch_bounds__(32 * kPartRows) cache_part_kernel(const PromptArgs a) {
+  constexpr int kRows = PromptCfg<DH>::kTiles * kRowsT, kVecs = DH / 128 > 0 ? DH / 128 : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int piece = blockIdx.y + 1;
+  const int* plan = a.plan + kPlanHead;
+  auto same_job = [&](int i) {
+    const int *p = plan + piece * 8, *q = plan + i * 8;
+    return q[4] > 0 && q[0] == p[0] && q[1] == p[1] && q[2] == p[2];
+  };
+  const int* p = plan + piece * 8;
+  if (p[4] <= 0 || p[3] == 0) return;                                  // no piece, or one that begins a job
+  if (same_job(piece - 1) && plan[(piece - 1) * 8 + 3] != 0) return;     // not the first inside its job
+  int n = 2;
+  while (piece + n - 1 < kPieces && same_job(piece + n - 1) && plan[(piece + n - 1) * 8 + 3] != 0) ++n;
+  const int r = blockIdx.x * kPartRows + warp, tile = r / kRowsT;
+  const CacheSeq s = prompt_seq(a, p[0]);
+  const int t = p[2] * a.span + (a.by_heads ? r % kRowsT : r);
+  const int head = p[1] * (a.by_heads ? 2 : 1) + (a.by_heads ? tile : 0);
+  if (t >= s.fresh) return;
+  // the job's first part ends the piece before, the others begin theirs
+  auto row_of = [&](int k) { return (static_cast<size_t>(piece - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
+  float top = -INFINITY;
+  for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[row_of(k)].x);
+  top = warp_max(top);
+  float l = 0.f, o[kVecs * 4] = {};
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = a.part_ml[row_of(k)];
+    const float f = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - top);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      if (DH == 64 && lane >= 16) break;
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + row_of(k) * DH + v * 128 + lane * 4);
+      o[4 * v] = fmaf(y.x, f, o[4 * v]);
+      o[4 * v + 1] = fmaf(y.y, f, o[4 * v + 1]);
+      o[4 * v + 2] = fmaf(y.z, f, o[4 * v + 2]);
+      o[4 * v + 3] = fmaf(y.w, f, o[4 * v + 3]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(p[0]) * a.c.tokens + t) * a.c.ld_out + head * DH;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    if (DH == 64 && lane >= 16) break;
+    *reinterpret_cast<uint2*>(out + v * 128 + lane * 4) =
+        make_uint2(pack_bf16x2(o[4 * v] * inv, o[4 * v + 1] * inv), pack_bf16x2(o[4 * v + 2] * inv, o[4 * v + 3] * inv));
+  }
 }
 
 template <int DH>
-cudaError_t launch(const mtj_cache_attn_args& a, cudaStream_t s) {
+cudaError_t launch(PromptArgs a, bool join, cudaStream_t s) {
   using C = PromptCfg<DH>;
-  CUtensorMap mq, mk, mv;
-  const int64_t pool_rows = static_cast<int64_t>(a.n_pages) * a.kv_heads * kPageTokens;
-  cudaError_t e = make_tensor_map_bf16(&mq, a.q_dev, static_cast<int64_t>(a.batch) * a.tokens, static_cast<int64_t>(a.heads) * DH, kRowsT, a.ld_q);
-  if (e == cudaSuccess) e = make_tensor_map_bf16(&mk, a.kpool_dev, pool_rows, DH, kPageTokens);
-  if (e == cudaSuccess) e = make_tensor_map_bf16(&mv, a.vpool_dev, pool_rows, DH, kPageTokens);
+  const mtj_cache_attn_args& c = a.c;
+  CUtensorMap mq, mk, mv, mkn, mvn;
+  const int64_t pool_rows = static_cast<int64_t>(c.n_pages) * c.kv_heads * kPageTokens, rows = static_cast<int64_t>(c.batch) * c.tokens;
+  cudaError_t e = make_tensor_map_bf16(&mq, c.q_dev, rows, static_cast<int64_t>(c.heads) * DH, kRowsT, c.ld_q);
+  if (e == cudaSuccess) e = make_tensor_map_bf16(&mk, c.kpool_dev, pool_rows, DH, kPageTokens);
+  if (e == cudaSuccess) e = make_tensor_map_bf16(&mv, c.vpool_dev, pool_rows, DH, kPageTokens);
+  mkn = mk;
+  mvn = mv;
+  if (e == cudaSuccess && c.k_new_dev) {
+    e = make_tensor_map_bf16(&mkn, c.k_new_dev, rows, static_cast<int64_t>(c.kv_heads) * DH, kPageTokens, c.ld_k);
+    if (e == cudaSuccess) e = make_tensor_map_bf16(&mvn, c.v_new_dev, rows, static_cast<int64_t>(c.kv_heads) * DH, kPageTokens, c.ld_v);
+  }
   static DeviceOnce once;
   if (e == cudaSuccess)
     e = once.run([&] { return cudaFuncSetAttribute(cache_prompt_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem)); });
   if (e != cudaSuccess) return e;
-  if (a.k_new_dev) {
-    const int64_t vecs = static_cast<int64_t>(a.batch) * a.tokens * a.kv_heads * (DH / 8);
-    e = launch_pdl(cache_append_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256)), dim3(256), 0, s, false, a);
-    if (e != cudaSuccess) return e;
-  }
-  const bool by_heads = C::kTiles == 2 && (a.heads / a.kv_heads) % 2 == 0;
-  const int span = C::kTiles == 2 && !by_heads ? 2 * kRowsT : kRowsT;
-  const int tiles = (a.tokens + span - 1) / span;
-  return launch_pdl(cache_prompt_kernel<DH>, dim3(a.heads / (by_heads ? 2 : 1), tiles, a.batch), dim3(kPromptThreads), C::kSmem, s,
-                    a.k_new_dev != nullptr, mq, mk, mv, a, a.scale * 1.4426950408889634f, by_heads ? 1 : 0, tiles);
+  e = launch_pdl(cache_begin_kernel, dim3(1 + static_cast<unsigned>((rows + kZeroRows - 1) / kZeroRows)), dim3(kBeginThreads), 0, s, false, a);
+  if (e == cudaSuccess) e = launch_pdl(cache_prompt_kernel<DH>, dim3(kPieces), dim3(kPromptThreads), C::kSmem, s, true, mq, mk, mv, mkn, mvn, a);
+  if (e == cudaSuccess && join)
+    e = launch_pdl(cache_part_kernel<DH>, dim3(C::kTiles * kRowsT / kPartRows, kPieces - 1), dim3(32 * kPartRows), 0, s, true, a);
+  return e;
+}
+
+bool pairs_heads(const mtj_cache_attn_args& c) { return c.d_head < 256 && (c.heads / c.kv_heads) % 2 == 0; }
+int job_span(const mtj_cache_attn_args& c) { return c.d_head < 256 && !pairs_heads(c) ? 2 * kRowsT : kRowsT; }
+constexpr int64_t kPlanBytes = ((kPlanList + kMostEntries) * 4 + 255) / 256 * 256;
+int64_t part_rows(const mtj_cache_attn_args& c) { return static_cast<int64_t>(kPieces) * 2 * (c.d_head < 256 ? 2 : 1) * kRowsT; }
+
+// whether no job can lie in several pieces: jobs of few blocks are taken whole
+bool all_whole(const mtj_cache_attn_args& c) {
+  const int64_t slots = (static_cast<int64_t>(c.pages) * kPageTokens + kKeysB - 1) / kKeysB + 1;      // and the block between cached and new
+  const int64_t seen = (static_cast<int64_t>(c.window) + job_span(c)) / kKeysB + 3 + (static_cast<int64_t>(c.sinks) + kKeysB - 1) / kKeysB + 1;
+  return std::min(slots, seen) <= kJoinCost;
 }
 
 }  // namespace
 
-cudaError_t run_cache_prompt(const mtj_cache_attn_args& a, cudaStream_t s) {
-  return a.d_head == 64 ? launch<64>(a, s) : a.d_head == 128 ? launch<128>(a, s) : launch<256>(a, s);
+int64_t cache_prompt_scratch(const mtj_cache_attn_args& c) { return kPlanBytes + part_rows(c) * (8 + c.d_head * 4); }
+
+bool cache_prompt_fits(const mtj_cache_attn_args& c) { return (c.tokens + job_span(c) - 1) / job_span(c) <= kMostEntries; }
+
+cudaError_t run_cache_prompt(const mtj_cache_attn_args& c, char* scratch, cudaStream_t s) {
+  PromptArgs a = {};
+  a.c = c;
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.by_heads = pairs_heads(c);
+  a.span = job_span(c);
+  a.head_jobs = c.heads / (a.by_heads ? 2 : 1);
+  a.token_jobs = (c.tokens + a.span - 1) / a.span;
+  a.plan = reinterpret_cast<int*>(scratch);
+  a.part_ml = reinterpret_cast<float2*>(scratch + kPlanBytes);
+  a.part_o = reinterpret_cast<float*>(scratch + kPlanBytes + part_rows(c) * 8);
+  const int most = kMostEntries / a.token_jobs;        // sequences of a launch
+  for (int b0 = 0; b0 < c.batch; b0 += most) {
+    a.c.batch = std::min(most, c.batch - b0);
+    const bool join = !all_whole(c);
+    const cudaError_t e = c.d_head == 64 ? launch<64>(a, join, s) : c.d_head == 128 ? launch<128>(a, join, s) : launch<256>(a, join, s);
+    if (e != cudaSuccess) return e;
+    const size_t rows = static_cast<size_t>(a.c.batch) * c.tokens;
+    auto step = [&](const void* p, int64_t ld) { return p ? static_cast<const __nv_bfloat16*>(p) + rows * ld : nullptr; };
+    a.c.q_dev = step(a.c.q_dev, c.ld_q);
+    a.c.k_new_dev = step(a.c.k_new_dev, c.ld_k);
+    a.c.v_new_dev = step(a.c.v_new_dev, c.ld_v);
+    a.c.out_dev = static_cast<__nv_bfloat16*>(a.c.out_dev) + rows * c.ld_out;
+    a.c.page_table_dev += static_cast<size_t>(a.c.batch) * c.pages;
+    a.c.lengths_dev += a.c.batch;
+    if (a.c.new_tokens_dev) a.c.new_tokens_dev += a.c.batch;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace mtj
