@@ -17,8 +17,9 @@
 // several pieces are joined by cache_part_kernel from their parts' (maximum, sum, weighted values).
 //
 // The new tokens' keys and values are read where the caller has them: key blocks are those of the cached slots, the last one filled up,
-// then 128 new tokens each.  Two warps of every block store them to their slots meanwhile (16 x 256, 2047 tokens: 67 MB, 16 us when a
-// kernel before did it).
+// then 128 new tokens each.  Where new tokens begin a page, the block that has 64 of them in shared memory as keys of their own job
+// stores them from there, by TMA; a warp of every block, and whoever has run out of jobs, stores the others row by row.  (16 x 256, 2047
+// tokens: storing in a kernel before took 16 us, row by row beside the products it was longer than they were.)
 //
 // Scores, maxima, sums and O are 32-bit; P is rounded to bf16, half a step on average as large as the rounding of the output (a second
 // term would be half as many products again).  O is rescaled when a row's maximum has grown by more than 2^8.  The rows of V
@@ -72,6 +73,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1)
+               : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -470,6 +476,53 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return j == 0 && n == k.blocks; }
 };
 
+// Whether the 64 new tokens from t on fill a page of their own and are stored from shared memory.
+__device__ __forceinline__ bool stored_by_page(const JobKeys& k, int t) { return k.first % kPageTokens == 0 && t / kPageTokens * kPageTokens + kPageTokens <= k.fresh; }
+
+// The other new rows into their slots, a warp a row, dealt out to all warps but those of TMA and products: the two that do nothing else
+// begin at once, the softmax warps when they have run out of jobs.
+constexpr int kStoreWarps = (kPromptThreads - 64) / 32;
+template <int DH>
+__device__ __forceinline__ void store_rows(const PromptArgs& a, int worker) {
+  const int lane = threadIdx.x & 31;
+  const int vecs = a.c.kv_heads * (DH / 8), stride = a.c.kv_heads * kPageTokens * (DH / 8);
+  const int rows = a.c.batch * a.c.tokens;
+  for (int row = blockIdx.x * kStoreWarps + worker; row < rows; row += kPieces * kStoreWarps) {
+    const int b = row / a.c.tokens, t = row - b * a.c.tokens;
+    const CacheSeq s = prompt_seq(a, b);
+    JobKeys k;
+    k.fresh = s.fresh;
+    k.first = s.length - s.fresh;
+    if (t >= s.fresh || stored_by_page(k, t)) continue;
+    const int slot = k.first + t, page = a.c.page_table_dev[static_cast<size_t>(b) * a.c.pages + slot / kPageTokens];
+    if (!cache_page_ok(page, a.c.n_pages)) {
+      if (lane == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+      continue;
+    }
+    const __nv_bfloat16* kn = static_cast<const __nv_bfloat16*>(a.c.k_new_dev) + static_cast<size_t>(row) * a.c.ld_k;
+    const __nv_bfloat16* vn = static_cast<const __nv_bfloat16*>(a.c.v_new_dev) + static_cast<size_t>(row) * a.c.ld_v;
+    const size_t at = static_cast<size_t>(page) * stride + slot % kPageTokens * (DH / 8);
+    constexpr int kFlight = 4;
+    for (int i = lane; i < vecs; i += 32 * kFlight) {
+      uint4 xk[kFlight], xv[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+        if (i + 32 * f < vecs) {
+          xk[f] = load8_bf16(kn + (i + 32 * f) * 8);
+          xv[f] = load8_bf16(vn + (i + 32 * f) * 8);
+        }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f)
+        if (i + 32 * f < vecs) {
+          const int e = i + 32 * f;
+          const size_t to = at + static_cast<size_t>(e / (DH / 8)) * (kPageTokens * (DH / 8)) + e % (DH / 8);
+          static_cast<uint4*>(a.c.kpool_dev)[to] = xk[f];
+          static_cast<uint4*>(a.c.vpool_dev)[to] = xv[f];
+        }
+    }
+  }
+}
+
 template <int DH>
 __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
@@ -481,6 +534,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
   __shared__ __align__(8) uint64_t bars[2 + 2 * C::kKSlots + 2 * C::kVSlots + 10];
   __shared__ uint32_t tmem_slot, failed;
+  __shared__ int to_store[C::kKSlots + C::kVSlots][2];      // rows of the pools that a slot's pages of new rows go to
   __shared__ int notes[kBlockNotes];                   // valid rows of a key block's pages: first | second << 8
   __shared__ float part_max[2][kRowsT];                // d_head 256: of the two threads of a row
   const uint32_t base = smem_u32(prompt_smem);
@@ -521,7 +575,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     // ---- TMA ----
     if (lane == 0 && work) {
       int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
+      uint32_t storing_k = 0, storing_v = 0;               // slots with rows to store
       bool ok = true;
+      // a slot's new rows go to their pages when the products have read it, before it is filled again
+      auto store_k = [&](int st) {
+        const int* rows = to_store[st];
+        storing_k &= ~(1u << st);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            if (rows[h] >= 0) tma_store(&map_k, c * 64, rows[h], sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128));
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+      };
+      auto store_v = [&](int st) {
+        const int* rows = to_store[C::kKSlots + st];
+        storing_v &= ~(1u << st);
+#pragma unroll
+        for (int h = 0; h < C::kVPages; ++h)
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            if (rows[h] >= 0)
+              tma_store(&map_v, c * 64, rows[h], sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128));
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+      };
       do {
         const int head0 = w.head_job * (a.by_heads ? 2 : 1), kvh = head0 / group;
         if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1);
@@ -534,74 +611,113 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
             tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t : 0)) * DH + c * 64,
                     w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : t * kRowsT), q_full);
         const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
-        // a key block's pages, or its rows of new tokens: the row and column where the 64 begin, and how many hold something
-        int row[2], valid[2];
-        bool cached = true;
+        // a key block's pages, or its rows of new tokens: the row where each 64 begin, how many hold something, the page they are stored
+        // to; looked up before the slot is waited for, because the products wait for what comes behind that
+        struct Block {
+          int row[2], valid[2], target[2];
+          bool cached;
+        };
         auto look_up = [&](int j) {
+          Block x;
           const int place = w.k.place(w.j + j);
-          cached = place < w.k.tail;
+          x.cached = place < w.k.tail;
+          // a key head's new rows are stored by the job that has these tokens and the group's first head
+          const bool mine = !x.cached && place - w.k.tail >= w.k.t_first && place - w.k.tail < w.k.t_end && head0 % group == 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!cached) {
+            x.target[h] = -1;
+            if (!x.cached) {
               const int t = place - w.k.tail + h * kPageTokens;
-              valid[h] = min(kPageTokens, max(0, w.k.fresh - t));
-              row[h] = w.b * a.c.tokens + t;
+              x.valid[h] = min(kPageTokens, max(0, w.k.fresh - t));
+              x.row[h] = w.b * a.c.tokens + t;
+              if (mine && x.valid[h] > 0 && stored_by_page(w.k, t)) {
+                const int page = table[(w.k.first + t) / kPageTokens];
+                if (cache_page_ok(page, a.c.n_pages)) x.target[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
+                else if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+              }
               continue;
             }
             const int at = place / kPageTokens + h;
-            valid[h] = min(kPageTokens, max(0, w.k.cached - at * kPageTokens));
-            int page = valid[h] > 0 ? table[at] : 0;
+            x.valid[h] = min(kPageTokens, max(0, w.k.cached - at * kPageTokens));
+            int page = x.valid[h] > 0 ? table[at] : 0;
             if (!cache_page_ok(page, a.c.n_pages)) {
               // not read: page 0 stands in, nobody sees its scores
-              valid[h] = page = 0;
+              x.valid[h] = page = 0;
               if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
             }
-            row[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
+            x.row[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
           }
+          return x;
         };
-        auto load_k = [&](int j) {
+        auto load_k = [&](const Block& x) {
           const int st = kc % C::kKSlots;
+          const CUtensorMap* map = x.cached ? &map_k : &map_k_new;
+          const int col = x.cached ? 0 : kvh * DH;
           if (kc >= C::kKSlots && !mbar_wait(k_empty + 8 * st, (kc / C::kKSlots - 1) & 1)) return false;
-          look_up(j);
-          notes[kc % kBlockNotes] = valid[0] | valid[1] << 8;
+          if (storing_k >> st & 1u) store_k(st);
           mbar_expect_tx(k_full + 8 * st, C::kKBytes);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c) {
-              const uint32_t dst = sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128);
-              if (cached) tma_box(dst, &map_k, c * 64, row[h], k_full + 8 * st);
-              else tma_box(dst, &map_k_new, kvh * DH + c * 64, row[h], k_full + 8 * st);
-            }
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_box(sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), map, col + c * 64, x.row[h], k_full + 8 * st);
+          if (x.target[0] >= 0 || x.target[1] >= 0) {
+            storing_k |= 1u << st;
+            to_store[st][0] = x.target[0];
+            to_store[st][1] = x.target[1];
+          }
           ++kc;
           return true;
         };
-        auto load_v = [&](int j) {
-          look_up(j);
+        auto load_v = [&](const Block& x) {
+          const CUtensorMap* map = x.cached ? &map_v : &map_v_new;
+          const int col = x.cached ? 0 : kvh * DH;
           for (int i = 0; i < 2 / C::kVPages; ++i, ++vc) {
             const int st = vc % C::kVSlots;
             if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
+            if (storing_v >> st & 1u) store_v(st);
             mbar_expect_tx(v_full + 8 * st, C::kVBytes);
 #pragma unroll
             for (int h = 0; h < C::kVPages; ++h)
 #pragma unroll
-              for (int c = 0; c < C::kChunks; ++c) {
-                const uint32_t dst = sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128);
-                const int at = row[C::kVPages == 2 ? h : i];
-                if (cached) tma_box(dst, &map_v, c * 64, at, v_full + 8 * st);
-                else tma_box(dst, &map_v_new, kvh * DH + c * 64, at, v_full + 8 * st);
-              }
+              for (int c = 0; c < C::kChunks; ++c)
+                tma_box(sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128), map, col + c * 64,
+                        x.row[C::kVPages == 2 ? h : i], v_full + 8 * st);
+            const int t0 = x.target[C::kVPages == 2 ? 0 : i], t1 = C::kVPages == 2 ? x.target[1] : -1;
+            if (t0 >= 0 || t1 >= 0) {
+              storing_v |= 1u << st;
+              to_store[C::kKSlots + st][0] = t0;
+              to_store[C::kKSlots + st][1] = t1;
+            }
           }
           return true;
         };
-        // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...
-        ok = load_k(0);
+        // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...; the softmax warps' note of a block is written
+        // before the arrival that its products wait for
+        Block now = look_up(0), then;
+        notes[kc % kBlockNotes] = now.valid[0] | now.valid[1] << 8;
+        ok = load_k(now);
         for (int j = 0; ok && j < w.n; ++j) {
-          if (j + 1 < w.n) ok = load_k(j + 1);
-          if (ok) ok = load_v(j);
+          if (j + 1 < w.n) {
+            then = look_up(j + 1);
+            notes[kc % kBlockNotes] = then.valid[0] | then.valid[1] << 8;
+            ok = load_k(then);
+          }
+          if (ok) ok = load_v(now);
+          now = then;
         }
         ++seg;
       } while (ok && w.next(a));
+      // what the last round of slots holds
+      for (int n = max(0, kc - C::kKSlots); ok && n < kc; ++n) {
+        ok = mbar_wait(k_empty + 8 * (n % C::kKSlots), (n / C::kKSlots) & 1);
+        if (ok && (storing_k >> (n % C::kKSlots) & 1u)) store_k(n % C::kKSlots);
+      }
+      for (int n = max(0, vc - C::kVSlots); ok && n < vc; ++n) {
+        ok = mbar_wait(v_empty + 8 * (n % C::kVSlots), (n / C::kVSlots) & 1);
+        if (ok && (storing_v >> (n % C::kVSlots) & 1u)) store_v(n % C::kVSlots);
+      }
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (!ok) atomicOr(&failed, 1u);
     }
   } else if (warp == 9) {
@@ -669,43 +785,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       if (!ok && leader) atomicOr(&failed, 1u);
     }
   } else if (warp >= 10) {
-    // ---- the new rows into their slots, this block's share ----
-    // a warp a token, so that what it has to work out for one is little beside the softmax warps' arithmetic on the same schedulers
-    if (a.c.k_new_dev) {
-      const int vecs = a.c.kv_heads * (DH / 8), stride = a.c.kv_heads * kPageTokens * (DH / 8);
-      const int rows = a.c.batch * a.c.tokens;
-      for (int row = blockIdx.x * (kCopyThreads / 32) + warp - 10; row < rows; row += kPieces * (kCopyThreads / 32)) {
-        const int b = row / a.c.tokens, t = row - b * a.c.tokens;
-        const CacheSeq s = prompt_seq(a, b);
-        if (t >= s.fresh) continue;
-        const int slot = s.length - s.fresh + t, page = a.c.page_table_dev[static_cast<size_t>(b) * a.c.pages + slot / kPageTokens];
-        if (!cache_page_ok(page, a.c.n_pages)) {
-          if (lane == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
-          continue;
-        }
-        const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.c.k_new_dev) + static_cast<size_t>(row) * a.c.ld_k;
-        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v_new_dev) + static_cast<size_t>(row) * a.c.ld_v;
-        const size_t at = static_cast<size_t>(page) * stride + slot % kPageTokens * (DH / 8);
-        constexpr int kFlight = 4;
-        for (int i = lane; i < vecs; i += 32 * kFlight) {
-          uint4 xk[kFlight], xv[kFlight];
-#pragma unroll
-          for (int f = 0; f < kFlight; ++f)
-            if (i + 32 * f < vecs) {
-              xk[f] = load8_bf16(k + (i + 32 * f) * 8);
-              xv[f] = load8_bf16(v + (i + 32 * f) * 8);
-            }
-#pragma unroll
-          for (int f = 0; f < kFlight; ++f)
-            if (i + 32 * f < vecs) {
-              const int e = i + 32 * f;
-              const size_t to = at + static_cast<size_t>(e / (DH / 8)) * (kPageTokens * (DH / 8)) + e % (DH / 8);
-              static_cast<uint4*>(a.c.kpool_dev)[to] = xk[f];
-              static_cast<uint4*>(a.c.vpool_dev)[to] = xv[f];
-            }
-        }
-      }
-    }
+    // ---- the new rows into their slots ----
+    if (a.c.k_new_dev) store_rows<DH>(a, warp - 10);
   }
   } else {
     // ---- weights ----
@@ -874,6 +955,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     } while (w.next(a));
     if (!ok) atomicOr(&failed, 1u);
     }
+    if (a.c.k_new_dev) store_rows<DH>(a, 2 + warp);
   }
   fence_before();
   __syncthreads();
