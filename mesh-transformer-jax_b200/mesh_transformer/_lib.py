@@ -45,6 +45,8 @@ class MtjStackDesc(ctypes.Structure):
                 + [("act_f32", ctypes.c_int32), ("tc_min_rows", ctypes.c_int32)])
 
 
+# Arguments of the calls over caller-owned caches and of the verification of drafts, passed by address: an instance of these (by
+# reference) or the same bytes.
 class MtjCacheAttnArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in (
         "kpool", "vpool", "page_table", "lengths", "new_tokens", "status", "q", "k_new", "v_new", "out", "weights_in",
@@ -124,11 +126,11 @@ def _load():
         "mtj_k_prefill_attn": (i32, [vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp]),
         "mtj_k_all_reduce_buffer_bytes": (i64, [vp, i32]),
         "mtj_k_all_reduce": (i32, [vp, ctypes.POINTER(vp), i32, i32, i32, i32, vp, vp, vp, i32, vp]),
-        "mtj_k_cache_attn_scratch_bytes": (i64, [ctypes.POINTER(MtjCacheAttnArgs)]),
-        "mtj_k_cache_attn": (i32, [ctypes.POINTER(MtjCacheAttnArgs), vp, i64, vp]),
-        "mtj_k_cache_evict": (i32, [ctypes.POINTER(MtjCacheEvictArgs), vp]),
-        "mtj_verify_scratch_bytes": (i64, [ctypes.POINTER(MtjVerifyArgs)]),
-        "mtj_verify_drafts": (i32, [ctypes.POINTER(MtjVerifyArgs), vp, i64, vp]),
+        "mtj_k_cache_attn_scratch_bytes": (i64, [vp]),
+        "mtj_k_cache_attn": (i32, [vp, vp, i64, vp]),
+        "mtj_k_cache_evict": (i32, [vp, vp]),
+        "mtj_verify_scratch_bytes": (i64, [vp]),
+        "mtj_verify_drafts": (i32, [vp, vp, i64, vp]),
         "mtj_k_decode_attn": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64, vp, i32, vp]),
     }
     partial = not LIB_PATH.endswith("libmtj_b200.so")

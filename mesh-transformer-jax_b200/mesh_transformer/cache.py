@@ -9,18 +9,19 @@ reads nothing back, and can be captured into a CUDA graph.  Nothing here records
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
-from ._lib import MTJ_BF16, MTJ_F32, MtjCacheAttnArgs, MtjCacheEvictArgs, check, lib
+from ._lib import MTJ_BF16, MTJ_F32, check, lib
 
 PAGE_TOKENS = 64
 _DTYPES = {torch.bfloat16: MTJ_BF16, torch.float32: MTJ_F32}
-
-
-def _stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+# mtj_cache_attn_args and mtj_cache_evict_args as the C side lays them out (the fields of MtjCacheAttnArgs, MtjCacheEvictArgs): a
+# token's call is launched in a few microseconds, of which filling a ctypes structure would be a quarter
+_ATTN_ARGS = struct.Struct("@12P4q10if4x").pack
+_EVICT_ARGS = struct.Struct("@11P8i").pack
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _want(t, name, dtype, shape, device):
@@ -41,20 +42,24 @@ def _pool_shape(kpool, vpool, page_table, lengths):
     return shape, table, device
 
 
-def _rows(t, name, heads, d_head, like):
+def _rows(t, name, shape, like):
     """``t`` [batch, tokens, heads, d_head] with heads side by side in a row, rows at one stride and 16-byte aligned (a slice
     of a fused projection is one); anything else is copied."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or \
-            t.shape[:2] != like.shape[:2] or t.shape[2] != heads or t.shape[3] != d_head:
-        raise ValueError(f"{name} must be a {like.dtype} tensor {[*like.shape[:2], heads, d_head]} on {like.device}")
-    s = t.stride()
-    if t.is_contiguous() and not t.data_ptr() & 15:
-        return t, heads * d_head
-    ld = s[1] if t.shape[1] > 1 else s[0] if t.shape[0] > 1 else heads * d_head
-    if s[3] == 1 and (s[2] == d_head or heads == 1) and ld >= heads * d_head and not ld & 7 and not t.data_ptr() & 15 and \
-            (t.shape[0] == 1 or s[0] == ld * t.shape[1]):
-        return t, ld
-    return t.contiguous() if not t.is_contiguous() else t.clone(), heads * d_head
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise ValueError(f"{name} must be a {like.dtype} tensor {list(shape)} on {like.device}")
+    at = t.data_ptr()
+    if t.is_contiguous():
+        if at & 15:
+            t = t.clone()
+            at = t.data_ptr()
+        return t, at, shape[2] * shape[3]
+    s, (batch, tokens, heads, d_head) = t.stride(), shape
+    ld = s[1] if tokens > 1 else s[0] if batch > 1 else heads * d_head
+    if s[3] == 1 and (s[2] == d_head or heads == 1) and ld >= heads * d_head and not ld & 7 and not at & 15 and \
+            (batch == 1 or s[0] == ld * tokens):
+        return t, at, ld
+    t = t.contiguous()
+    return t, t.data_ptr(), heads * d_head
 
 
 def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window=None, sinks=0, scale=None, weights=None,
@@ -73,43 +78,55 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
 
     ``status`` int32 [1], if given, collects what the GPU found wrong: bit 1 a length or a page number outside the cache (that
     sequence counts as empty, that page as unseen), bit 0 a wait that ran out."""
-    (n_pages, kv_heads, _, d_head), (batch, pages), device = _pool_shape(kpool, vpool, page_table, lengths)
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES or q.device != device or q.shape[0] != batch or \
-            q.shape[3] != d_head or q.shape[1] < 1 or q.shape[2] < 1:
+    pool, table, device = _pool_shape(kpool, vpool, page_table, lengths)
+    n_pages, kv_heads, _, d_head = pool
+    batch, pages = table
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES or q.device != device:
         raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
-    tokens, heads = q.shape[1:3]
-    if (k is None) != (v is None):
+    shape = q.shape
+    tokens, heads = shape[1], shape[2]
+    if shape[0] != batch or shape[3] != d_head or tokens < 1 or heads < 1:
+        raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
+    dtype = _DTYPES[q.dtype]
+    q, at_q, ld_q = _rows(q, "q", shape, q)
+    at_k = at_v = ld_k = ld_v = 0
+    if k is not None and v is not None:
+        new_shape = (batch, tokens, kv_heads, d_head)
+        k, at_k, ld_k = _rows(k, "k", new_shape, q)
+        v, at_v, ld_v = _rows(v, "v", new_shape, q)
+    elif k is not None or v is not None:
         raise ValueError("k and v come together")
-    q, ld_q = _rows(q, "q", heads, d_head, q)
-    ld_k = ld_v = 0
-    if k is not None:
-        k, ld_k = _rows(k, "k", kv_heads, d_head, q)
-        v, ld_v = _rows(v, "v", kv_heads, d_head, q)
+    at_new = at_status = at_in = at_out = 0
     if new is not None:
-        _want(new, "new", torch.int32, lengths.shape, device)
+        _want(new, "new", torch.int32, (batch,), device)
+        at_new = new.data_ptr()
     if status is not None:
         _want(status, "status", torch.int32, (1,), device)
+        at_status = status.data_ptr()
     if weights is not None or weights_out is not None:
         if weights_out is None:
             weights_out = weights
-        _want(weights_out, "weights_out", torch.float32, (batch, kv_heads, pages * PAGE_TOKENS), device)
-        if weights is not None and weights is not weights_out:
-            _want(weights, "weights", torch.float32, weights_out.shape, device)
+        slots = (batch, kv_heads, pages * PAGE_TOKENS)
+        _want(weights_out, "weights_out", torch.float32, slots, device)
+        at_out = weights_out.data_ptr()
+        if weights is not None:
+            _want(weights, "weights", torch.float32, slots, device)
+            at_in = weights.data_ptr()
     if out is None:
-        out = torch.empty((batch, tokens, heads, d_head), dtype=q.dtype, device=device)
-        ld_out = heads * d_head
+        out = torch.empty(shape, dtype=q.dtype, device=device)
+        at, ld_out = out.data_ptr(), heads * d_head
     else:
         given = out
-        out, ld_out = _rows(out, "out", heads, d_head, q)
+        out, at, ld_out = _rows(out, "out", shape, q)
         if out is not given:
             raise ValueError("out must have its heads side by side, rows at one stride and a 16-byte alignment")
-    a = MtjCacheAttnArgs(
-        kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), new.data_ptr() if new is not None else None,
-        status.data_ptr() if status is not None else None, q.data_ptr(), k.data_ptr() if k is not None else None,
-        v.data_ptr() if k is not None else None, out.data_ptr(), weights.data_ptr() if weights is not None else None,
-        weights_out.data_ptr() if weights_out is not None else None, ld_q, ld_k, ld_v, ld_out, n_pages, batch, pages, heads,
-        kv_heads, d_head, tokens, _DTYPES[q.dtype], pages * PAGE_TOKENS if window is None else min(int(window), 0x7fffffff),
-        min(int(sinks), 0x7fffffff), d_head ** -0.5 if scale is None else scale)
+    try:
+        a = _ATTN_ARGS(kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), at_new, at_status, at_q, at_k, at_v, at,
+                       at_in, at_out, ld_q, ld_k, ld_v, ld_out, n_pages, batch, pages, heads, kv_heads, d_head, tokens, dtype,
+                       pages * PAGE_TOKENS if window is None else min(window, 0x7fffffff), min(sinks, 0x7fffffff),
+                       d_head ** -0.5 if scale is None else scale)
+    except (struct.error, OverflowError, TypeError) as e:
+        raise ValueError(f"window and sinks must be whole numbers, scale a number: {e}") from None
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
@@ -120,12 +137,11 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
 
 
 def _run_attention(a, device, index):
-    ref = ctypes.byref(a)
-    nbytes = lib.mtj_k_cache_attn_scratch_bytes(ref)
+    nbytes = lib.mtj_k_cache_attn_scratch_bytes(a)
     if nbytes < 0:
         raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
-    check(lib.mtj_k_cache_attn(ref, scratch.data_ptr(), nbytes, _stream(index)))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    check(lib.mtj_k_cache_attn(a, scratch.data_ptr(), nbytes, _stream(index)))
 
 
 def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, first=0, last=0, status=None):
@@ -147,14 +163,14 @@ def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, f
         _want(status, "status", torch.int32, (1,), device)
     kept = torch.empty((batch, kv_heads, keep), dtype=torch.int32, device=device)
     lengths_out, weights_out, table_out = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(page_table)
-    a = MtjCacheEvictArgs(
+    a = _EVICT_ARGS(
         kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), weights.data_ptr(), spare_pages.data_ptr(),
         kept.data_ptr(), lengths_out.data_ptr(), weights_out.data_ptr(), table_out.data_ptr(),
-        status.data_ptr() if status is not None else None, n_pages, batch, pages, kv_heads, d_head, keep, first, last)
+        status.data_ptr() if status is not None else 0, n_pages, batch, pages, kv_heads, d_head, keep, first, last)
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            check(lib.mtj_k_cache_evict(ctypes.byref(a), _stream(index)))
+            check(lib.mtj_k_cache_evict(a, _stream(index)))
     else:
-        check(lib.mtj_k_cache_evict(ctypes.byref(a), _stream(index)))
+        check(lib.mtj_k_cache_evict(a, _stream(index)))
     return kept, lengths_out, weights_out, table_out

@@ -11,12 +11,12 @@ the kernel's own selection); the top-k branch of the reference filter
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import numpy as np
 import torch
 
-from ._lib import MTJ_BF16, MTJ_F32, MtjVerifyArgs, check, lib
+from ._lib import MTJ_BF16, MTJ_F32, check, lib
 
 TINY = float(np.finfo(np.float32).tiny)
 
@@ -98,6 +98,7 @@ def nucleaus_filter(logits, top_p=0.9, top_k=None):
 
 
 _LOGIT_TYPES = {torch.float32: MTJ_F32, torch.bfloat16: MTJ_BF16}
+_VERIFY_ARGS = struct.Struct("@10P4q4if4x").pack           # mtj_verify_args, the fields of MtjVerifyArgs
 
 
 def _logit_rows(t, name, like, rows):
@@ -153,10 +154,10 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
     out = torch.empty((batch, rows), dtype=torch.int32, device=dev)
     taken = torch.empty((batch,), dtype=torch.int32, device=dev)
     logprobs = torch.empty((batch, rows), dtype=torch.float32, device=dev)
-    a = MtjVerifyArgs(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else None, tokens.data_ptr(),
-                      accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else None,
-                      temps.data_ptr() if temps is not None else None, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
-                      ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
+    a = _VERIFY_ARGS(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else 0, tokens.data_ptr(),
+                     accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else 0,
+                     temps.data_ptr() if temps is not None else 0, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
+                     ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev.index):
             _run_verify(a, dev)
@@ -166,9 +167,8 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
 
 
 def _run_verify(a, dev):
-    ref = ctypes.byref(a)
-    nbytes = lib.mtj_verify_scratch_bytes(ref)
+    nbytes = lib.mtj_verify_scratch_bytes(a)
     if nbytes < 0:
         raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
     scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    check(lib.mtj_verify_drafts(ref, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev.index)))
+    check(lib.mtj_verify_drafts(a, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev.index)))

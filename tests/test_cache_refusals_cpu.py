@@ -120,3 +120,15 @@ def test_host_layer_wants_tensors_of_one_gpu(L):
         cache_evict(pool, pool, table, lengths, torch.zeros((1, 2, 128)), table[:, :1], 64)
     with pytest.raises(ValueError):
         verify_drafts(torch.zeros((1, 2, 10)), None, torch.zeros((1, 1), dtype=torch.int32), torch.zeros((1, 1)), torch.zeros((1, 10)))
+
+
+def test_packed_arguments_are_laid_out_as_the_structures(L):
+    """The host layer packs the arguments itself: same size, and every field at its place."""
+    import struct
+    for cls, fmt in ((L.MtjCacheAttnArgs, "@12P4q10if4x"), (L.MtjCacheEvictArgs, "@11P8i"), (L.MtjVerifyArgs, "@10P4q4if4x")):
+        assert struct.calcsize(fmt) == ctypes.sizeof(cls)
+        values = [i + 1 for i in range(len(cls._fields_))]
+        back = cls.from_buffer_copy(struct.pack(fmt, *values))
+        assert [getattr(back, n) for n, _ in cls._fields_] == values
+    src = open(__import__("mesh_transformer.cache", fromlist=["x"]).__file__).read() + open(__import__("mesh_transformer.sampling", fromlist=["x"]).__file__).read()
+    assert all(f'"{fmt}"' in src for fmt in ("@12P4q10if4x", "@11P8i", "@10P4q4if4x"))
