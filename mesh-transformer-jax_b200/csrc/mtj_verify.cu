@@ -1,16 +1,19 @@
 // Verification of drafted tokens against the target model's logits (mtj_verify_drafts).
 //
-// verify_rows_kernel: every row of logits that takes part is read once, in chunks of kChunk entries, one block each: the
-//   chunk's maximum (and where it first stands) and the sum of exp((l - maximum) / temp).  A thread holds its entries in
-//   registers, so the maximum is known before the first exponential.
+// verify_rows_kernel: every row of logits that takes part is read once, kChunk entries a warp at a time: their maximum (greedy: and where it
+//   first stands) and the sum of exp((l - maximum) / temp).  A lane holds its entries in registers, so the maximum is known before
+//   the first exponential, and has the next ones on their way meanwhile.  The rows that take part stand in one line that is cut into
+//   equal pieces, one a warp: rows behind a sequence's drafts cost nothing.
 // verify_pick_kernel: a cluster of blocks a sequence.  Every block joins the chunks of all rows to shares, in 64 bits, and
 //   decides alike how many drafts are taken; then the cluster shares out the one row that the next token comes from.
 //   The race r_i / -log(noise_i) is run in 32 bits with a bound on the error of every entry; those that can win it are run
-//   again in 64 bits, so that the token does not hang on the rounding of a near-tie or of a difference of near-equal shares.
+//   again in 64 bits, so that the token does not hang on the rounding of a near-tie or of a difference of near-equal shares.  What does
+//   not hang on the rows kernel (noise, the drafts' own logits) is read and worked out while that one runs.
 //
 // Bound by the bytes of the logits: 32-bit sums of exponentials of a chunk, 64-bit sums over chunks.
 #include <math.h>
 
+#include <algorithm>
 #include <string>
 
 #include "mtj_cache.cuh"
@@ -19,16 +22,21 @@
 namespace mtj {
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr int kPerThread = 16;
-constexpr int kChunk = kRowThreads * kPerThread;
+constexpr int kRowThreads = 768;
+constexpr int kPerLane = 32;
+constexpr int kChunk = 32 * kPerLane;
+constexpr int kRowBlocks = 148;            // one an SM
+constexpr int kRowBatch = 4096;            // sequences of a launch
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickCluster = 8;
+constexpr int kHeld = 16;                  // entries of the race that a thread has at once
+constexpr float kLowestTemp = 8.673617e-19f;      // 2^-60
+constexpr float kLog2e = 1.442695041f;
 
 struct ChunkStat {
   float top, sum;      // largest entry; sum of exp((l - top) / temp) over the chunk
-  int32_t at, pad;     // where it first stands
+  int32_t at, pad;     // where it first stands (greedy)
 };
 
 __device__ __forceinline__ float value_at(const float* p, int i) { return p[i]; }
@@ -38,20 +46,20 @@ __device__ __forceinline__ int drafts_of(const mtj_verify_args& a, int b) {
   return a.counts_dev ? min(max(a.counts_dev[b], 0), a.drafts) : a.drafts;
 }
 __device__ __forceinline__ float temp_of(const mtj_verify_args& a, int b) { return a.temp_dev ? a.temp_dev[b] : a.temp; }
+// no temperature (nor one so low that scaled logits leave 32 bits): the largest logit has it all
+__device__ __forceinline__ bool is_greedy(float temp) { return !(temp >= kLowestTemp); }
 
-// exp((l - top) / temp) = 2^((l - top) * scale), the scale as the sum of two numbers so that its rounding does not lean on every entry
-struct ExpScale {
-  float hi, lo;
-  __device__ __forceinline__ explicit ExpScale(float temp) {
-    const double c = 1.4426950408889634074 / static_cast<double>(temp);
-    hi = static_cast<float>(c);
-    lo = isfinite(hi) ? static_cast<float>(c - static_cast<double>(hi)) : 0.f;
-  }
-  __device__ __forceinline__ float operator()(float l, float top) const {
-    const float d = fmaxf(l - top, -1e30f);      // -inf (and NaN): a finite number whose products cannot cancel
-    return d == 0.f ? 1.f : exp2f(fmaf(d, hi, d * lo));
-  }
-};
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void untwo(uint64_t d, float* x, float* y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*x), "=f"(*y) : "l"(d)); }
 
 // rows of one sequence: 0 .. drafts the target's, then the draft's
 template <typename T>
@@ -59,85 +67,192 @@ __device__ __forceinline__ const T* row_of(const mtj_verify_args& a, int b, int 
   return r <= a.drafts ? static_cast<const T*>(a.target_dev) + b * a.batch_target + r * a.ld_target
                        : static_cast<const T*>(a.draft_dev) + b * a.batch_draft + (r - a.drafts - 1) * a.ld_draft;
 }
+// how many of them take part: the target's 0 .. n, the draft's 0 .. n - 1 where the target does not choose by itself
+__device__ __forceinline__ int rows_in(const mtj_verify_args& a, int b) {
+  const int n = drafts_of(a, b);
+  return n + 1 + (a.draft_dev && !is_greedy(temp_of(a, b)) ? n : 0);
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const mtj_verify_args a, ChunkStat* stats, int rows, int chunks) {
-  const int c = blockIdx.x % chunks, r = blockIdx.x / chunks % rows, b = blockIdx.x / chunks / rows;
+__global__ void __launch_bounds__(kRowThreads, 1) verify_rows_kernel(const mtj_verify_args a, ChunkStat* stats, int rows, int chunks) {
+  constexpr int kVec = 16 / sizeof(T), kLoads = kPerLane / kVec;
+  __shared__ int before[kRowBatch + 1], scan[kRowThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ float sm_top[kRowThreads / 32], sm_sum[kRowThreads / 32];
-  __shared__ int sm_at[kRowThreads / 32];
   pdl_launch_dependents();
-  const int n = drafts_of(a, b);
-  const float temp = temp_of(a, b);
-  const bool greedy = !(temp > 0.f);
-  if (r <= a.drafts ? r > n : (r - a.drafts - 1 >= n || greedy)) return;      // this row takes no part
-  const T* row = row_of<T>(a, b, r);
-  constexpr int kVec = 16 / sizeof(T);
-  // chunks begin at 16-byte boundaries: `skew` entries before the row's first one
-  const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-  float v[kPerThread];
-  float top = -INFINITY;
-  int at = 0x7fffffff;
+  // before[b]: rows of the line before sequence b
+  {
+    const int per = (a.batch + kRowThreads - 1) / kRowThreads, b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += before[b] = rows_in(a, b);
+    int x = sum;
 #pragma unroll
-  for (int u = 0; u < kPerThread / kVec; ++u) {
-    const int i0 = c * kChunk + (u * kRowThreads + tid) * kVec - skew;
-    float* w = v + u * kVec;
-    if (i0 >= 0 && i0 + kVec <= a.vocab) {
-      const uint4 x = ld_cached16(row + i0);
-      if constexpr (sizeof(T) == 2) {
-        unpack8(x, w);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    x -= sum;
+    int all = 0;
+    for (int w = 0; w < kRowThreads / 32; ++w) {
+      if (w < warp) x += scan[w];
+      all += scan[w];
+    }
+    for (int b = b0; b < b1; ++b) {
+      const int n = before[b];
+      before[b] = x;
+      x += n;
+    }
+    if (tid == 0) before[a.batch] = all;
+    __syncthreads();
+  }
+  const int64_t line = static_cast<int64_t>(before[a.batch]) * chunks;
+  // pieces are dealt out block by block, so that a short line has all SMs
+  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x, workers = static_cast<int64_t>(gridDim.x) * (kRowThreads / 32);
+  const int64_t begin = line * worker / workers, end = line * (worker + 1) / workers;
+
+  // where this warp is in the line; the next chunk is looked up while the last one's entries are worked on
+  struct Place {
+    int b, k, c, n, rows;      // sequence, row and chunk of it; drafted tokens, rows that take part
+  } at = {};
+  struct Item {
+    const T* row;
+    ChunkStat* out;
+    int i0;                    // first entry: chunks begin at 16-byte boundaries, up to a vector before the row's first entry
+    float temp;
+  };
+  auto enter = [&]() {
+    at.n = drafts_of(a, at.b);
+    at.rows = before[at.b + 1] - before[at.b];
+  };
+  auto item = [&]() {
+    const int r = at.k <= at.n ? at.k : a.drafts + at.k - at.n;
+    Item it;
+    it.row = row_of<T>(a, at.b, r);
+    it.out = stats + (static_cast<int64_t>(at.b) * rows + r) * chunks + at.c;
+    it.i0 = at.c * kChunk - static_cast<int>((reinterpret_cast<uintptr_t>(it.row) & 15) / sizeof(T));
+    it.temp = temp_of(a, at.b);
+    return it;
+  };
+  auto step = [&]() {
+    if (++at.c < chunks) return;
+    at.c = 0;
+    if (++at.k < at.rows) return;
+    at.k = 0;
+    ++at.b;                    // every sequence has a row
+    enter();
+  };
+  auto fetch = [&](const Item& it, uint4* x) {
+    if (it.i0 >= 0 && it.i0 + kChunk <= a.vocab) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) x[u] = ld_cached16(it.row + it.i0 + (u * 32 + lane) * kVec);
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      // a row's ends
+      const int i = it.i0 + (u * 32 + lane) * kVec;
+      float v[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = i + e >= 0 && i + e < a.vocab ? value_at(it.row, i + e) : -INFINITY;
+      if constexpr (sizeof(T) == 4)
+        x[u] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        x[u] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4 % kVec], v[5 % kVec]), pack_bf16x2(v[6 % kVec], v[7 % kVec]));
+    }
+  };
+  auto entry = [&](const uint4* x, int u, int e) {
+    const int word = e * static_cast<int>(sizeof(T)) >> 2;
+    const uint32_t w = word == 0 ? x[u].x : word == 1 ? x[u].y : word == 2 ? x[u].z : x[u].w;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else return e & 1 ? bf16_hi(w) : bf16_lo(w);
+  };
+  auto work = [&](const Item& it, const uint4* x) {
+    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int e = 0; e < kVec; e += 4) {
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(t0) : "f"(entry(x, u, e)), "f"(entry(x, u, e + 1)));
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(t1) : "f"(entry(x, u, e + 2)), "f"(entry(x, u, e + 3)));
+      }
+    const float top = warp_max(fmaxf(t0, t1));
+    int where = 0x7fffffff;
+    float sum = 0.f;
+    if (is_greedy(it.temp)) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (entry(x, u, e) == top) where = min(where, it.i0 + (u * 32 + lane) * kVec + e);
+      where = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(where)));
+    } else if (top > -INFINITY) {
+      // 2^(l scale - base), and the rounding of base = top scale taken out of the sum
+      const float scale = kLog2e / it.temp, base = top * scale;
+      if (fabsf(base) < 1e30f) {
+        const uint64_t scale2 = two(scale, scale), base2 = two(-base, -base);
+        uint64_t s0 = 0, s1 = 0;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+          for (int e = 0; e < kVec; e += 4) {
+            uint64_t y0, y1;
+            float f0, f1, f2, f3;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y0) : "l"(two(entry(x, u, e), entry(x, u, e + 1))), "l"(scale2), "l"(base2));
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y1) : "l"(two(entry(x, u, e + 2), entry(x, u, e + 3))), "l"(scale2), "l"(base2));
+            untwo(y0, &f0, &f1);
+            untwo(y1, &f2, &f3);
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s0) : "l"(two(ex2(f0), ex2(f1))));
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s1) : "l"(two(ex2(f2), ex2(f3))));
+          }
+        float f0, f1, f2, f3;
+        untwo(s0, &f0, &f1);
+        untwo(s1, &f2, &f3);
+        sum = (f0 + f1) + (f2 + f3);
+        sum = fmaf(-0.6931472f * fmaf(top, scale, -base), sum, sum);
       } else {
-        w[0] = __uint_as_float(x.x);
-        w[1] = __uint_as_float(x.y);
-        w[2] = __uint_as_float(x.z);
-        w[3] = __uint_as_float(x.w);
+        // a largest logit at the end of the type's range
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) sum += ex2(fmaxf(entry(x, u, e) - top, -1e30f) * fminf(scale, 1e8f));
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) w[e] = i0 + e >= 0 && i0 + e < a.vocab ? value_at(row, i0 + e) : -INFINITY;
+      sum = warp_sum(sum);
     }
-#pragma unroll
-    for (int e = 0; e < kVec; ++e)
-      if (w[e] > top) {
-        top = w[e];
-        at = i0 + e;
-      }
-  }
-  // the block's maximum, at its lowest place
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-    if (t2 > top || (t2 == top && a2 < at)) {
-      top = t2;
-      at = a2;
+    if (lane == 0) *it.out = {top, sum, where, 0};
+  };
+  if (begin >= end) return;
+  {
+    const int64_t line_row = begin / chunks;
+    at.c = static_cast<int>(begin - line_row * chunks);
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before[mid] <= line_row) lo = mid;
+      else hi = mid - 1;
     }
+    at.b = lo;
+    at.k = static_cast<int>(line_row) - before[lo];
+    enter();
   }
-  if (lane == 0) {
-    sm_top[warp] = top;
-    sm_at[warp] = at;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kRowThreads / 32; ++w)
-    if (sm_top[w] > top || (sm_top[w] == top && sm_at[w] < at)) {
-      top = sm_top[w];
-      at = sm_at[w];
+  uint4 x[2][kLoads];
+  Item it[2];
+  it[0] = item();
+  fetch(it[0], x[0]);
+  for (int64_t i = begin; i < end; i += 2) {
+    if (i + 1 < end) {
+      step();
+      it[1] = item();
+      fetch(it[1], x[1]);
     }
-  float sum = 0.f;
-  if (!greedy && top > -INFINITY) {
-    const ExpScale e(temp);
-#pragma unroll
-    for (int u = 0; u < kPerThread; ++u) sum += e(v[u], top);
-  }
-  sum = warp_sum(sum);
-  if (lane == 0) sm_sum[warp] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowThreads / 32; ++w) sum += sm_sum[w];
-    stats[blockIdx.x] = {top, sum, at, 0};
+    work(it[0], x[0]);
+    if (i + 1 >= end) break;
+    if (i + 2 < end) {
+      step();
+      it[0] = item();
+      fetch(it[0], x[0]);
+    }
+    work(it[1], x[1]);
   }
 }
 
@@ -145,11 +260,12 @@ struct RowShare {
   float top;           // largest logit of the row
   int at;              // its first place
   double sum;          // sum of exp((l - top) / temp)
+  double log_sum;
 };
 
 // log of the share of logit l in a row
 __device__ __forceinline__ double log_share(const RowShare& s, float l, double temp) {
-  return (static_cast<double>(l) - static_cast<double>(s.top)) / temp - log(s.sum);
+  return (static_cast<double>(l) - static_cast<double>(s.top)) / temp - s.log_sum;
 }
 __device__ __forceinline__ double share(const RowShare& s, float l, double temp) {
   return l == s.top ? 1.0 / s.sum : exp((static_cast<double>(l) - static_cast<double>(s.top)) / temp) / s.sum;
@@ -174,48 +290,68 @@ __device__ __forceinline__ uint32_t pick_rank() {
 __device__ __forceinline__ void pick_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-template <typename V>
-__device__ __forceinline__ V peer_value(const V* p, uint32_t rank) {
-  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "one register or a pair");
+__device__ __forceinline__ void put_to_first(Racer* slot, const Racer& x) {
   uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  V v;
-  if constexpr (sizeof(V) == 4) {
-    uint32_t x;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
-    memcpy(&v, &x, 4);
-  } else {
-    unsigned long long x;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
-    memcpy(&v, &x, 8);
-  }
-  return v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(slot)));
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(x.score) : "memory");
+  asm volatile("st.shared::cluster.u32 [%0 + 8], %1;" ::"r"(at), "r"(x.at) : "memory");
 }
 
+// Blocks of a cluster a sequence: as many as keep two an SM, up to eight.
 template <typename T>
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const mtj_verify_args a, const ChunkStat* stats, int rows, int chunks,
+__global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_verify_args a, const ChunkStat* stats, int rows, int chunks,
                                                                    int cluster) {
   extern __shared__ RowShare row_share[];          // [rows]
-  __shared__ float sm_best[kPickWarps], s_best;
-  __shared__ double sm_score[kPickWarps], s_score;
-  __shared__ int sm_at[kPickWarps], s_at, s_taken;
+  __shared__ float sm_best[kPickWarps];
+  __shared__ Racer sm_win[kPickWarps], racers[kPickCluster];      // of the warps; in the first block, of the blocks
+  __shared__ int s_taken;
   const int b = blockIdx.x / cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = pick_rank();
   const int n = drafts_of(a, b), n_out = a.drafts + 1;
   const float temp = temp_of(a, b);
-  const bool greedy = !(temp > 0.f);
+  const bool greedy = is_greedy(temp);
   const int32_t* tokens = a.draft_tokens_dev + static_cast<size_t>(b) * a.drafts;
+  const float* noise = a.noise_dev + static_cast<size_t>(b) * a.vocab;
+  const int per = (a.vocab + cluster - 1) / cluster;
+  const int i0 = static_cast<int>(rank) * per, i1 = min(a.vocab, i0 + per);
+  pick_sync();                                     // all blocks of the cluster are there: the first one's memory may be written
+
+  // before the rows kernel has ended: the drafts' own entries (the first 32), the noise
+  int x0 = -1;
+  float p0 = 0.f, q0 = 0.f, u0 = 0.f, wait_of[kHeld];
+  if (warp == 0 && lane < n) {
+    x0 = tokens[lane];
+    if (x0 < 0 || x0 >= a.vocab) x0 = -1;
+    if (x0 >= 0 && !greedy) {
+      p0 = value_at(row_of<T>(a, b, lane), x0);
+      if (a.draft_dev) q0 = value_at(row_of<T>(a, b, a.drafts + 1 + lane), x0);
+      u0 = a.accept_dev[static_cast<size_t>(b) * a.drafts + lane];
+    }
+  }
+  auto fetch_noise = [&](int first) {
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+      const int i = first + h * kPickThreads + tid;
+      wait_of[h] = i < i1 ? noise[i] : 0.5f;
+    }
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) wait_of[h] = -logf(wait_of[h]);
+  };
+  if (!greedy) fetch_noise(i0);
   pdl_wait();
+  const double t64 = greedy ? 1.0 : static_cast<double>(temp);
   for (int r = warp; r < rows; r += kPickWarps) {
     if (r <= a.drafts ? r > n : (r - a.drafts - 1 >= n || greedy)) continue;
-    const ChunkStat* st = stats + (static_cast<size_t>(b) * rows + r) * chunks;
+    const ChunkStat* st = stats + (static_cast<int64_t>(b) * rows + r) * chunks;
     float top = -INFINITY;
     int at = 0x7fffffff;
-    for (int c = lane; c < chunks; c += 32)
-      if (st[c].top > top) {
-        top = st[c].top;
-        at = st[c].at;
+    for (int c = lane; c < chunks; c += 32) {
+      const ChunkStat s = st[c];
+      if (s.top > top) {
+        top = s.top;
+        at = s.at;
       }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
@@ -227,30 +363,38 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const mtj_ver
     }
     double sum = 0.0;
     if (!greedy)
-      for (int c = lane; c < chunks; c += 32)
-        if (st[c].top > -INFINITY)
-          sum += static_cast<double>(st[c].sum) *
-                 (st[c].top == top ? 1.0 : exp((static_cast<double>(st[c].top) - static_cast<double>(top)) / static_cast<double>(temp)));
+      for (int c = lane; c < chunks; c += 32) {
+        const ChunkStat s = st[c];
+        if (s.top > -INFINITY)
+          sum += static_cast<double>(s.sum) * (s.top == top ? 1.0 : exp((static_cast<double>(s.top) - static_cast<double>(top)) / t64));
+      }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) row_share[r] = {top, top > -INFINITY ? at : 0, sum};
+    if (lane == 0) row_share[r] = {top, greedy && top > -INFINITY ? at : 0, sum, greedy ? 0.0 : log(sum)};
   }
   __syncthreads();
-  const double t64 = greedy ? 1.0 : static_cast<double>(temp);
   if (warp == 0) {
     int taken = 0;
     for (int k0 = 0; k0 < n && taken == k0; k0 += 32) {
       const int k = k0 + lane;
       bool good = false;
       if (k < n) {
-        const int x = tokens[k];
-        if (x >= 0 && x < a.vocab) {
+        if (k0 > 0) {
+          x0 = tokens[k];
+          if (x0 < 0 || x0 >= a.vocab) x0 = -1;
+          if (x0 >= 0 && !greedy) {
+            p0 = value_at(row_of<T>(a, b, k), x0);
+            if (a.draft_dev) q0 = value_at(row_of<T>(a, b, a.drafts + 1 + k), x0);
+            u0 = a.accept_dev[static_cast<size_t>(b) * a.drafts + k];
+          }
+        }
+        if (x0 >= 0) {
           if (greedy) {
-            good = x == row_share[k].at;
+            good = x0 == row_share[k].at;
           } else {
-            const double p = share(row_share[k], value_at(row_of<T>(a, b, k), x), t64);
-            const double q = a.draft_dev ? share(row_share[a.drafts + 1 + k], value_at(row_of<T>(a, b, a.drafts + 1 + k), x), t64) : 1.0;
-            good = static_cast<double>(a.accept_dev[static_cast<size_t>(b) * a.drafts + k]) * q < p;
+            const double p = share(row_share[k], p0, t64);
+            const double q = a.draft_dev ? share(row_share[a.drafts + 1 + k], q0, t64) : 1.0;
+            good = static_cast<double>(u0) * q < p;
           }
         }
       }
@@ -272,72 +416,79 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const mtj_ver
     const T* qrow = known ? row_of<T>(a, b, a.drafts + 1 + taken) : prow;
     const RowShare qs = known ? row_share[a.drafts + 1 + taken] : ps;
     const int without = refused && !known ? tokens[taken] : -1;
-    const float* noise = a.noise_dev + static_cast<size_t>(b) * a.vocab;
-    const ExpScale e(temp);
+    const float scale = kLog2e / temp;
     const float p_inv = static_cast<float>(1.0 / ps.sum), q_inv = known ? static_cast<float>(1.0 / qs.sum) : 0.f;
-    const int per = (a.vocab + cluster - 1) / cluster;
-    const int i0 = static_cast<int>(rank) * per, i1 = min(a.vocab, i0 + per);
-    // 32 bits: lower bounds first, their best over the cluster, then whoever's upper bound reaches it
-    constexpr float kSlack = 4e-6f;       // on a share: argument, exponential, sum and product, each below 2^-20 of it in all
-    auto bounds = [&](int i, float* lower, float* upper) {
-      const float p = e(value_at(prow, i), ps.top) * p_inv;
-      const float q = known ? e(value_at(qrow, i), qs.top) * q_inv : 0.f;
-      const float x = -logf(noise[i]);
-      const float r = i == without ? 0.f : p - q, slack = i == without ? 0.f : kSlack * (p + q);
-      *lower = (r - slack) / x * (1.f - 1e-6f);
-      *upper = (r + slack) / x * (1.f + 1e-6f);
-    };
-    float best = 0.f;
-    for (int i = i0 + tid; i < i1; i += kPickThreads) {
-      float lower, upper;
-      bounds(i, &lower, &upper);
-      best = fmaxf(best, lower);
-    }
-    best = warp_max(best);
-    if (lane == 0) sm_best[warp] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < kPickWarps; ++w) best = fmaxf(best, sm_best[w]);
-      s_best = best;
-    }
-    pick_sync();
-    best = 0.f;
-    for (int r = 0; r < cluster; ++r) best = fmaxf(best, peer_value(&s_best, r));
+    // on a share: its argument up to 126, rounded three times, the exponential, the sum and the product are below 2^-16 of it
+    constexpr float kSlack = 1.6e-5f;
     Racer win = {0.0, 0x7fffffff};
-    bool difference = true;
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int i = i0 + tid; i < i1; i += kPickThreads) {
-        float lower, upper;
-        if (difference) bounds(i, &lower, &upper);
-        if (difference && !(upper > 0.f && upper >= best)) continue;
-        const double p = share(ps, value_at(prow, i), t64);
-        const double q = !difference ? 0.0 : known ? share(qs, value_at(qrow, i), t64) : i == without ? p : 0.0;
-        const double r = p - q;
-        if (r > 0.0) take_better(win, r / -log(static_cast<double>(noise[i])), i);
+    auto run = [&](int i, bool difference) {
+      const double p = share(ps, value_at(prow, i), t64);
+      const double q = !difference ? 0.0 : known ? share(qs, value_at(qrow, i), t64) : i == without ? p : 0.0;
+      const double r = p - q;
+      if (r > 0.0) take_better(win, r / -log(static_cast<double>(noise[i])), i);
+    };
+    // 32 bits: this block's entries, kHeld a thread at a time, their lower bounds, and whose upper bound reaches the best of them
+    float best = 0.f;
+    for (int first = i0; first < i1; first += kHeld * kPickThreads) {
+      if (first > i0) fetch_noise(first);
+      float lp[kHeld], upper[kHeld];
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        const int i = first + h * kPickThreads + tid;
+        lp[h] = i < i1 ? value_at(prow, i) : -INFINITY;
+        upper[h] = i < i1 && known ? value_at(qrow, i) : -INFINITY;
       }
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        const float p = ex2(fmaxf(lp[h] - ps.top, -1e30f) * scale) * p_inv;
+        const float q = known ? ex2(fmaxf(upper[h] - qs.top, -1e30f) * scale) * q_inv : 0.f;
+        const bool out = first + h * kPickThreads + tid == without;
+        const float r = out ? 0.f : p - q, slack = out ? 0.f : kSlack * (p + q);
+        best = fmaxf(best, __fdividef(r - slack, wait_of[h]) * (1.f - 4e-6f));
+        upper[h] = __fdividef(r + slack, wait_of[h]) * (1.f + 4e-6f);
+      }
+      best = warp_max(best);
+      if (lane == 0) sm_best[warp] = best;
+      __syncthreads();
+      best = warp_max(lane < kPickWarps ? sm_best[lane] : 0.f);
+      __syncthreads();
+      uint32_t can = 0;
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+        if (upper[h] > 0.f && upper[h] >= best && first + h * kPickThreads + tid < i1) can |= 1u << h;
+      for (; can; can &= can - 1) run(first + (__ffs(can) - 1) * kPickThreads + tid, true);
+    }
+    auto block_best = [&]() {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double s2 = __shfl_xor_sync(0xffffffffu, win.score, o);
         const int a2 = __shfl_xor_sync(0xffffffffu, win.at, o);
         take_better(win, s2, a2);
       }
-      if (lane == 0) {
-        sm_score[warp] = win.score;
-        sm_at[warp] = win.at;
-      }
+      if (lane == 0) sm_win[warp] = win;
       __syncthreads();
-      if (tid == 0) {
-        for (int w = 0; w < kPickWarps; ++w) take_better(win, sm_score[w], sm_at[w]);
-        s_score = win.score;
-        s_at = win.at;
+      if (lane < kPickWarps) win = sm_win[lane];
+#pragma unroll
+      for (int o = kPickWarps / 2; o > 0; o >>= 1) {
+        const double s2 = __shfl_xor_sync(0xffffffffu, win.score, o);
+        const int a2 = __shfl_xor_sync(0xffffffffu, win.at, o);
+        take_better(win, s2, a2);
       }
-      pick_sync();
-      for (int r = 0; r < cluster; ++r) take_better(win, peer_value(&s_score, r), peer_value(&s_at, r));
-      pick_sync();                                    // all have read: the next pass may overwrite, and a block may leave
-      if (win.at < a.vocab) break;                    // alike in every thread of the cluster
-      difference = false;                             // the difference is zero everywhere: the target's own shares
+      win.score = __shfl_sync(0xffffffffu, win.score, 0);
+      win.at = __shfl_sync(0xffffffffu, win.at, 0);
+    };
+    block_best();
+    if (tid == 0) put_to_first(&racers[rank], win);
+    pick_sync();
+    if (rank != 0) return;
+    for (int r = 0; r < cluster; ++r) take_better(win, racers[r].score, racers[r].at);
+    if (win.at >= a.vocab) {
+      // the difference is zero everywhere: the target's own shares
+      for (int i = tid; i < a.vocab; i += kPickThreads) run(i, false);
+      __syncthreads();
+      block_best();
     }
-    next = win.at < a.vocab ? win.at : ps.at;
+    next = win.at < a.vocab ? win.at : 0;
   }
   if (rank == 0)
     for (int k = tid; k < n_out; k += kPickThreads) {
@@ -353,7 +504,7 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const mtj_ver
 int rows_of(const mtj_verify_args& a) { return a.drafts + 1 + (a.draft_dev ? a.drafts : 0); }
 int chunks_of(const mtj_verify_args& a) { return (a.vocab + kChunk + 15) / kChunk; }      // room for the skew of a row's start
 int64_t stats_bytes(const mtj_verify_args& a) {
-  return static_cast<int64_t>(a.batch) * rows_of(a) * chunks_of(a) * static_cast<int64_t>(sizeof(ChunkStat));
+  return static_cast<int64_t>(std::min(a.batch, kRowBatch)) * rows_of(a) * chunks_of(a) * static_cast<int64_t>(sizeof(ChunkStat));
 }
 
 int32_t check_args(const mtj_verify_args* a, std::string* err) {
@@ -380,25 +531,45 @@ int32_t check_args(const mtj_verify_args* a, std::string* err) {
 }
 
 template <typename T>
-cudaError_t run(const mtj_verify_args& a, ChunkStat* stats, cudaStream_t s) {
-  const int rows = rows_of(a), chunks = chunks_of(a);
-  verify_rows_kernel<T><<<static_cast<unsigned>(a.batch * rows * chunks), kRowThreads, 0, s>>>(a, stats, rows, chunks);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int cluster = a.vocab > 2 * kPickThreads ? kPickCluster : 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch * cluster));
-  cfg.blockDim = dim3(kPickThreads);
-  cfg.dynamicSmemBytes = rows * sizeof(RowShare);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, a, static_cast<const ChunkStat*>(stats), rows, chunks, cluster);
+cudaError_t run(const mtj_verify_args& all, ChunkStat* stats, cudaStream_t s) {
+  const int rows = rows_of(all), chunks = chunks_of(all);
+  for (int b0 = 0; b0 < all.batch; b0 += kRowBatch) {
+    mtj_verify_args a = all;
+    a.batch = std::min(kRowBatch, all.batch - b0);
+    a.target_dev = static_cast<const T*>(all.target_dev) + b0 * all.batch_target;
+    if (all.draft_dev) a.draft_dev = static_cast<const T*>(all.draft_dev) + b0 * all.batch_draft;
+    const int64_t per = all.drafts;
+    if (all.draft_tokens_dev) a.draft_tokens_dev += b0 * per;
+    if (all.accept_dev) a.accept_dev += b0 * per;
+    a.noise_dev += static_cast<int64_t>(b0) * all.vocab;
+    if (all.counts_dev) a.counts_dev += b0;
+    if (all.temp_dev) a.temp_dev += b0;
+    a.tokens_out_dev += b0 * (per + 1);
+    a.accepted_out_dev += b0;
+    if (all.logprobs_out_dev) a.logprobs_out_dev += b0 * (per + 1);
+    const int64_t items = static_cast<int64_t>(a.batch) * rows * chunks;
+    verify_rows_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(kRowBlocks, items)), kRowThreads, 0, s>>>(a, stats, rows, chunks);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // as many blocks a sequence as leave two an SM, and no more than its entries are worth
+    int cluster = kPickCluster;
+    while (cluster > 1 && (static_cast<int64_t>(a.batch) * cluster > 2 * kRowBlocks || a.vocab <= cluster / 2 * 2 * kPickThreads)) cluster /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch * cluster));
+    cfg.blockDim = dim3(kPickThreads);
+    cfg.dynamicSmemBytes = rows * sizeof(RowShare);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, a, static_cast<const ChunkStat*>(stats), rows, chunks, cluster);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
