@@ -1,9 +1,10 @@
 // Eviction from a paged cache by accumulated attention weight (mtj_k_cache_evict).
 //
 // cache_select_kernel: one block a (sequence, key head).  The weights become integers that order as the numbers do; a
-//   radix selection over four digits of eight bits finds the key of the last one that is kept and how many of its equals are,
-//   and a pass in slot order writes the kept slots and their weights.
-// cache_move_kernel: one block a (spare page, key head, sequence) copies the kept rows of keys and values.
+//   radix selection over digits of 11, 11 and 10 bits finds the key of the last one that is kept and how many of its equals are
+//   (it ends early when a digit's whole bin is kept); a thread has kEach neighbouring slots, so that two sums over the block
+//   give every kept slot its place.  Up to kEach * kSelThreads slots are read once and stay in registers.
+// cache_move_kernel: one block a (spare page, key head, sequence) copies the kept rows of keys and values; bound by their bytes.
 #include <string>
 
 #include "mtj_cache.cuh"
@@ -14,6 +15,9 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kMoveThreads = 256;
+constexpr int kEach = 16;                  // neighbouring slots of a thread
+constexpr int kStage = 4096;               // kept slots on their way out
+constexpr int kBins = 2048;                // the first digit is sign, exponent and two bits: weights of one size are in several bins
 
 // ascending integer order is ascending order of the numbers; -0 and +0 are equal
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -46,11 +50,14 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* all) {
 }
 
 __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const mtj_cache_evict_args a) {
-  __shared__ int hist[256], warp_sums[32];
+  __shared__ int hist[kBins], warp_sums[32];
+  __shared__ int stage_slot[kStage];
+  __shared__ float stage_weight[kStage];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+  __shared__ int s_need, s_all;
   const int b = blockIdx.x / a.kv_heads, tid = threadIdx.x;
   const int slots = a.pages * kPageTokens;
+  pdl_launch_dependents();
   const CacheSeq s = cache_seq(a.lengths_dev, nullptr, b, 0, a.pages);
   const bool moves = s.length > a.keep;
   const float* w = a.weights_dev + static_cast<size_t>(blockIdx.x) * slots;
@@ -74,50 +81,114 @@ __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const mtj_cac
     return;
   }
   const int lo = a.first, hi = s.length - a.last, need = a.keep - a.first - a.last;
-  // the `need` largest of [lo, hi): all keys above `prefix`, and the first `ties` equal to it
+  // neighbouring slots of a thread, fewer where the sequence is short; a block goes over the sequence in steps of `span`
+  const int each = min(kEach, (s.length + 4 * kSelThreads - 1) / (4 * kSelThreads) * 4), span = each * kSelThreads;
+  const bool once = s.length <= span;
+  float v[kEach];
+  auto load = [&](int base) {
+    const int i0 = base + tid * each;
+#pragma unroll
+    for (int e0 = 0; e0 < kEach; e0 += 4) {
+      if (e0 >= each) break;
+      if (i0 + e0 + 4 <= s.length && !(reinterpret_cast<uintptr_t>(w) & 15)) {
+        const float4 x = *reinterpret_cast<const float4*>(w + i0 + e0);
+        v[e0] = x.x;
+        v[e0 + 1] = x.y;
+        v[e0 + 2] = x.z;
+        v[e0 + 3] = x.w;
+      } else {
+#pragma unroll
+        for (int e = e0; e < e0 + 4; ++e) v[e] = i0 + e < s.length ? w[i0 + e] : 0.f;
+      }
+    }
+  };
+  if (once) load(0);
+  // the `need` largest of [lo, hi): all keys above `prefix` in the digits of `mask`, and the first `ties` equal to it there
   uint32_t prefix = 0, mask = 0;
   int ties = need;
   if (need > 0) {
     if (tid == 0) s_need = need;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+      const uint32_t digits = digit == 2 ? 1023u : 2047u;
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t k = order_key(w[i]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      for (int base = 0; base < s.length; base += span) {
+        if (!once) load(base);
+        const int i0 = base + tid * each;
+        if (i0 >= s.length) continue;
+#pragma unroll
+        for (int e0 = 0; e0 < kEach; e0 += 4) {
+          if (e0 >= each) break;
+#pragma unroll
+          for (int e = e0; e < e0 + 4; ++e) {
+            const uint32_t k = order_key(v[e]);
+            if (i0 + e >= lo && i0 + e < hi && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
+          }
+        }
       }
       __syncthreads();
-      // digits from the largest down: thread t holds digit 255 - t
+      // digits from the largest down: a thread holds two
+      const int top = kBins - 1 - 2 * tid;
       int all;
-      const int here = tid < 256 ? hist[255 - tid] : 0;
-      const int above = block_scan(here, warp_sums, &all);
+      const int first = hist[top], second = hist[top - 1];
+      const int above = block_scan(first + second, warp_sums, &all);
       const int want = s_need;
       __syncthreads();
-      if (tid < 256 && above < want && above + here >= want) {
-        s_prefix = prefix | (static_cast<uint32_t>(255 - tid) << shift);
-        s_need = want - above;
+      if (above < want && above + first + second >= want) {
+        const bool upper = above + first >= want;
+        s_prefix = prefix | (static_cast<uint32_t>(upper ? top : top - 1) << shift);
+        s_need = want - above - (upper ? 0 : first);
+        s_all = above + first + (upper ? 0 : second) == want;
       }
       __syncthreads();
       prefix = s_prefix;
-      mask |= 255u << shift;
+      mask |= digits << shift;
+      if (s_all) break;
     }
     ties = s_need;
   }
   int out = 0, equal_before = 0;
-  for (int i0 = 0; i0 < s.length; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const bool in = i < s.length;
-    const float v = in ? w[i] : 0.f;
-    const bool middle = in && i >= lo && i < hi && need > 0;
-    const uint32_t k = order_key(v);
-    const bool equal = middle && k == prefix;
+  for (int base = 0; base < s.length; base += span) {
+    if (!once) load(base);
+    const int i0 = base + tid * each;
+    uint32_t equal = 0, sure = 0;          // bits of this thread's slots
+    if (i0 < s.length) {
+#pragma unroll
+      for (int e0 = 0; e0 < kEach; e0 += 4) {
+        if (e0 >= each) break;
+#pragma unroll
+        for (int e = e0; e < e0 + 4; ++e) {
+          const int i = i0 + e;
+          const uint32_t k = order_key(v[e]) & mask;
+          const bool middle = i >= lo && i < hi;
+          if (i < s.length && (!middle || (need > 0 && k > prefix))) sure |= 1u << e;
+          if (middle && need > 0 && k == prefix) equal |= 1u << e;
+        }
+      }
+    }
     int all_equal, all_keep;
-    const int rank = block_scan(equal ? 1 : 0, warp_sums, &all_equal);
-    const bool keep = in && (i < lo || i >= hi || (middle && (k > prefix || (equal && equal_before + rank < ties))));
-    const int at = block_scan(keep ? 1 : 0, warp_sums, &all_keep);
-    if (keep) {
-      kept[out + at] = i;
-      w_out[out + at] = v;      // at or before slot i, which this block has read
+    int rank = equal_before + block_scan(__popc(equal), warp_sums, &all_equal);
+    for (uint32_t rest = equal; rest && rank < ties; rest &= rest - 1, ++rank) sure |= rest & (0u - rest);
+    const int first_place = block_scan(__popc(sure), warp_sums, &all_keep);
+    // through shared memory: neighbouring threads' places are neighbours, a thread's own are too, a warp's at one time are not
+    for (int r0 = 0; r0 < all_keep; r0 += kStage) {
+      int place = first_place - r0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (sure >> e & 1u) {
+          if (place >= 0 && place < kStage) {
+            stage_slot[place] = i0 + e;
+            stage_weight[place] = v[e];
+          }
+          ++place;
+        }
+      __syncthreads();
+      for (int i = tid; i < min(kStage, all_keep - r0); i += kSelThreads) {
+        kept[out + r0 + i] = stage_slot[i];
+        w_out[out + r0 + i] = stage_weight[i];      // at or before its slot, which this block has read
+      }
+      __syncthreads();
     }
     out += all_keep;
     equal_before += all_equal;
@@ -130,8 +201,12 @@ __global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const mtj_cach
   const int spare = (a.keep + kPageTokens - 1) / kPageTokens;
   const int i = blockIdx.x % spare, kvh = blockIdx.x / spare % a.kv_heads, b = blockIdx.x / spare / a.kv_heads;
   const CacheSeq s = cache_seq(a.lengths_dev, nullptr, b, 0, a.pages);
-  if (s.length <= a.keep) return;
+  if (s.length <= a.keep) {
+    pdl_wait();                            // a launch that ends before the one it is chained to would let the next one overtake both
+    return;
+  }
   const int to = a.spare_pages_dev[static_cast<size_t>(b) * spare + i];
+  pdl_wait();
   if (!cache_page_ok(to, a.n_pages)) {
     if (threadIdx.x == 0 && a.status_dev) atomicOr(a.status_dev, kDevErrBadIndex);
     return;
@@ -191,9 +266,10 @@ int32_t mtj_k_cache_evict(const mtj_cache_evict_args* a, mtj_stream stream) {
   if (rc) return mtj_set_error(rc, err.c_str());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   mtj::cache_select_kernel<<<a->batch * a->kv_heads, mtj::kSelThreads, 0, s>>>(*a);
+  cudaError_t e = cudaGetLastError();
   const int spare = (a->keep + mtj::kPageTokens - 1) / mtj::kPageTokens;
-  mtj::cache_move_kernel<<<static_cast<unsigned>(spare * a->kv_heads * a->batch), mtj::kMoveThreads, 0, s>>>(*a);
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = mtj::launch_pdl(mtj::cache_move_kernel, dim3(static_cast<unsigned>(spare * a->kv_heads * a->batch)), dim3(mtj::kMoveThreads), 0, s, true, *a);
   if (e != cudaSuccess) return mtj_set_error(MTJ_ERR_CUDA, cudaGetErrorString(e));
   return MTJ_OK;
 }

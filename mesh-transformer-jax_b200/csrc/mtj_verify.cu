@@ -274,12 +274,13 @@ __device__ __forceinline__ double share(const RowShare& s, float l, double temp)
 struct Racer {
   double score;
   int at;
+  float l;             // its logit
 };
-__device__ __forceinline__ void take_better(Racer& x, double score, int at) {
-  if (score > x.score || (score == x.score && at < x.at)) {
-    x.score = score;
-    x.at = at;
-  }
+__device__ __forceinline__ void take_better(Racer& x, const Racer& y) {
+  if (y.score > x.score || (y.score == x.score && y.at < x.at)) x = y;
+}
+__device__ __forceinline__ Racer from_lane(const Racer& x, int mask) {
+  return {__shfl_xor_sync(0xffffffffu, x.score, mask), __shfl_xor_sync(0xffffffffu, x.at, mask), __shfl_xor_sync(0xffffffffu, x.l, mask)};
 }
 
 __device__ __forceinline__ uint32_t pick_rank() {
@@ -295,6 +296,7 @@ __device__ __forceinline__ void put_to_first(Racer* slot, const Racer& x) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(slot)));
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(x.score) : "memory");
   asm volatile("st.shared::cluster.u32 [%0 + 8], %1;" ::"r"(at), "r"(x.at) : "memory");
+  asm volatile("st.shared::cluster.f32 [%0 + 12], %1;" ::"r"(at), "f"(x.l) : "memory");
 }
 
 // Blocks of a cluster a sequence: as many as keep two an SM, up to eight.
@@ -338,20 +340,27 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     for (int h = 0; h < kHeld; ++h) wait_of[h] = -logf(wait_of[h]);
   };
   if (!greedy) fetch_noise(i0);
+  const float p0_first = p0;                       // of draft `lane`
   pdl_wait();
-  const double t64 = greedy ? 1.0 : static_cast<double>(temp);
+  const double t64 = greedy ? 1.0 : static_cast<double>(temp), inv_t64 = 1.0 / t64;
   for (int r = warp; r < rows; r += kPickWarps) {
     if (r <= a.drafts ? r > n : (r - a.drafts - 1 >= n || greedy)) continue;
     const ChunkStat* st = stats + (static_cast<int64_t>(b) * rows + r) * chunks;
+    constexpr int kSeen = 2;                       // chunks that a lane keeps: vocabularies up to 65536 are read once
+    ChunkStat seen[kSeen];
+#pragma unroll
+    for (int i = 0; i < kSeen; ++i) seen[i] = lane + 32 * i < chunks ? st[lane + 32 * i] : ChunkStat{-INFINITY, 0.f, 0x7fffffff, 0};
     float top = -INFINITY;
     int at = 0x7fffffff;
-    for (int c = lane; c < chunks; c += 32) {
-      const ChunkStat s = st[c];
+    auto larger = [&](const ChunkStat& s) {
       if (s.top > top) {
         top = s.top;
         at = s.at;
       }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kSeen; ++i) larger(seen[i]);
+    for (int c = lane + 32 * kSeen; c < chunks; c += 32) larger(st[c]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
@@ -362,12 +371,15 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
       }
     }
     double sum = 0.0;
-    if (!greedy)
-      for (int c = lane; c < chunks; c += 32) {
-        const ChunkStat s = st[c];
+    if (!greedy) {
+      auto add = [&](const ChunkStat& s) {
         if (s.top > -INFINITY)
-          sum += static_cast<double>(s.sum) * (s.top == top ? 1.0 : exp((static_cast<double>(s.top) - static_cast<double>(top)) / t64));
-      }
+          sum += static_cast<double>(s.sum) * (s.top == top ? 1.0 : exp((static_cast<double>(s.top) - static_cast<double>(top)) * inv_t64));
+      };
+#pragma unroll
+      for (int i = 0; i < kSeen; ++i) add(seen[i]);
+      for (int c = lane + 32 * kSeen; c < chunks; c += 32) add(st[c]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) row_share[r] = {top, greedy && top > -INFINITY ? at : 0, sum, greedy ? 0.0 : log(sum)};
@@ -405,7 +417,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
   }
   __syncthreads();
   const int taken = s_taken;
+  // the taken tokens, while the next one is looked for
+  int32_t* out = a.tokens_out_dev + static_cast<size_t>(b) * n_out;
+  float* logs = a.logprobs_out_dev ? a.logprobs_out_dev + static_cast<size_t>(b) * n_out : nullptr;
+  if (rank == 0 && warp == 0) {
+    for (int k = lane; k < n_out; k += 32) {
+      if (k == taken) continue;
+      out[k] = k < taken ? tokens[k] : -1;
+      if (logs) logs[k] = k >= taken || greedy ? 0.f : static_cast<float>(log_share(row_share[k], k < 32 ? p0_first : value_at(row_of<T>(a, b, k), tokens[k]), t64));
+    }
+    if (lane == 0) a.accepted_out_dev[b] = taken;
+  }
   int next;
+  float next_log = 0.f;
   if (greedy) {
     next = row_share[taken].at;
   } else {
@@ -420,12 +444,13 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     const float p_inv = static_cast<float>(1.0 / ps.sum), q_inv = known ? static_cast<float>(1.0 / qs.sum) : 0.f;
     // on a share: its argument up to 126, rounded three times, the exponential, the sum and the product are below 2^-16 of it
     constexpr float kSlack = 1.6e-5f;
-    Racer win = {0.0, 0x7fffffff};
+    Racer win = {0.0, 0x7fffffff, 0.f};
     auto run = [&](int i, bool difference) {
-      const double p = share(ps, value_at(prow, i), t64);
+      const float l = value_at(prow, i);
+      const double p = share(ps, l, t64);
       const double q = !difference ? 0.0 : known ? share(qs, value_at(qrow, i), t64) : i == without ? p : 0.0;
       const double r = p - q;
-      if (r > 0.0) take_better(win, r / -log(static_cast<double>(noise[i])), i);
+      if (r > 0.0) take_better(win, {r / -log(static_cast<double>(noise[i])), i, l});
     };
     // 32 bits: this block's entries, kHeld a thread at a time, their lower bounds, and whose upper bound reaches the best of them
     float best = 0.f;
@@ -460,28 +485,18 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     }
     auto block_best = [&]() {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double s2 = __shfl_xor_sync(0xffffffffu, win.score, o);
-        const int a2 = __shfl_xor_sync(0xffffffffu, win.at, o);
-        take_better(win, s2, a2);
-      }
+      for (int o = 16; o > 0; o >>= 1) take_better(win, from_lane(win, o));
       if (lane == 0) sm_win[warp] = win;
       __syncthreads();
-      if (lane < kPickWarps) win = sm_win[lane];
+      win = sm_win[lane % kPickWarps];
 #pragma unroll
-      for (int o = kPickWarps / 2; o > 0; o >>= 1) {
-        const double s2 = __shfl_xor_sync(0xffffffffu, win.score, o);
-        const int a2 = __shfl_xor_sync(0xffffffffu, win.at, o);
-        take_better(win, s2, a2);
-      }
-      win.score = __shfl_sync(0xffffffffu, win.score, 0);
-      win.at = __shfl_sync(0xffffffffu, win.at, 0);
+      for (int o = kPickWarps / 2; o > 0; o >>= 1) take_better(win, from_lane(win, o));
     };
     block_best();
     if (tid == 0) put_to_first(&racers[rank], win);
     pick_sync();
     if (rank != 0) return;
-    for (int r = 0; r < cluster; ++r) take_better(win, racers[r].score, racers[r].at);
+    for (int r = 0; r < cluster; ++r) take_better(win, racers[r]);
     if (win.at >= a.vocab) {
       // the difference is zero everywhere: the target's own shares
       for (int i = tid; i < a.vocab; i += kPickThreads) run(i, false);
@@ -489,16 +504,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
       block_best();
     }
     next = win.at < a.vocab ? win.at : 0;
+    next_log = static_cast<float>(log_share(ps, win.at < a.vocab ? win.l : value_at(prow, 0), t64));
   }
-  if (rank == 0)
-    for (int k = tid; k < n_out; k += kPickThreads) {
-      const int x = k < taken ? tokens[k] : k == taken ? next : -1;
-      a.tokens_out_dev[static_cast<size_t>(b) * n_out + k] = x;
-      if (a.logprobs_out_dev)
-        a.logprobs_out_dev[static_cast<size_t>(b) * n_out + k] =
-            x < 0 || greedy ? 0.f : static_cast<float>(log_share(row_share[k], value_at(row_of<T>(a, b, k), x), t64));
-      if (k == 0) a.accepted_out_dev[b] = taken;
-    }
+  if (rank == 0 && tid == 0) {
+    out[taken] = next;
+    if (logs) logs[taken] = next_log;
+  }
 }
 
 int rows_of(const mtj_verify_args& a) { return a.drafts + 1 + (a.draft_dev ? a.drafts : 0); }
@@ -547,13 +558,16 @@ cudaError_t run(const mtj_verify_args& all, ChunkStat* stats, cudaStream_t s) {
     a.tokens_out_dev += b0 * (per + 1);
     a.accepted_out_dev += b0;
     if (all.logprobs_out_dev) a.logprobs_out_dev += b0 * (per + 1);
-    const int64_t items = static_cast<int64_t>(a.batch) * rows * chunks;
-    verify_rows_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(kRowBlocks, items)), kRowThreads, 0, s>>>(a, stats, rows, chunks);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
     // as many blocks a sequence as leave two an SM, and no more than its entries are worth
     int cluster = kPickCluster;
     while (cluster > 1 && (static_cast<int64_t>(a.batch) * cluster > 2 * kRowBlocks || a.vocab <= cluster / 2 * 2 * kPickThreads)) cluster /= 2;
+    // a short line leaves SMs to the blocks of the second kernel, which have something to do before they need its results
+    const int64_t items = static_cast<int64_t>(a.batch) * rows * chunks;
+    int64_t row_blocks = std::min<int64_t>(kRowBlocks, (items + 5) / 6);
+    if (items <= 2 * kRowBlocks * (kRowThreads / 32)) row_blocks = std::min<int64_t>(row_blocks, std::max(kRowBlocks / 2, kRowBlocks - (a.batch * cluster + 1) / 2));
+    verify_rows_kernel<T><<<static_cast<unsigned>(row_blocks), kRowThreads, 0, s>>>(a, stats, rows, chunks);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.batch * cluster));
     cfg.blockDim = dim3(kPickThreads);
