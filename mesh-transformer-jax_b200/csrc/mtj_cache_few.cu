@@ -14,7 +14,8 @@
 // tcgen05 would be as empty (M is at least 64 there) and has the accumulators a trip through tensor memory away; the bound is
 // traffic.  Queries in 32 bits are the exact sum of three bf16 numbers, three products each.  The weights P go into the
 // product as two bf16 numbers (three for 32-bit queries), an error of 2^-16 (2^-24): one would cost as much as the rounding of
-// the output.  Scores, maxima, sums and outputs are 32-bit.
+// the output (and save 6 of 44 us with 5 drafts, 4 heads a key head and 8 sequences of up to 8191 slots).  Scores, maxima, sums and
+// outputs are 32-bit.
 //
 // New keys and values are laid over the rows of the tile that has just arrived, and stored to their slots by the blocks of the
 // first row tile: nobody reads in this launch what it stores.  Slots behind the sequence are zeroed in the tile, since weight
@@ -54,7 +55,7 @@ struct FewCfg {
   static constexpr int kParts = kWorkers / kRowWarps;      // warps with results for one row
   static constexpr int kChains = kSub * kNt >= 4 ? 1 : 2;  // of sums for a score
   static constexpr int kRows = 8 * NT;
-  static constexpr int kQTerms = sizeof(T) == 2 ? 1 : 3, kPTerms = sizeof(T) == 2 ? 2 : 3;
+  static constexpr int kQTerms = sizeof(T) == 2 ? 1 : 3, kPTerms = sizeof(T) == 4 ? 3 : 2;
   // 32-bit queries: the product adds 16 terms at a time, what it adds them to is rounded towards zero, so the sums over steps and
   // keys are taken with additions that round to the nearest (a token behind 2052 keys: 1.1e-6 off without)
   static constexpr bool kExactSums = sizeof(T) == 4;
@@ -176,6 +177,41 @@ static_assert(kFewBatch <= 2 * kFewThreads, "two sequences a thread");
 template <int KEYS>
 __device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* held, int* prefix, int* first, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = 2 * tid;
+  if (a.c.batch <= 32) {
+    // one warp, without the block's barriers
+    if (warp == 0) {
+      auto before = [&](int n, int* all) {
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        *all = __shfl_sync(0xffffffffu, x, 31);
+        return x - n;
+      };
+      auto put = [&](int* at, int* out, int x, int all) {
+        if (lane < a.c.batch) at[lane] = x;
+        if (lane == 0) at[a.c.batch] = all;
+        if (out && blockIdx.x == 0 && lane < a.c.batch) out[lane] = x;
+        if (out && blockIdx.x == 0 && lane == 0) out[a.c.batch] = all;
+      };
+      int tiles = 0, total, pieces;
+      if (lane < a.c.batch) {
+        held[lane] = few_held(a, lane, blockIdx.x == 0);
+        tiles = few_seq<KEYS>(a, held[lane]).tiles;
+      }
+      const int tiles_before = before(tiles * units, &total);
+      put(prefix, a.prefix, tiles_before, total);
+      if (a.aligned) {
+        const int n = lane < a.c.batch ? pieces_in(tiles, piece_width(a, total, a.c.batch * units)) * units : 0;
+        const int x = before(n, &pieces);
+        put(first, nullptr, x, pieces);
+      }
+    }
+    __syncthreads();
+    return;
+  }
   int n0 = 0, n1 = 0;
   if (b < a.c.batch) {
     held[b] = few_held(a, b, blockIdx.x == 0);
@@ -200,10 +236,9 @@ __device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* 
   }
   if (b <= a.c.batch) prefix[b] = before;
   if (b + 1 <= a.c.batch) prefix[b + 1] = before + n0;
-  int* second = a.prefix;                  // for the second kernel
-  if (blockIdx.x == 0) {
-    if (b <= a.c.batch) second[b] = before;
-    if (b + 1 <= a.c.batch) second[b + 1] = before + n0;
+  if (blockIdx.x == 0) {                   // for the second kernel
+    if (b <= a.c.batch) a.prefix[b] = before;
+    if (b + 1 <= a.c.batch) a.prefix[b + 1] = before + n0;
   }
   if (a.aligned) {
     // pieces of sequence b: first[b] before it, its units' after one another
@@ -223,11 +258,6 @@ __device__ __forceinline__ void lay_out(const CacheFewArgs& a, int units, int2* 
     for (int w = 0; w < warp; ++w) before += scan[w];
     if (b <= a.c.batch) first[b] = before;
     if (b + 1 <= a.c.batch) first[b + 1] = before + n0;
-    if (blockIdx.x == 0) {
-      second += kFewBatch + 1;
-      if (b <= a.c.batch) second[b] = before;
-      if (b + 1 <= a.c.batch) second[b + 1] = before + n0;
-    }
   }
   __syncthreads();
 }
@@ -243,9 +273,6 @@ __device__ __forceinline__ int sequence_of(const int* prefix, int batch, int x) 
 // no piece is empty
 __device__ __forceinline__ int pieces_of(int64_t total, int most) { return static_cast<int>(min(total, static_cast<int64_t>(most))); }
 __device__ __forceinline__ int piece_begin(int64_t total, int pieces, int i) { return static_cast<int>(total * i / pieces); }
-__device__ __forceinline__ int piece_of(int64_t total, int pieces, int x) {
-  return static_cast<int>(((static_cast<int64_t>(x) + 1) * pieces + total - 1) / total) - 1;
-}
 
 template <int DH, int NT, typename T>
 __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_constant__ CUtensorMap map_k,
@@ -638,6 +665,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
           }
         }
       }
+      else if (a.scores) {
+        // a page that does not exist: nobody sees its keys
+        for (int v = lane; v < 16 * kSub * a.score_rows; v += 32)
+          a.scores[(static_cast<size_t>(x + i) * kKeys + key0) * a.score_rows + v] = -INFINITY;
+      }
       // every load of the tile has been used by a product that was issued: which lane hands it back hangs on the last one
       const int by = __any_sync(0xffffffffu, __float_as_uint(o[kSteps - 1][kNt - 1][0]) == 0x7fc0deadu) ? 1 : 0;
       if (lane == by) arrive(empty_bar(st));
@@ -681,6 +713,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
       worker_sync();
     }
     const bool starts = tile0 == 0, whole_unit = starts && n_tiles == s.tiles;
+    if (tid == 0 && starts) a.unit_blocks[2 * (b * units + unit)] = blockIdx.x;
+    if (tid == 0 && tile0 + n_tiles == s.tiles) a.unit_blocks[2 * (b * units + unit) + 1] = blockIdx.x;
     const size_t part = static_cast<size_t>(blockIdx.x) * 2 + (starts ? 1 : 0);
     for (int i = tid; i < kRows * (DH / 8); i += 32 * kWorkers) {
       const int r = i / (DH / 8), d = i % (DH / 8) * 8, t = (row0 + r) / group;
@@ -720,10 +754,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
   }
 }
 
-// Second kernel: blocks [0, join_blocks) one a (sequence, unit, row) join the parts of units that several blocks worked on, and
-// write the zeros of rows that nobody worked on; the others add the attention weights of kWeightSlots slots of one key head.
+// Second kernel, a sequence and key head by blockIdx.z and .y: the first join_rows blocks in x join a row's parts where several blocks
+// worked on its unit, and write the zeros of rows that nobody worked on; the others add the attention weights of kWeightSlots slots.
 template <int DH, typename T>
-__global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const CacheFewArgs a, int tile_rows, int most, int join_blocks) {
+__global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const CacheFewArgs a, int tile_rows, int join_rows) {
   constexpr int kKeys = 4096 / DH;
   constexpr int kLanes = DH / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 sm_o[kGroups][kLanes];
@@ -732,25 +766,18 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = a.c.heads / a.c.kv_heads, rows = a.tokens * group, row_tiles = (rows + tile_rows - 1) / tile_rows;
   const int units = a.c.kv_heads * row_tiles;
-  const int slots = a.c.pages * kPageTokens, chunks = (slots + kWeightSlots - 1) / kWeightSlots;
-  const bool joins = static_cast<int>(blockIdx.x) < join_blocks;
-  const int at = joins ? blockIdx.x : blockIdx.x - join_blocks, per = joins ? rows : chunks;
-  const int inner = at % per, kvh = at / per % a.c.kv_heads, b = at / per / a.c.kv_heads;      // inner: row, or chunk of slots
+  const int slots = a.c.pages * kPageTokens;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const bool joins = static_cast<int>(blockIdx.x) < join_rows;
+  const int inner = joins ? blockIdx.x : blockIdx.x - join_rows;         // row, or part of the slots
   const FewSeq s = few_seq<kKeys>(a, few_held(a, b, false));
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t total = a.prefix[a.c.batch];
-  const int begin = a.prefix[b], pieces = a.aligned ? a.prefix[kFewBatch + 1 + b] : pieces_of(total, most);
-  const int each = a.aligned ? (a.prefix[kFewBatch + 1 + b + 1] - pieces) / units : 0;
   // the blocks that worked on a unit: the first one and how many
   auto blocks_of = [&](int unit, int* n) {
-    if (a.aligned) {
-      *n = each;
-      return pieces + unit * each;
-    }
-    const int u0 = begin + unit * s.tiles, fb = piece_of(total, pieces, u0);
-    *n = piece_of(total, pieces, u0 + s.tiles - 1) - fb + 1;
-    return fb;
+    const int2 ends = *reinterpret_cast<const int2*>(a.unit_blocks + 2 * (b * units + unit));
+    *n = ends.y - ends.x + 1;
+    return ends.x;
   };
 
   // part k of the unit that lies at [u0, u1) in the line: the end of the first block's piece, then the beginnings of the next ones'
@@ -807,82 +834,80 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
   }
 
   // attention weights
-  const int chunk = inner;
-  if (chunk * kWeightSlots >= s.length) return;
+  if (inner * kWeightSlots >= s.length) return;
   const size_t base = (static_cast<size_t>(b) * a.c.kv_heads + kvh) * slots;
-  const bool in_place = a.c.weights_in_dev == a.c.weights_out_dev;
   constexpr int kEach = kWeightSlots / kJoinThreads;
-  float sum[kEach] = {};
-  int tile[kEach], key[kEach];                                           // where the slot's scores stand in its units
-  bool held[kEach], some = false;
+  float sum[kEach], old[kEach];
+  int at_key[kEach];                                                     // where the slot's scores stand in its units, in keys; -1: nobody sees it
+  const int fresh0 = s.length - s.fresh;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int j = chunk * kWeightSlots + i * kJoinThreads + tid;
-    held[i] = j < s.length;
-    const int tl = j / kKeys;
-    key[i] = j % kKeys;
-    tile[i] = !held[i] || s.tiles == 0 ? -1 : tl < s.sink_tiles ? tl : tl >= s.low_tile ? s.sink_tiles + tl - s.low_tile : -1;
-    if (tile[i] >= 0) {
-      // a page that does not exist has left no scores
-      const int page = a.c.page_table_dev[static_cast<size_t>(b) * a.c.pages + j / kPageTokens];
-      if (!cache_page_ok(page, a.c.n_pages)) tile[i] = -1;
-    }
-    some |= tile[i] >= 0;
+    const int j = inner * kWeightSlots + i * kJoinThreads + tid, tl = j / kKeys;
+    sum[i] = 0.f;
+    old[i] = a.c.weights_in_dev && j < fresh0 ? a.c.weights_in_dev[base + j] : 0.f;
+    const int tile = tl < s.sink_tiles ? tl : tl >= s.low_tile ? s.sink_tiles + tl - s.low_tile : -1;
+    at_key[i] = j < s.length && s.tiles > 0 && tile >= 0 ? tile * kKeys + j % kKeys : -1;
   }
-  if (s.tiles > 0 && __syncthreads_or(some ? 1 : 0)) {
-    for (int rt = 0; rt < row_tiles; ++rt) {
-      const int unit = kvh * row_tiles + rt;
-      const int u0 = begin + unit * s.tiles;
-      int n;
-      const int fb = blocks_of(unit, &n);
-      __syncthreads();
-      for (int r = warp; r < tile_rows; r += kJoinThreads / 32) {
-        float top = -INFINITY, l = 0.f;
-        if (n == 1) {
-          const float2 ml = a.lse[(static_cast<size_t>(b) * units + unit) * tile_rows + r];
-          top = ml.x;
-          l = ml.y;
-        } else {
-          auto part_of = [&](int k) { return (static_cast<size_t>(fb + k) * 2 + (k == 0 ? 1 : 0)) * tile_rows + r; };
-          for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[part_of(k)].x);
-          top = warp_max(top);
-          for (int k = lane; k < n; k += 32) {
-            const float2 ml = a.part_ml[part_of(k)];
-            if (ml.x > -INFINITY) l = fmaf(ml.y, exp2_fast(ml.x - top), l);
-          }
-          l = warp_sum(l);
-        }
-        if (lane == 0) {
-          row_m[r] = top == -INFINITY ? 0.f : top;
-          row_inv[r] = l > 0.f ? 1.f / l : 0.f;
-        }
-      }
-      __syncthreads();
-      const int live = min(tile_rows, rows - rt * tile_rows);
+  const bool fours = (a.score_rows & 3) == 0;
+  for (int rt = 0; rt < (s.tiles > 0 ? row_tiles : 0); ++rt) {
+    const int unit = kvh * row_tiles + rt, live = min(tile_rows, rows - rt * tile_rows);
+    const float* scores = a.scores + static_cast<size_t>(a.prefix[b] + unit * s.tiles) * kKeys * a.score_rows;
+    // the first rows' scores are on their way while the rows' maxima and sums are put together
+    float4 head[kEach];
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        if (tile[i] < 0) continue;
-        const float* sc = a.scores + (static_cast<size_t>(u0 + tile[i]) * kKeys + key[i]) * a.score_rows;
-        int r = 0;
-        if ((a.score_rows & 3) == 0)
-          for (; r + 4 <= live; r += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(sc + r);
-            sum[i] = fmaf(exp2_fast(x.x - row_m[r]), row_inv[r], sum[i]);
-            sum[i] = fmaf(exp2_fast(x.y - row_m[r + 1]), row_inv[r + 1], sum[i]);
-            sum[i] = fmaf(exp2_fast(x.z - row_m[r + 2]), row_inv[r + 2], sum[i]);
-            sum[i] = fmaf(exp2_fast(x.w - row_m[r + 3]), row_inv[r + 3], sum[i]);
-          }
-        for (; r < live; ++r) sum[i] = fmaf(exp2_fast(sc[r] - row_m[r]), row_inv[r], sum[i]);
+    for (int i = 0; i < kEach; ++i)
+      if (fours && at_key[i] >= 0) head[i] = *reinterpret_cast<const float4*>(scores + static_cast<size_t>(at_key[i]) * a.score_rows);
+    int n;
+    const int fb = blocks_of(unit, &n);
+    __syncthreads();                                                     // the tile before has been worked off
+    for (int r = warp; r < live; r += kJoinThreads / 32) {
+      float top = -INFINITY, l = 0.f;
+      if (n == 1) {
+        const float2 ml = a.lse[(static_cast<size_t>(b) * units + unit) * tile_rows + r];
+        top = ml.x;
+        l = ml.y;
+      } else {
+        auto part_of = [&](int k) { return (static_cast<size_t>(fb + k) * 2 + (k == 0 ? 1 : 0)) * tile_rows + r; };
+        for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[part_of(k)].x);
+        top = warp_max(top);
+        for (int k = lane; k < n; k += 32) {
+          const float2 ml = a.part_ml[part_of(k)];
+          if (ml.x > -INFINITY) l = fmaf(ml.y, exp2_fast(ml.x - top), l);
+        }
+        l = warp_sum(l);
+      }
+      if (lane == 0) {
+        row_m[r] = top == -INFINITY ? 0.f : top;
+        row_inv[r] = l > 0.f ? 1.f / l : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (at_key[i] < 0) continue;
+      const float* sc = scores + static_cast<size_t>(at_key[i]) * a.score_rows;
+      for (int r = 0; r < live; r += 4) {
+        float4 x = head[i];
+        if (!fours) {
+          x.x = sc[r];
+          x.y = r + 1 < live ? sc[r + 1] : -INFINITY;
+          x.z = r + 2 < live ? sc[r + 2] : -INFINITY;
+          x.w = r + 3 < live ? sc[r + 3] : -INFINITY;
+        } else if (r > 0) {
+          x = *reinterpret_cast<const float4*>(sc + r);
+        }
+        sum[i] = fmaf(exp2_fast(x.x - row_m[r]), row_inv[r], sum[i]);
+        if (r + 1 < live) sum[i] = fmaf(exp2_fast(x.y - row_m[r + 1]), row_inv[r + 1], sum[i]);
+        if (r + 2 < live) sum[i] = fmaf(exp2_fast(x.z - row_m[r + 2]), row_inv[r + 2], sum[i]);
+        if (r + 3 < live) sum[i] = fmaf(exp2_fast(x.w - row_m[r + 3]), row_inv[r + 3], sum[i]);
       }
     }
   }
+  const bool in_place = a.c.weights_in_dev == a.c.weights_out_dev;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    if (!held[i]) continue;
-    const int j = chunk * kWeightSlots + i * kJoinThreads + tid;
-    const bool fresh = j >= s.length - s.fresh;
-    if (tile[i] < 0 && in_place && !fresh) continue;
-    a.c.weights_out_dev[base + j] = (a.c.weights_in_dev && !fresh ? a.c.weights_in_dev[base + j] : 0.f) + sum[i];
+    const int j = inner * kWeightSlots + i * kJoinThreads + tid;
+    if (j < s.length && (at_key[i] >= 0 || !in_place || j >= fresh0)) a.c.weights_out_dev[base + j] = old[i] + sum[i];
   }
 }
 
@@ -910,12 +935,10 @@ cudaError_t launch(const CacheFewArgs& a, const CUtensorMap& mk, const CUtensorM
   if (e != cudaSuccess) return e;
   e = launch_pdl(cache_few_kernel<DH, NT, T>, dim3(pieces), dim3(kFewThreads), C::kSmem, s, false, mk, mv, a);
   if (e != cudaSuccess) return e;
-  const int rows = a.tokens * (a.c.heads / a.c.kv_heads);
-  const int join = a.whole ? 0 : a.c.batch * a.c.kv_heads * rows;
-  const int slots = a.c.pages * kPageTokens;
-  const int weigh = a.c.weights_out_dev ? a.c.batch * a.c.kv_heads * ((slots + kWeightSlots - 1) / kWeightSlots) : 0;
+  const int join = a.whole ? 0 : a.tokens * (a.c.heads / a.c.kv_heads);
+  const int weigh = a.c.weights_out_dev ? (a.c.pages * kPageTokens + kWeightSlots - 1) / kWeightSlots : 0;
   if (join + weigh == 0) return cudaSuccess;
-  return launch_pdl(cache_join_kernel<DH, T>, dim3(join + weigh), dim3(kJoinThreads), 0, s, true, a, C::kRows, pieces, join);
+  return launch_pdl(cache_join_kernel<DH, T>, dim3(join + weigh, a.c.kv_heads, a.c.batch), dim3(kJoinThreads), 0, s, true, a, C::kRows, join);
 }
 
 template <int DH, typename T>
@@ -957,12 +980,12 @@ CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c) {
     p.total += (bytes + 255) / 256 * 256;
     return at;
   };
-  p.prefix_off = take(2 * (kFewBatch + 1) * 4);
+  p.prefix_off = take((kFewBatch + 1) * 4);
+  p.units_off = take(units * 8);
   p.ml_off = take(static_cast<int64_t>(p.pieces) * 2 * p.tile_rows * 8);
   p.o_off = take(static_cast<int64_t>(p.pieces) * 2 * p.tile_rows * c.d_head * 4);
   p.lse_off = take(c.weights_out_dev ? units * p.tile_rows * 8 : 0);
   p.scores_off = take(c.weights_out_dev ? tiles * (4096 / c.d_head) * p.score_rows * 4 : 0);
-  p.line = tiles;
   return p;
 }
 
@@ -1008,6 +1031,7 @@ cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, c
       a.least = p.least;
       a.teams = p.teams;
       a.prefix = reinterpret_cast<int32_t*>(scratch + p.prefix_off);
+      a.unit_blocks = reinterpret_cast<int32_t*>(scratch + p.units_off);
       a.part_ml = reinterpret_cast<float2*>(scratch + p.ml_off);
       a.part_o = reinterpret_cast<float*>(scratch + p.o_off);
       const bool f32 = c.dtype == MTJ_F32;

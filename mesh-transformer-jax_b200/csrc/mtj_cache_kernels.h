@@ -14,7 +14,8 @@ struct CacheFewArgs {
   int score_rows;                          // rows of a key's scores
   int aligned, whole;                      // pieces end where units do; every unit is one piece
   int least, teams;                        // tiles of a piece at least, and the multiple that it is of
-  int32_t* prefix;                         // [2][kFewBatch + 1] tiles, and pieces, before each sequence
+  int32_t* prefix;                         // [kFewBatch + 1] tiles before each sequence
+  int32_t* unit_blocks;                    // [units][2] the first and the last block that worked on a unit
   float2* part_ml;                         // [pieces][2][tile rows]: maximum (base 2), sum
   float* part_o;                           // [pieces][2][tile rows][d_head]
   float2* lse;                             // [units][tile rows] of units that one block had, with weights
@@ -22,7 +23,7 @@ struct CacheFewArgs {
 };
 struct CacheFewPlan {
   int tokens, batch, tile_rows, pieces, score_rows, aligned, whole, least, teams;
-  int64_t line, prefix_off, ml_off, o_off, lse_off, scores_off, total;
+  int64_t prefix_off, units_off, ml_off, o_off, lse_off, scores_off, total;
 };
 CacheFewPlan plan_cache_few(const mtj_cache_attn_args& c);
 cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, char* scratch, cudaStream_t s);
