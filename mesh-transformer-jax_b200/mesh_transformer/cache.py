@@ -81,13 +81,11 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
     pool, table, device = _pool_shape(kpool, vpool, page_table, lengths)
     n_pages, kv_heads, _, d_head = pool
     batch, pages = table
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype not in _DTYPES or q.device != device:
+    shape = q.shape if isinstance(q, torch.Tensor) else ()
+    dtype = _DTYPES.get(q.dtype) if len(shape) == 4 else None
+    if dtype is None or q.device != device or shape[0] != batch or shape[3] != d_head or shape[1] < 1 or shape[2] < 1:
         raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
-    shape = q.shape
-    tokens, heads = shape[1], shape[2]
-    if shape[0] != batch or shape[3] != d_head or tokens < 1 or heads < 1:
-        raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
-    dtype = _DTYPES[q.dtype]
+    _, tokens, heads, _ = shape
     q, at_q, ld_q = _rows(q, "q", shape, q)
     at_k = at_v = ld_k = ld_v = 0
     if k is not None and v is not None:
@@ -113,7 +111,7 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
             _want(weights, "weights", torch.float32, slots, device)
             at_in = weights.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = torch.empty(batch, tokens, heads, d_head, dtype=q.dtype, device=device)
         at, ld_out = out.data_ptr(), heads * d_head
     else:
         given = out
@@ -161,7 +159,7 @@ def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, f
     _want(spare_pages, "spare_pages", torch.int32, (batch, (keep + PAGE_TOKENS - 1) // PAGE_TOKENS), device)
     if status is not None:
         _want(status, "status", torch.int32, (1,), device)
-    kept = torch.empty((batch, kv_heads, keep), dtype=torch.int32, device=device)
+    kept = torch.empty(batch, kv_heads, keep, dtype=torch.int32, device=device)
     lengths_out, weights_out, table_out = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(page_table)
     a = _EVICT_ARGS(
         kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), weights.data_ptr(), spare_pages.data_ptr(),

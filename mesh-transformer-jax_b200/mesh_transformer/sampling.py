@@ -101,22 +101,21 @@ _LOGIT_TYPES = {torch.float32: MTJ_F32, torch.bfloat16: MTJ_BF16}
 _VERIFY_ARGS = struct.Struct("@10P4q4if4x").pack           # mtj_verify_args, the fields of MtjVerifyArgs
 
 
-def _logit_rows(t, name, like, rows):
+def _logit_rows(t, name, like, shape):
     """``t`` [batch, rows, vocab] with unit stride inside a row; anything else is copied."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype != like.dtype or t.device != like.device or \
-            t.shape != (like.shape[0], rows, like.shape[2]):
-        raise ValueError(f"{name} must be a {like.dtype} tensor {[like.shape[0], rows, like.shape[2]]} on {like.device}")
-    s = t.stride()
-    if s[2] != 1 and t.shape[2] > 1 or s[1] < t.shape[2]:
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise ValueError(f"{name} must be a {like.dtype} tensor {list(shape)} on {like.device}")
+    vocab, s = shape[2], t.stride()
+    if s[2] != 1 and vocab > 1 or s[1] < vocab:
         t = t.contiguous()
         s = t.stride()
-    return t, max(s[1], t.shape[2]), s[0]
+    return t, max(s[1], vocab), s[0]
 
 
 def _plain_rows(t, name, dtype, shape, device):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
         raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on {device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, count=None, temp=1.0):
@@ -139,10 +138,10 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
         raise ValueError("target_logits must be a float32 or bfloat16 CUDA tensor [batch, drafts + 1, vocab]")
     batch, rows, vocab = target_logits.shape
     drafts, dev = rows - 1, target_logits.device
-    target, ld_target, batch_target = _logit_rows(target_logits, "target_logits", target_logits, rows)
+    target, ld_target, batch_target = _logit_rows(target_logits, "target_logits", target_logits, (batch, rows, vocab))
     draft, ld_draft, batch_draft = None, 0, 0
     if draft_logits is not None:
-        draft, ld_draft, batch_draft = _logit_rows(draft_logits, "draft_logits", target, drafts)
+        draft, ld_draft, batch_draft = _logit_rows(draft_logits, "draft_logits", target, (batch, drafts, vocab))
     tokens = _plain_rows(draft_tokens, "draft_tokens", torch.int32, (batch, drafts), dev)
     accept = _plain_rows(accept, "accept", torch.float32, (batch, drafts), dev)
     noise = _plain_rows(noise, "noise", torch.float32, (batch, vocab), dev)
@@ -151,9 +150,9 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
     temps = None
     if isinstance(temp, torch.Tensor):
         temps, temp = _plain_rows(temp, "temp", torch.float32, (batch,), dev), 1.0
-    out = torch.empty((batch, rows), dtype=torch.int32, device=dev)
-    taken = torch.empty((batch,), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((batch, rows), dtype=torch.float32, device=dev)
+    out = torch.empty(batch, rows, dtype=torch.int32, device=dev)
+    taken = torch.empty(batch, dtype=torch.int32, device=dev)
+    logprobs = torch.empty(batch, rows, dtype=torch.float32, device=dev)
     a = _VERIFY_ARGS(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else 0, tokens.data_ptr(),
                      accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else 0,
                      temps.data_ptr() if temps is not None else 0, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
@@ -170,5 +169,5 @@ def _run_verify(a, dev):
     nbytes = lib.mtj_verify_scratch_bytes(a)
     if nbytes < 0:
         raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
-    scratch = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     check(lib.mtj_verify_drafts(a, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev.index)))
