@@ -1,9 +1,12 @@
 // Attention of many new tokens over a paged cache (prompts and portions of prompts of mtj_k_cache_attn), on the tensor cores.
 //
-// A block has 256 query rows: two tiles of 128, two heads of one group at the same tokens, or where groups are odd 256 tokens of one
-// head (d_head 64 and 128), or one tile of 128 (d_head 256, whose accumulator fills tensor memory).  Keys come in blocks of 128 (two pages):
-// first those of the first tokens, then those of the window; a block of keys serves both tiles, so K and V cross from L2 once
-// for 256 rows.  A unit of work is one tile on one key block,
+// A job is 256 query rows: two tiles of 128, two heads of one group at the same tokens, or where groups are odd 256 tokens of one
+// head.  Keys come in blocks of 128 (two pages): first those of the first tokens, then those of the window; a block of keys serves
+// both tiles, so K and V cross from L2 once for 256 rows.  With d_head 64 and 128 one block has both tiles.  With d_head 256 an
+// accumulator fills tensor memory, and two blocks, a cluster of 2, have a tile each: their products are cta_group::2 ones, each holds
+// one page of K and half the columns of V, so that an SM reads 32 bytes a cycle (with a tile of its own 64, which is more than L2
+// gives 148 of them: 3900 cycles a block of keys instead of 2048 of products).  A unit of work is one tile (d_head 256: both) on one
+// key block,
 //     S[128, 128] = Q K^T        tcgen05, operands in shared memory by TMA (128-byte swizzle), fp32 in tensor memory
 //     P = 2^(S c - m)            a thread a row (d_head 256: two threads a row, 64 keys each), written over S as bf16
 //     O[128, d] += P V           P from tensor memory, V as MN-major operand straight from the pages
@@ -22,7 +25,7 @@
 // tokens: storing in a kernel before took 16 us, row by row beside the products it was longer than they were.)
 //
 // Scores, maxima, sums and O are 32-bit; P is rounded to bf16, half a step on average as large as the rounding of the output (a second
-// term would be half as many products again).  O is rescaled when a row's maximum has grown by more than 2^8.  The rows of V
+// term would be half as many products again).  O is rescaled when a row's scores have outgrown its reference, which waits for the products before.  The rows of V
 // behind the sequence, or of a page that does not exist, are zeroed in shared memory before they meet their zero weights.
 // Every wait is bounded.
 #include <cuda.h>
@@ -41,27 +44,30 @@ constexpr int kSoftThreads = 256;
 constexpr int kCopyThreads = 64;
 constexpr int kPromptThreads = kSoftThreads + 64 + kCopyThreads;      // and the warps of TMA and of the products
 constexpr int kBlockNotes = 8;
-constexpr int kPieces = 148;               // one block on each of a B200's SMs
+constexpr int kBlocks = 148;               // one on each of a B200's SMs
+constexpr int kMostPieces = kBlocks;       // pieces: one a block, or one a pair of blocks
 constexpr int kLeastBlocks = 4;            // of a piece that a job is cut into: the join costs about as much as three
 constexpr int kMostEntries = 8192;         // (sequence, token range) pairs of a launch
 constexpr int kJoinCost = 8;               // what cutting and joining costs, in key blocks of every piece
-constexpr int kPlanHead = 8, kPlanList = kPlanHead + kPieces * 8;      // places in the plan
+constexpr int kPlanHead = 8, kPlanList = kPlanHead + kMostPieces * 8;      // places in the plan
 constexpr int kSizeBins = 1024;
 constexpr int kPolyOf = 4;                 // of this many pairs of weights one is worked out on the multiply-add units
 constexpr float kExp0 = 0.99992806f, kExp1 = 0.69326097f, kExp2 = 0.24261114f, kExp3 = 0.05517167f;
 
+constexpr int kJobTiles = 2;
 template <int DH>
 struct PromptCfg {
-  static constexpr int kTiles = DH == 256 ? 1 : 2;
+  static constexpr bool kPair = DH == 256;
+  static constexpr int kTiles = kPair ? 1 : kJobTiles;           // of a block
   static constexpr int kKeysThread = kTiles == 2 ? 128 : 64;
-  static constexpr int kChunks = DH / 64;              // 64-column parts of a row
-  static constexpr int kHalves = kTiles;               // in which a thread announces its weights
+  static constexpr int kChunks = DH / 64;                        // 64-column parts of a row
+  static constexpr int kHalves = kTiles;                         // in which a thread announces its weights
+  static constexpr int kKPages = kPair ? 1 : 2;                  // of a block's keys that this block holds
+  static constexpr int kVChunks = kPair ? kChunks / 2 : kChunks;
   static constexpr uint32_t kQBytes = kTiles * kRowsT * DH * 2;
-  static constexpr uint32_t kKBytes = kKeysB * DH * 2;
-  // d_head 256: one block of keys, and values by the page
-  static constexpr int kKSlots = DH == 256 ? 1 : DH == 128 ? 2 : 4, kVSlots = DH == 256 ? 3 : DH == 128 ? 2 : 4;
-  static constexpr int kVPages = DH == 256 ? 1 : 2;    // of a slot
-  static constexpr uint32_t kVBytes = kVPages * kPageTokens * DH * 2;
+  static constexpr uint32_t kKBytes = kKPages * kPageTokens * DH * 2;
+  static constexpr uint32_t kVBytes = kKeysB * kVChunks * 128;
+  static constexpr int kKSlots = DH == 64 ? 4 : 2, kVSlots = DH == 64 ? 4 : DH == 128 ? 2 : 3;
   static constexpr uint32_t kSmem = kQBytes + kKSlots * kKBytes + kVSlots * kVBytes;
   static constexpr uint32_t kColS = 0, kColO = 256;    // tensor memory: S0 | S1 | O
   static constexpr uint32_t kTmemCols = 512;
@@ -110,6 +116,44 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+// the forms of a pair of blocks: arrivals in both, products over both blocks' operands and accumulators
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+      ::"r"(bar), "h"(static_cast<uint16_t>(3)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ss_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_pair(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// on the first block's barrier
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b32 x;\n\tmapa.shared::cluster.u32 x, %0, 0;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [x];\n\t}"
+      ::"r"(bar)
       : "memory");
 }
 // shared-memory matrix descriptor, 128-byte swizzle; lbo / sbo in bytes
@@ -165,6 +209,12 @@ __device__ __forceinline__ void exp2_pair(uint64_t x, float* y0, float* y1) {
   unpair(n, &n0, &n1);
   *y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
   *y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
+// 32 bytes in one store: a thread's part of a row fills whole sectors
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 // bits 0 .. n - 1
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
@@ -234,12 +284,12 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
 struct PromptArgs {
   mtj_cache_attn_args c;                   // pointers from the launch's first sequence on
   float scale_log2;
-  int by_heads, span;                      // a job's tiles are two heads; tokens of a job
+  int by_heads, span, pieces;              // a job's tiles are two heads; tokens of a job; pieces
   int head_jobs, token_jobs;               // jobs of a token range, token ranges of a sequence
-  int* plan;                               // whole jobs or not, jobs | [kPieces][8]: sequence, head job, token job, first key
+  int* plan;                               // whole jobs or not, jobs | [pieces][8]: sequence, head job, token job, first key
                                            // block, key blocks | entries by size
-  float2* part_ml;                         // [kPieces][2][tiles * 128]
-  float* part_o;                           // [kPieces][2][tiles * 128][d_head]
+  float2* part_ml;                         // [pieces][2][kJobTiles * 128]
+  float* part_o;                           // [pieces][2][kJobTiles * 128][d_head]
 };
 
 // The key blocks of a job: those with first tokens, then those of the window.  Places of keys: cached slots, up to a multiple of
@@ -329,9 +379,9 @@ __global__ void __launch_bounds__(kBeginThreads) cache_begin_kernel(const Prompt
   most = s_most;
   const int64_t line = static_cast<int64_t>(total) * a.head_jobs;
   const int64_t job_count = static_cast<int64_t>(all_jobs) * a.head_jobs;
-  const int64_t turns = (job_count + kPieces - 1) / kPieces;
-  const bool whole = job_count == 0 || max(static_cast<int64_t>(most), turns * line / job_count) <= line / kPieces + kJoinCost;
-  const bool cut_jobs = !whole && job_count <= kPieces / 2;
+  const int64_t turns = (job_count + a.pieces - 1) / a.pieces;
+  const bool whole = job_count == 0 || max(static_cast<int64_t>(most), turns * line / job_count) <= line / a.pieces + kJoinCost;
+  const bool cut_jobs = !whole && job_count <= a.pieces / 2;
   if (tid == 0) {
     a.plan[0] = whole ? 1 : 0;
     a.plan[1] = static_cast<int>(job_count);
@@ -356,11 +406,11 @@ __global__ void __launch_bounds__(kBeginThreads) cache_begin_kernel(const Prompt
     __syncthreads();
     for (int e = e0; e < e1; ++e)
       if (before[e] > 0) a.plan[kPlanList + atomicAdd(&bins[kSizeBins - min(before[e], kSizeBins)], 1)] = e;
-    if (tid < kPieces) a.plan[kPlanHead + tid * 8 + 4] = 0;
+    if (tid < a.pieces) a.plan[kPlanHead + tid * 8 + 4] = 0;
     return;
   }
-  // with pieces this wide they are at most kPieces
-  const int width = cut_jobs ? max(kLeastBlocks, static_cast<int>((line + kPieces - job_count - 1) / (kPieces - job_count))) : 0;
+  // with pieces this wide they are at most a.pieces
+  const int width = cut_jobs ? max(kLeastBlocks, static_cast<int>((line + a.pieces - job_count - 1) / (a.pieces - job_count))) : 0;
   if (cut_jobs) {
     mine = 0;
     for (int e = e0; e < e1; ++e) mine += before[e] = (before[e] + width - 1) / width;
@@ -374,8 +424,8 @@ __global__ void __launch_bounds__(kBeginThreads) cache_begin_kernel(const Prompt
   if (tid == 0) before[entries] = total;
   __syncthreads();
   const int64_t pieces_line = cut_jobs ? static_cast<int64_t>(total) * a.head_jobs : line;
-  if (tid < kPieces) {
-    const int64_t used = min(pieces_line, static_cast<int64_t>(kPieces));      // no piece before the last one is empty
+  if (tid < a.pieces) {
+    const int64_t used = min(pieces_line, static_cast<int64_t>(a.pieces));      // no piece before the last one is empty
     const int64_t at = cut_jobs || tid >= used ? tid : line * tid / used;
     int n = tid >= used ? 0 : cut_jobs ? 1 : static_cast<int>(line * (tid + 1) / used - at);
     int b = 0, head_job = 0, token_job = 0, j = 0;
@@ -415,16 +465,17 @@ __global__ void __launch_bounds__(kBeginThreads) cache_begin_kernel(const Prompt
   }
 }
 
-// A block's way through its jobs; every role of a block goes it on its own.
+// A block's (or pair's) way through its jobs; every role goes it on its own.
 struct Walk {
-  int b, head_job, token_job, j, left, turn, jobs;
+  int b, head_job, token_job, j, left, turn, jobs, piece;
   JobKeys k;
   int n;                                   // key blocks of the current job that belong to the block
-  __device__ __forceinline__ bool begin(const PromptArgs& a) {
+  __device__ __forceinline__ bool begin(const PromptArgs& a, int which) {
+    piece = which;
     turn = a.plan[0] ? 0 : -1;
     jobs = a.plan[1];
     if (turn >= 0) return take(a);
-    const int* p = a.plan + kPlanHead + blockIdx.x * 8;
+    const int* p = a.plan + kPlanHead + piece * 8;
     b = p[0];
     head_job = p[1];
     token_job = p[2];
@@ -435,7 +486,7 @@ struct Walk {
   }
   // whole jobs: turn by turn, every other turn from the last block to the first
   __device__ __forceinline__ bool take(const PromptArgs& a) {
-    const int64_t at = static_cast<int64_t>(turn) * kPieces + (turn & 1 ? kPieces - 1 - blockIdx.x : blockIdx.x);
+    const int64_t at = static_cast<int64_t>(turn) * a.pieces + (turn & 1 ? a.pieces - 1 - piece : piece);
     if (at >= jobs) return false;
     const int e = a.plan[kPlanList + at / a.head_jobs];
     b = e / a.token_jobs;
@@ -487,7 +538,7 @@ __device__ __forceinline__ void store_rows(const PromptArgs& a, int worker) {
   const int lane = threadIdx.x & 31;
   const int vecs = a.c.kv_heads * (DH / 8), stride = a.c.kv_heads * kPageTokens * (DH / 8);
   const int rows = a.c.batch * a.c.tokens;
-  for (int row = blockIdx.x * kStoreWarps + worker; row < rows; row += kPieces * kStoreWarps) {
+  for (int row = blockIdx.x * kStoreWarps + worker; row < rows; row += kBlocks * kStoreWarps) {
     const int b = row / a.c.tokens, t = row - b * a.c.tokens;
     const CacheSeq s = prompt_seq(a, b);
     JobKeys k;
@@ -531,8 +582,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
                                                                       const __grid_constant__ CUtensorMap map_v_new, const PromptArgs a) {
   using C = PromptCfg<DH>;
   constexpr int kTiles = C::kTiles, kKeysThread = C::kKeysThread, kHalves = C::kHalves;
+  constexpr bool kPair = C::kPair;
+  constexpr int kBars = 2 + 2 * C::kKSlots + 2 * C::kVSlots + 10, kPeerBars = kPair ? 1 + C::kKSlots + C::kVSlots : 0;
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
-  __shared__ __align__(8) uint64_t bars[2 + 2 * C::kKSlots + 2 * C::kVSlots + 10];
+  __shared__ __align__(8) uint64_t bars[kBars + kPeerBars];
   __shared__ uint32_t tmem_slot, failed;
   __shared__ int to_store[C::kKSlots + C::kVSlots][2];      // rows of the pools that a slot's pages of new rows go to
   __shared__ int notes[kBlockNotes];                   // valid rows of a key block's pages: first | second << 8
@@ -544,22 +597,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   const uint32_t q_full = bar0, q_empty = bar0 + 8, k_full = bar0 + 16, k_empty = k_full + 8 * C::kKSlots, v_full = k_empty + 8 * C::kKSlots,
                  v_empty = v_full + 8 * C::kVSlots, s_full = v_empty + 8 * C::kVSlots, p_full = s_full + 16, p_half = p_full + 16,
                  o_done = p_half + 16, o_free = o_done + 16;
+  // the first block of a pair: the other one has its part
+  const uint32_t q_peer = bar0 + 8 * kBars, k_peer = q_peer + 8, v_peer = k_peer + 8 * C::kKSlots;
+  const uint32_t rank = kPair ? pair_rank() : 0;
+  const int piece = kPair ? blockIdx.x >> 1 : blockIdx.x;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 + 2 * C::kKSlots + 2 * C::kVSlots + 10; ++i) mbar_init(bar0 + 8u * i, 1);
+    for (int i = 0; i < kBars + kPeerBars; ++i) mbar_init(bar0 + 8u * i, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(p_full + 8u * i, kSoftThreads / kTiles);
-      mbar_init(p_half + 8u * i, kSoftThreads / kTiles);
-      mbar_init(o_free + 8u * i, kSoftThreads / kTiles);
+      constexpr int kArrivals = kPair ? 2 * kSoftThreads / 32 : kSoftThreads / kTiles;      // a pair: both blocks' warps
+      mbar_init(p_full + 8u * i, kArrivals);
+      mbar_init(p_half + 8u * i, kArrivals);
+      mbar_init(o_free + 8u * i, kArrivals);
     }
     mbar_fence_init();
     failed = 0;
   }
   if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(C::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   fence_before();
-  __syncthreads();
+  if constexpr (kPair) pair_sync();                    // both blocks' barriers exist before either is signalled
+  else __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_wait();
@@ -570,11 +634,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     // registers: 8 warps of 200 and 4 of 88 are 62464 of the 64512 that the block is launched with
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     Walk w;
-    const bool work = w.begin(a);
+    const bool work = w.begin(a, piece);
   if (warp == 8) {
     // ---- TMA ----
     if (lane == 0 && work) {
       int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
+      constexpr int kKChunk = C::kKPages * kPageTokens * 128;      // bytes of 64 columns of a slot of keys
+      const int v_chunk0 = kPair ? rank * C::kVChunks : 0;
       uint32_t storing_k = 0, storing_v = 0;               // slots with rows to store
       bool ok = true;
       // a slot's new rows go to their pages when the products have read it, before it is filled again
@@ -582,21 +648,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         const int* rows = to_store[st];
         storing_k &= ~(1u << st);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < C::kKPages; ++h)
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
-            if (rows[h] >= 0) tma_store(&map_k, c * 64, rows[h], sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128));
+            if (rows[h] >= 0) tma_store(&map_k, c * 64, rows[h], sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128));
         asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       };
       auto store_v = [&](int st) {
         const int* rows = to_store[C::kKSlots + st];
         storing_v &= ~(1u << st);
 #pragma unroll
-        for (int h = 0; h < C::kVPages; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
+          for (int c = 0; c < C::kVChunks; ++c)
             if (rows[h] >= 0)
-              tma_store(&map_v, c * 64, rows[h], sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128));
+              tma_store(&map_v, (v_chunk0 + c) * 64, rows[h], sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128));
         asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       };
       do {
@@ -608,8 +674,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
-            tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t : 0)) * DH + c * 64,
-                    w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : t * kRowsT), q_full);
+            tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t + rank : 0)) * DH + c * 64,
+                    w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : (t + rank) * kRowsT), q_full);
         const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
         // a key block's pages, or its rows of new tokens: the row where each 64 begin, how many hold something, the page they are stored
         // to; looked up before the slot is waited for, because the products wait for what comes behind that
@@ -657,14 +723,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           if (storing_k >> st & 1u) store_k(st);
           mbar_expect_tx(k_full + 8 * st, C::kKBytes);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < C::kKPages; ++h)
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c)
-              tma_box(sK + st * C::kKBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), map, col + c * 64, x.row[h], k_full + 8 * st);
-          if (x.target[0] >= 0 || x.target[1] >= 0) {
+              tma_box(sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128), map, col + c * 64, kPair && rank ? x.row[1] : x.row[h],
+                      k_full + 8 * st);
+          const int t0 = kPair && rank ? x.target[1] : x.target[0], t1 = kPair ? -1 : x.target[1];
+          if (t0 >= 0 || t1 >= 0) {
             storing_k |= 1u << st;
-            to_store[st][0] = x.target[0];
-            to_store[st][1] = x.target[1];
+            to_store[st][0] = t0;
+            to_store[st][1] = t1;
           }
           ++kc;
           return true;
@@ -672,24 +740,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         auto load_v = [&](const Block& x) {
           const CUtensorMap* map = x.cached ? &map_v : &map_v_new;
           const int col = x.cached ? 0 : kvh * DH;
-          for (int i = 0; i < 2 / C::kVPages; ++i, ++vc) {
-            const int st = vc % C::kVSlots;
-            if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
-            if (storing_v >> st & 1u) store_v(st);
-            mbar_expect_tx(v_full + 8 * st, C::kVBytes);
+          const int st = vc % C::kVSlots;
+          if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
+          if (storing_v >> st & 1u) store_v(st);
+          mbar_expect_tx(v_full + 8 * st, C::kVBytes);
 #pragma unroll
-            for (int h = 0; h < C::kVPages; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int c = 0; c < C::kChunks; ++c)
-                tma_box(sV + st * C::kVBytes + c * (C::kVPages * kPageTokens * 128) + h * (kPageTokens * 128), map, col + c * 64,
-                        x.row[C::kVPages == 2 ? h : i], v_full + 8 * st);
-            const int t0 = x.target[C::kVPages == 2 ? 0 : i], t1 = C::kVPages == 2 ? x.target[1] : -1;
-            if (t0 >= 0 || t1 >= 0) {
-              storing_v |= 1u << st;
-              to_store[C::kKSlots + st][0] = t0;
-              to_store[C::kKSlots + st][1] = t1;
-            }
+            for (int c = 0; c < C::kVChunks; ++c)
+              tma_box(sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), map, col + (v_chunk0 + c) * 64, x.row[h], v_full + 8 * st);
+          if (x.target[0] >= 0 || x.target[1] >= 0) {
+            storing_v |= 1u << st;
+            to_store[C::kKSlots + st][0] = x.target[0];
+            to_store[C::kKSlots + st][1] = x.target[1];
           }
+          ++vc;
           return true;
         };
         // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...; the softmax warps' note of a block is written
@@ -722,63 +787,92 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     }
   } else if (warp == 9) {
     // ---- products ----
-    if (work) {
+    if (kPair && rank != 0) {
+      // the second block of a pair tells the first what has landed, in the order in which the products want it
+      if (lane == 0 && work) {
+        int kc = 0, vc = 0, seg = 0;
+        bool ok = true;
+        auto tell = [&](uint32_t full, uint32_t peer, int n, int slots) {
+          ok = ok && mbar_wait(full + 8 * (n % slots), (n / slots) & 1);
+          if (ok) arrive_first(peer + 8 * (n % slots));
+        };
+        do {
+          tell(q_full, q_peer, seg++, 1);
+          tell(k_full, k_peer, kc++, C::kKSlots);
+          for (int j = 0; ok && j < w.n; ++j) {
+            if (j + 1 < w.n) tell(k_full, k_peer, kc++, C::kKSlots);
+            tell(v_full, v_peer, vc++, C::kVSlots);
+          }
+        } while (ok && w.next(a));
+        if (!ok) atomicOr(&failed, 1u);
+      }
+    } else if (work) {
       const uint32_t leader = elected();
       auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
-      constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kRowsT >> 4) << 24);
-      constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kRowsT >> 4) << 24);
-      int k0 = 0, v0 = 0, u0 = 0, seg = 0;                 // key blocks, value slots, units and jobs before the current job
+      auto commit = [&](uint32_t bar) {
+        if constexpr (kPair) commit_pair(bar, leader);
+        else commit_to(bar, leader);
+      };
+      constexpr uint32_t kM = kPair ? 2 * kRowsT : kRowsT;
+      constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kM >> 4) << 24);
+      constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kM >> 4) << 24);
+      int k0 = 0, u0 = 0, seg = 0;                         // key blocks, units and jobs before the current job
       bool ok = true;
       do {
         // the same in all lanes, and known to be: what hangs on it stays in uniform registers
         const int blocks = __reduce_max_sync(0xffffffffu, w.n), units = blocks * kTiles;
         auto issue_s = [&](int u) {
           const int j = k0 + u / kTiles, t = u % kTiles, st = j % C::kKSlots, buf = (u0 + u) & 1;
-          if (t == 0 && !wait(k_full + 8 * st, (j / C::kKSlots) & 1)) return false;
+          const uint32_t parity = (j / C::kKSlots) & 1;
+          if (t == 0 && !wait(k_full + 8 * st, parity)) return false;
+          if (kPair && !wait(k_peer + 8 * st, parity)) return false;
           fence_after();
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c) {
             const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
-            const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (kKeysB * 128), 16, 1024);
+            const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (C::kKPages * kPageTokens * 128), 16, 1024);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ss(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (kPair) mma_ss_pair(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+              else mma_ss(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+            }
           }
-          commit_to(s_full + 8 * buf, leader);
-          if (t == kTiles - 1) commit_to(k_empty + 8 * st, leader);
-          if (u == units - 1) commit_to(q_empty, leader);
+          commit(s_full + 8 * buf);
+          if (t == kTiles - 1) commit(k_empty + 8 * st);
+          if (u == units - 1) commit(q_empty);
           return true;
         };
         auto issue_pv = [&](int u) {
-          const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1;
-          const uint32_t parity = ((u0 + u) >> 1) & 1;
+          const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1, n = k0 + j, st = n % C::kVSlots;
+          const uint32_t parity = ((u0 + u) >> 1) & 1, landed = (n / C::kVSlots) & 1;
           // the accumulator's last job has been read
           if (seg > 0 && u < kTiles && !wait(o_free + 8 * t, (seg - 1) & 1)) return false;
           if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
+          if (t == 0 && !wait(v_full + 8 * st, landed)) return false;
+          if (kPair && !wait(v_peer + 8 * st, landed)) return false;
+          const uint64_t vd = smem_desc(sV + st * C::kVBytes, kKeysB * 128, 1024);
+          const uint32_t pa = tmem + C::kColS + buf * kKeysB;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {                    // by the page: the second half of the weights comes later
             if (C::kHalves == 2 && h == 1 && !wait(p_full + 8 * buf, parity)) return false;
-            const int n = v0 + (C::kVPages == 2 ? j : 2 * j + h), st = n % C::kVSlots;
-            if (t == 0 && (C::kVPages == 1 || h == 0) && !wait(v_full + 8 * st, (n / C::kVSlots) & 1)) return false;
             fence_after();
-            const uint64_t vd = smem_desc(sV + st * C::kVBytes, C::kVPages * kPageTokens * 128, 1024);
-            const uint32_t pa = tmem + C::kColS + buf * kKeysB + h * (kPageTokens / 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>(((C::kVPages == 2 ? h * 4 + k : k) * 2048) >> 4), kIdO,
-                     (j | h | k) ? 1u : 0u, leader);
-            if (t == kTiles - 1 && (C::kVPages == 1 || h == 1)) commit_to(v_empty + 8 * st, leader);
+            for (int k = 4 * h; k < 4 * h + 4; ++k) {
+              if constexpr (kPair) mma_ts_pair(tmem + C::kColO, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | k) ? 1u : 0u, leader);
+              else mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | k) ? 1u : 0u, leader);
+            }
           }
-          commit_to(o_done + 8 * buf, leader);
+          if (t == kTiles - 1) commit(v_empty + 8 * st);
+          commit(o_done + 8 * buf);
           return true;
         };
-        ok = wait(q_full, seg & 1) && issue_s(0);
+        ok = wait(q_full, seg & 1) && (!kPair || wait(q_peer, seg & 1)) && issue_s(0);
         if (ok && units > 1) ok = issue_s(1);
         for (int u = 0; ok && u < units; ++u) {
           ok = issue_pv(u);
           if (ok && u + 2 < units) ok = issue_s(u + 2);
         }
         k0 += blocks;
-        v0 += blocks * (2 / C::kVPages);
         u0 += units;
         ++seg;
       } while (__any_sync(0xffffffffu, ok && w.next(a)));
@@ -792,16 +886,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     // ---- weights ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     Walk w;
-    if (w.begin(a)) {
+    if (w.begin(a, piece)) {
     const int wg = warp >> 2, quad = warp & 3;
-    const int tile = kTiles == 2 ? wg : 0, part = kTiles == 2 ? 0 : wg;      // of the keys of a block
+    const int tile = kTiles == 2 ? wg : 0, part = kTiles == 2 ? 0 : wg;      // of this block; of the keys of a block
+    const int job_tile = kPair ? rank : tile;
+    auto announce = [&](uint32_t bar) {
+      fence_before();
+      if constexpr (kPair) {
+        __syncwarp();
+        if (lane == 0) arrive_first(bar);
+      } else {
+        arrive_at(bar);
+      }
+    };
     const int r = quad * 32 + lane;                        // row of the tile = lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     int block = 0;                                         // key blocks so far
     bool ok = true;
     do {
-      const int head = w.head_job * (a.by_heads ? 2 : 1) + (a.by_heads ? tile : 0);
-      const int t0 = w.k.t_first + (a.by_heads ? 0 : tile * kRowsT), t = t0 + r;
+      const int head = w.head_job * (a.by_heads ? 2 : 1) + (a.by_heads ? job_tile : 0);
+      const int t0 = w.k.t_first + (a.by_heads ? 0 : job_tile * kRowsT), t = t0 + r;
       const int p = t < w.k.fresh ? w.k.first + t : -1;
       const int p_last = w.k.first + w.k.t_end - 1;
       const int warp_first = w.k.first + t0 + quad * 32;   // slots of the warp's rows: warp_first .. + 31
@@ -822,17 +926,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         constexpr int kFullNote = kPageTokens | kPageTokens << 8;
         // V's rows that hold nothing: zeroed before anybody's weights are announced
         if (note != kFullNote) {
-#pragma unroll
-          for (int i = 0; i < 2 / C::kVPages; ++i) {
-            const int n = block * (2 / C::kVPages) + i, st = n % C::kVSlots;
-            if (ok) ok = mbar_wait(v_full + 8 * st, (n / C::kVSlots) & 1);
-            if (tile == 0) {
-              // [64-column part][page][64 rows][128 bytes]
-              for (int e = threadIdx.x; e < static_cast<int>(C::kVBytes / 16); e += kSoftThreads / kTiles) {
-                const int row = e / 8 % kPageTokens, h = C::kVPages == 2 ? e / 8 / kPageTokens % 2 : i;
-                if (row >= ((note >> (8 * h)) & 255))
-                  *reinterpret_cast<uint4*>(prompt_smem + (sV - base) + st * C::kVBytes + e * 16) = make_uint4(0, 0, 0, 0);
-              }
+          const int st = block % C::kVSlots;
+          if (ok) ok = mbar_wait(v_full + 8 * st, (block / C::kVSlots) & 1);
+          if (tile == 0) {
+            // [64-column part][page][64 rows][128 bytes]
+            for (int e = threadIdx.x; e < static_cast<int>(C::kVBytes / 16); e += kSoftThreads / kTiles) {
+              const int row = e / 8 % kPageTokens, h = e / 8 / kPageTokens % 2;
+              if (row >= ((note >> (8 * h)) & 255))
+                *reinterpret_cast<uint4*>(prompt_smem + (sV - base) + st * C::kVBytes + e * 16) = make_uint4(0, 0, 0, 0);
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -865,8 +966,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           top = fmaxf(top, part_max[part ^ 1][r]);
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
         }
+        // the reference stays until a score is 2^8 above it, and is then put 2^8 above that score: weights are below 2^8, and a row whose
+        // first keys are poor ones (a few first tokens, the edge of its window) does not have O rescaled for its next ones
         float m_new = m_ref;
-        if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top;
+        if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top + 8.0f;
         const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
         if (__any_sync(0xffffffffu, corr != 1.0f)) {
           // O changes scale: the tile's products so far must have landed
@@ -908,8 +1011,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
 #pragma unroll
           for (int i = half * (kKeysThread / kHalves / 2); i < (half + 1) * (kKeysThread / kHalves / 2); i += 32) tmem_store32(at_p + i, x + i);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          fence_before();
-          arrive_at((half < kHalves - 1 ? p_half : p_full) + 8 * (u & 1));
+          announce((half < kHalves - 1 ? p_half : p_full) + 8 * (u & 1));
         }
         float sum0, sum1;
         unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
@@ -928,40 +1030,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       }
       const bool whole = w.whole();
       const float inv = l > 0.f ? 1.0f / l : 0.f;
-      const size_t part_row = (static_cast<size_t>(blockIdx.x) * 2 + (w.j == 0 ? 1 : 0)) * (kTiles * kRowsT) + tile * kRowsT + r;
+      const bool wide_out = ((reinterpret_cast<uintptr_t>(a.c.out_dev) & 31) | (a.c.ld_out & 15)) == 0;
+      const size_t part_row = (static_cast<size_t>(piece) * 2 + (w.j == 0 ? 1 : 0)) * (kJobTiles * kRowsT) + job_tile * kRowsT + r;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(w.b) * a.c.tokens + min(t, a.c.tokens - 1)) * a.c.ld_out + head * DH;
 #pragma unroll 1
       for (int c0 = part * (DH / 2); c0 < (kTiles == 2 ? DH : (part + 1) * (DH / 2)); c0 += 32) {
         uint32_t o[32];
         tmem_load32(tmem + lanes + C::kColO + tile * DH + c0, o);
         if (whole && p >= 0) {
+          uint32_t y[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float v[8];
+          for (int i = 0; i < 16; ++i) y[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          if (wide_out) {
+            store32(out + c0, y);
+            store32(out + c0 + 16, y + 8);
+          } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[i + e]);
-            store8(out + c0 + i, v, inv);
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(out + c0 + 2 * i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
           }
         } else if (!whole) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + part_row * DH + c0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          for (int i = 0; i < 32; i += 8) store32(a.part_o + part_row * DH + c0 + i, o + i);
         }
       }
       if (!whole && part == 0) a.part_ml[part_row] = make_float2(m_ref, l);
-      fence_before();
-      arrive_at(o_free + 8 * tile);
+      announce(o_free + 8 * tile);
     } while (w.next(a));
     if (!ok) atomicOr(&failed, 1u);
     }
     if (a.c.k_new_dev) store_rows<DH>(a, 2 + warp);
   }
   fence_before();
-  __syncthreads();
+  if constexpr (kPair) pair_sync();                    // neither block leaves, or frees, while the other may still signal it
+  else __syncthreads();
   if (warp == 9) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+    if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
   }
   if (threadIdx.x == 0 && failed && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
 }
@@ -971,7 +1076,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
 constexpr int kPartRows = 8;
 template <int DH>
 __global__ void __launch_bounds__(32 * kPartRows) cache_part_kernel(const PromptArgs a) {
-  constexpr int kRows = PromptCfg<DH>::kTiles * kRowsT, kVecs = DH / 128 > 0 ? DH / 128 : 1;
+  constexpr int kRows = kJobTiles * kRowsT, kVecs = DH / 128 > 0 ? DH / 128 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
@@ -985,7 +1090,7 @@ __global__ void __launch_bounds__(32 * kPartRows) cache_part_kernel(const Prompt
   if (p[4] <= 0 || p[3] == 0) return;                                  // no piece, or one that begins a job
   if (same_job(piece - 1) && plan[(piece - 1) * 8 + 3] != 0) return;     // not the first inside its job
   int n = 2;
-  while (piece + n - 1 < kPieces && same_job(piece + n - 1) && plan[(piece + n - 1) * 8 + 3] != 0) ++n;
+  while (piece + n - 1 < a.pieces && same_job(piece + n - 1) && plan[(piece + n - 1) * 8 + 3] != 0) ++n;
   const int r = blockIdx.x * kPartRows + warp, tile = r / kRowsT;
   const CacheSeq s = prompt_seq(a, p[0]);
   const int t = p[2] * a.span + (a.by_heads ? r % kRowsT : r);
@@ -1041,16 +1146,30 @@ cudaError_t launch(PromptArgs a, bool join, cudaStream_t s) {
     e = once.run([&] { return cudaFuncSetAttribute(cache_prompt_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem)); });
   if (e != cudaSuccess) return e;
   e = launch_pdl(cache_begin_kernel, dim3(1 + static_cast<unsigned>((rows + kZeroRows - 1) / kZeroRows)), dim3(kBeginThreads), 0, s, false, a);
-  if (e == cudaSuccess) e = launch_pdl(cache_prompt_kernel<DH>, dim3(kPieces), dim3(kPromptThreads), C::kSmem, s, true, mq, mk, mv, mkn, mvn, a);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kBlocks);
+  cfg.blockDim = dim3(kPromptThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {2, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = C::kPair ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, cache_prompt_kernel<DH>, mq, mk, mv, mkn, mvn, a);
   if (e == cudaSuccess && join)
-    e = launch_pdl(cache_part_kernel<DH>, dim3(C::kTiles * kRowsT / kPartRows, kPieces - 1), dim3(32 * kPartRows), 0, s, true, a);
+    e = launch_pdl(cache_part_kernel<DH>, dim3(kJobTiles * kRowsT / kPartRows, a.pieces - 1), dim3(32 * kPartRows), 0, s, true, a);
   return e;
 }
 
-bool pairs_heads(const mtj_cache_attn_args& c) { return c.d_head < 256 && (c.heads / c.kv_heads) % 2 == 0; }
-int job_span(const mtj_cache_attn_args& c) { return c.d_head < 256 && !pairs_heads(c) ? 2 * kRowsT : kRowsT; }
+bool pairs_heads(const mtj_cache_attn_args& c) { return (c.heads / c.kv_heads) % 2 == 0; }
+int job_span(const mtj_cache_attn_args& c) { return pairs_heads(c) ? kRowsT : kJobTiles * kRowsT; }
+int pieces_for(const mtj_cache_attn_args& c) { return c.d_head == 256 ? kBlocks / 2 : kBlocks; }      // pairs of blocks, blocks
 constexpr int64_t kPlanBytes = ((kPlanList + kMostEntries) * 4 + 255) / 256 * 256;
-int64_t part_rows(const mtj_cache_attn_args& c) { return static_cast<int64_t>(kPieces) * 2 * (c.d_head < 256 ? 2 : 1) * kRowsT; }
+int64_t part_rows(const mtj_cache_attn_args& c) { return static_cast<int64_t>(pieces_for(c)) * 2 * kJobTiles * kRowsT; }
 
 // whether no job can lie in several pieces: jobs of few blocks are taken whole
 bool all_whole(const mtj_cache_attn_args& c) {
@@ -1071,6 +1190,7 @@ cudaError_t run_cache_prompt(const mtj_cache_attn_args& c, char* scratch, cudaSt
   a.scale_log2 = c.scale * 1.4426950408889634f;
   a.by_heads = pairs_heads(c);
   a.span = job_span(c);
+  a.pieces = pieces_for(c);
   a.head_jobs = c.heads / (a.by_heads ? 2 : 1);
   a.token_jobs = (c.tokens + a.span - 1) / a.span;
   a.plan = reinterpret_cast<int*>(scratch);
