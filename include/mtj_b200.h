@@ -483,7 +483,8 @@ int32_t mtj_k_decode_attn_noalloc(const float* q_dev, const void* kpool_dev, con
  * weights_in_dev NULL standing for zeros; both may be the same array.
  * A sequence whose length is negative, below its new_tokens or beyond its pages is treated as empty, a page number outside
  * [0, n_pages) as a page that nobody sees; either sets bit 1 of *status_dev (may be NULL), a bounded wait that runs out
- * bit 0.  Queries of one call see the values of all its tokens multiplied by weight zero, so new values must be finite.
+ * bit 0.  A slot that none of a sequence's new tokens sees may hold anything and its page need not exist (page_table -1);
+ * what some of them see, the others multiply by weight zero, so values in sight must be finite.
  * d_head 64, 128 or 256; at most MTJ_CACHE_MAX_GROUP query heads per key head.  The scratch needs no initial contents.
  * Calls that may overlap need scratch of their own. */
 #define MTJ_CACHE_MAX_GROUP 64

@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
     const int n_tiles = min(s.tiles - tile0, end - x);
     const int kvh = unit / row_tiles, row0 = unit % row_tiles * kRows;
     const int first = s.length - s.fresh;                                // slot of the slice's first token
+    const int low = cache_window_low(first, a.c.window);                 // and the first of its window
 
     // queries as the B operand: fragment (term, n tile, k step, lane); a thread brings 8 numbers of a row
     constexpr int kPieces = kRows * (DH / 8), kEach = (kPieces + 32 * kWorkers - 1) / (32 * kWorkers);
@@ -476,14 +477,14 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
       const int slot0 = tile_slot[st] + key0;
       if (tile_slot[st] >= 0) {
         const uint32_t sk = ring + st * kTileBytes, sv = sk + kTileBytes / 2;
-        // slots of new tokens and slots behind the sequence
-        if (slot0 + 16 * kSub > first) {
+        // slots of new tokens, and values that nobody sees: behind the sequence, or between the first tokens and the window
+        if (slot0 + 16 * kSub > first || (slot0 < low && slot0 + 16 * kSub > a.c.sinks)) {
           unsigned char* pk = ring_ptr + st * kTileBytes;
           const size_t page = static_cast<size_t>(tile_page[st]) * a.c.kv_heads + kvh;
           for (int v = lane; v < 16 * kSub * (DH / 8); v += 32) {
             const int r = v / (DH / 8), piece = v % (DH / 8), j = slot0 + r, t = j - first;
             const uint32_t at = piece_at<kKeys>(key0 + r, piece);
-            if (j >= s.length) {
+            if (j >= s.length || (j >= a.c.sinks && j < low)) {
               *reinterpret_cast<uint4*>(pk + kTileBytes / 2 + at) = make_uint4(0, 0, 0, 0);
             } else if (t >= 0 && a.c.k_new_dev) {
               const size_t row = static_cast<size_t>(b) * a.c.tokens + a.t0 + t;
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
 #pragma unroll
       for (int w = 0; w < C::kParts; ++w) sum += sm_m[w][r] == -INFINITY ? 0.f : sm_l[w][r] * exp2_fast(sm_m[w][r] - top);
       if (whole_unit) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
         if (row0 + r < rows) {
           T* out = static_cast<T*>(a.c.out_dev) + (static_cast<size_t>(b) * a.c.tokens + a.t0 + t) * a.c.ld_out +
                    (kvh * group + row0 + r - t * group) * DH + d;
@@ -828,7 +829,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
         v[7] += y.w;
         l += sm_l[k];
       }
-      store8(out + tid * 8, v, l > 0.f ? 1.f / l : 0.f);
+      store8(out + tid * 8, v, l != 0.f ? 1.f / l : 0.f);
     }
     return;
   }
@@ -878,7 +879,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
       }
       if (lane == 0) {
         row_m[r] = top == -INFINITY ? 0.f : top;
-        row_inv[r] = l > 0.f ? 1.f / l : 0.f;
+        row_inv[r] = l != 0.f ? 1.f / l : 0.f;
       }
     }
     __syncthreads();

@@ -189,9 +189,10 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// NaN if one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // 2^x of a pair on the multiply-add units, for x in [-126, 9]: x = n + f with |f| <= 1/2 by adding and taking away 1.5 * 2^23, a
@@ -298,6 +299,7 @@ struct JobKeys {
   int t_first, t_end;                      // its tokens
   int fresh, first;                        // new tokens, slot of the first of them
   int cached, tail;                        // slots that are read from pages; the first place of the call's tokens
+  int low, sinks;                          // slots from sinks on and below low are seen by none of its tokens
   int low_block, sink_blocks, blocks;
   __device__ __forceinline__ int place(int j) const { return (j < sink_blocks ? j : low_block + j - sink_blocks) * kKeysB; }
   __device__ __forceinline__ int slot_of(int place) const { return place < tail ? place : place - tail + cached; }
@@ -311,9 +313,10 @@ __device__ __forceinline__ JobKeys job_keys(const PromptArgs& a, const CacheSeq&
   k.tail = (k.cached + kKeysB - 1) / kKeysB * kKeysB;
   k.t_first = token_job * a.span;
   k.t_end = min(s.fresh, k.t_first + a.span);
-  const int low = cache_window_low(k.first + k.t_first, a.c.window), sinks = min(a.c.sinks, low);
-  k.low_block = k.place_of(low) / kKeysB;
-  k.sink_blocks = sinks > 0 ? min(k.place_of(sinks - 1) / kKeysB + 1, k.low_block) : 0;
+  k.low = cache_window_low(k.first + k.t_first, a.c.window);
+  k.sinks = min(a.c.sinks, k.low);
+  k.low_block = k.place_of(k.low) / kKeysB;
+  k.sink_blocks = k.sinks > 0 ? min(k.place_of(k.sinks - 1) / kKeysB + 1, k.low_block) : 0;
   k.blocks = k.t_end > k.t_first ? k.sink_blocks + k.place_of(k.first + k.t_end - 1) / kKeysB - k.low_block + 1 : 0;
   return k;
 }
@@ -704,7 +707,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
               continue;
             }
             const int at = place / kPageTokens + h;
-            x.valid[h] = min(kPageTokens, max(0, w.k.cached - at * kPageTokens));
+            const bool seen = at * kPageTokens < w.k.sinks || (at + 1) * kPageTokens > w.k.low;
+            x.valid[h] = seen ? min(kPageTokens, max(0, w.k.cached - at * kPageTokens)) : 0;
             int page = x.valid[h] > 0 ? table[at] : 0;
             if (!cache_page_ok(page, a.c.n_pages)) {
               // not read: page 0 stands in, nobody sees its scores
@@ -924,16 +928,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
 #pragma unroll
         for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
         constexpr int kFullNote = kPageTokens | kPageTokens << 8;
-        // V's rows that hold nothing: zeroed before anybody's weights are announced
-        if (note != kFullNote) {
+        // V's rows that hold nothing, or nothing that a token of the job sees: zeroed before anybody's weights are announced
+        const int slot0 = key - part * kKeysThread;
+        if (note != kFullNote || (slot0 < w.k.low && slot0 + kKeysB > w.k.sinks)) {
           const int st = block % C::kVSlots;
           if (ok) ok = mbar_wait(v_full + 8 * st, (block / C::kVSlots) & 1);
           if (tile == 0) {
-            // [64-column part][page][64 rows][128 bytes]
-            for (int e = threadIdx.x; e < static_cast<int>(C::kVBytes / 16); e += kSoftThreads / kTiles) {
-              const int row = e / 8 % kPageTokens, h = e / 8 / kPageTokens % 2;
-              if (row >= ((note >> (8 * h)) & 255))
-                *reinterpret_cast<uint4*>(prompt_smem + (sV - base) + st * C::kVBytes + e * 16) = make_uint4(0, 0, 0, 0);
+            // [64-column part][page][64 rows][128 bytes]: a thread has a row of some parts, its pieces in an order that meets all banks
+            const int h = r / kPageTokens, row = r % kPageTokens, slot = slot0 + r;
+            if (row >= ((note >> (8 * h)) & 255) || (slot >= w.k.sinks && slot < w.k.low)) {
+              unsigned char* at = prompt_smem + (sV - base) + st * C::kVBytes + r * 128;
+              for (int c = kTiles == 1 ? wg : 0; c < C::kVChunks; c += 3 - kTiles)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(at + c * (kKeysB * 128) + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -959,17 +966,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         for (int i = 0; i < kKeysThread; i += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;      // scale > 0
+        float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * a.scale_log2;      // scale > 0
         if constexpr (kTiles == 1) {
           part_max[part][r] = top;
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-          top = fmaxf(top, part_max[part ^ 1][r]);
+          top = max3(top, part_max[part ^ 1][r], top);
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
         }
         // the reference stays until a score is 2^8 above it, and is then put 2^8 above that score: weights are below 2^8, and a row whose
         // first keys are poor ones (a few first tokens, the edge of its window) does not have O rescaled for its next ones
         float m_new = m_ref;
-        if (top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY)) m_new = top + 8.0f;
+        if (!(top <= m_ref + 8.0f)) m_new = top + 8.0f;     // a score that is NaN makes the row NaN: the reference, and with it the sum
         const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
         if (__any_sync(0xffffffffu, corr != 1.0f)) {
           // O changes scale: the tile's products so far must have landed
@@ -1029,7 +1036,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         l = part_max[0][r] + part_max[1][r];
       }
       const bool whole = w.whole();
-      const float inv = l > 0.f ? 1.0f / l : 0.f;
+      const float inv = m_ref == -INFINITY ? 0.f : 1.0f / l;
       const bool wide_out = ((reinterpret_cast<uintptr_t>(a.c.out_dev) & 31) | (a.c.ld_out & 15)) == 0;
       const size_t part_row = (static_cast<size_t>(piece) * 2 + (w.j == 0 ? 1 : 0)) * (kJobTiles * kRowsT) + job_tile * kRowsT + r;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(w.b) * a.c.tokens + min(t, a.c.tokens - 1)) * a.c.ld_out + head * DH;
@@ -1116,7 +1123,7 @@ __global__ void __launch_bounds__(32 * kPartRows) cache_part_kernel(const Prompt
       o[4 * v + 3] = fmaf(y.w, f, o[4 * v + 3]);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = top == -INFINITY ? 0.f : 1.f / l;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(p[0]) * a.c.tokens + t) * a.c.ld_out + head * DH;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {

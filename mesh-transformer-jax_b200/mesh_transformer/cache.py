@@ -70,11 +70,15 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
     None when the cache holds them already.  ``lengths`` counts the slots in use with the new tokens; ``new`` int32 [batch] says
     how many of the ``tokens`` rows of each sequence are new ones (default: all).  Token t of sequence b sits in slot
     ``p = lengths[b] - new[b] + t`` and sees slot j when ``j <= p and (j < sinks or p - j < window)`` (``window`` None: all).
+    Slots that no new token sees are not looked at: they may hold anything, and pages of nothing else need not exist.
     Scores are multiplied by ``scale`` (default ``d_head ** -0.5``).  Returns ``out`` like ``q``; rows from ``new[b]`` on are zeros.
 
     ``weights`` float32 [batch, kv_heads, pages * 64]: the attention weight that each slot receives, summed over the tokens and
     over the query heads that read its head, is added to it, slots of new tokens beginning at zero.  With ``weights_out`` the
     sums go there and ``weights`` (may be None: zeros) stays as it is.
+
+    ``out`` [batch, tokens, heads, d_head], if given, is written instead of a new tensor.  It shares no memory with the others,
+    nor do ``weights`` and ``weights_out`` unless they are the same.
 
     ``status`` int32 [1], if given, collects what the GPU found wrong: bit 1 a length or a page number outside the cache (that
     sequence counts as empty, that page as unseen), bit 0 a wait that ran out."""

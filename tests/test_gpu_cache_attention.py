@@ -334,3 +334,47 @@ def test_many_long_sequences(cuda_device, heads, kv_heads, d_head, tokens, dtype
         assert ((out[b].double() - want).abs() <= rounding(dtype) * want.abs() + 2.0 ** -13 * spread).all(), b
         received = share.sum((1, 2))
         assert ((w[b, :, :n].double() - received).abs() <= 2.0 ** -13 * received).all(), b
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,d_head,heads,weights", [(1, 64, 4, True), (1, 128, 2, False), (6, 256, 4, True), (150, 64, 2, False), (150, 128, 2, False),
+                                                         (300, 128, 4, False), (150, 256, 2, False), (40, 256, 4, False)])
+def test_slots_that_no_token_sees_may_hold_anything(cuda_device, tokens, d_head, heads, weights, dtype):
+    """Between the first tokens and the window: NaN and infinities in pages that are seen in part, no page at all elsewhere."""
+    from mesh_transformer.cache import cache_attention
+    for length, window, sinks in ((tokens + 900, 200, 4), (tokens + 900, 129, 70), (tokens + 400, 320, 64), (tokens + 130, 100, 1)):
+        pages = (length + PAGE - 1) // PAGE
+        c = Cache(47, 1, pages, 2, d_head, [length])
+        q = c.rows(1, tokens, heads, d_head, dtype, 1.5)
+        outs, _, spread = _reference(c, q, [length], [tokens], window, sinks, d_head ** -0.5)
+        low = length - tokens - window + 1
+        for j in range(sinks, low):
+            c.kpool[int(c.table[0, j // PAGE]), :, j % PAGE] = (float("nan"), float("inf"), float("-inf"))[j % 3]
+            c.vpool[int(c.table[0, j // PAGE]), :, j % PAGE] = (float("inf"), float("nan"), float("-inf"))[j % 3]
+        hidden = [i for i in range(pages) if i * PAGE >= sinks and (i + 1) * PAGE <= low]
+        c.page_table[0, hidden] = -1
+        status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+        w = torch.zeros((1, 2, pages * PAGE), device="cuda") if weights else None
+        out = cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=window, sinks=sinks, weights_out=w, status=status)
+        assert int(status) == 0
+        _check(out, outs, spread, dtype, 2.0 ** -8)
+        if weights:
+            assert torch.isfinite(w).all() and float(w[:, :, sinks:low].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("tokens,d_head", [(1, 128), (4, 64), (200, 64), (200, 128), (200, 256)])
+def test_a_key_that_is_not_a_number(cuda_device, tokens, d_head):
+    """Rows that see it are NaN throughout, the others as without it, wherever in a block the key lies."""
+    from mesh_transformer.cache import cache_attention
+    length = tokens + 300
+    for place in list(range(120, 136)) + [length - tokens // 2 - 1]:
+        c = Cache(53, 1, 9, 2, d_head, [length])
+        q = c.rows(1, tokens, 4, d_head, torch.bfloat16)
+        call = lambda: cache_attention(q, None, None, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=250, sinks=4)
+        want = call()
+        c.kpool[int(c.table[0, place // PAGE]), 1, place % PAGE] = float("nan")
+        got = call()
+        p = torch.arange(length - tokens, length, device="cuda")
+        sees = (place <= p) & (p - place < 250)
+        assert got[0, sees][:, 2:].isnan().all()
+        assert torch.equal(got[0, :, :2], want[0, :, :2]) and torch.equal(got[0, ~sees], want[0, ~sees])
