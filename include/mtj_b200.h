@@ -546,8 +546,9 @@ int32_t mtj_k_cache_evict(const mtj_cache_evict_args* a, mtj_stream s);
  *     accept[k] * q_k(x_k) < p_k(x_k);
  * at the first k that is not, the next token comes from max(p_k - q_k, 0), behind all n from p_n, as arg max of
  *     r_i / -log(noise_i)          (the lowest index among equals; r = p where the difference is zero everywhere),
- * so that the tokens are distributed as samples of the target.  temp below 2^-60 (or NaN): p_k is 1 at the first largest entry of its row, a draft
- * is taken when it is that entry, and accept, noise and the draft's logits are not used.
+ * so that the tokens are distributed as samples of the target.  temp, finite, below 2^-60 (or
+ * NaN): p_k is 1 at the first largest entry of its row, a draft is taken when it is that entry, and accept, noise and the
+ * draft's logits are not used.
  * target [batch][drafts + 1][vocab], draft [batch][drafts][vocab], type `dtype`, with ld_* elements from row to row and
  * batch_* from sequence to sequence; -inf and the lowest value are shares of zero.  draft_tokens [batch][drafts] (outside
  * [0, vocab): never taken); accept [batch][drafts], noise [batch][vocab] uniforms in [tiny, 1); counts [batch] drafted

@@ -5,6 +5,8 @@
 
 namespace mtj {
 
+constexpr int kMostPages = 1 << 24;         // of a sequence: places of slots, and a few steps behind the last, are 32-bit numbers
+
 // Slots in use and new tokens of one sequence; numbers that do not fit the cache make it an empty one.
 struct CacheSeq {
   int length, fresh;

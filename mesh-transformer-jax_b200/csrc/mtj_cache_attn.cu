@@ -26,7 +26,8 @@ int32_t check_args(const mtj_cache_attn_args* a, std::string* err) {
   }
   if (a->n_pages <= 0 || a->batch <= 0 || a->pages <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->tokens <= 0)
     return bad("n_pages, batch, pages, heads, kv_heads and tokens must be positive");
-  if (a->pages > 0x7fffffff / kPageTokens || a->tokens > a->pages * kPageTokens) return bad("more tokens than the pages of a sequence hold");
+  if (a->pages > kMostPages) return bad("more than 2^30 slots a sequence");
+  if (a->tokens > a->pages * kPageTokens) return bad("more tokens than the pages of a sequence hold");
   if (a->heads % a->kv_heads || a->heads / a->kv_heads > MTJ_CACHE_MAX_GROUP)
     return bad("heads must be a multiple of kv_heads, at most MTJ_CACHE_MAX_GROUP times as many");
   if (a->window < 1 || a->sinks < 0) return bad("window must be positive and sinks not negative");

@@ -247,7 +247,7 @@ int32_t check_args(const mtj_cache_evict_args* a, std::string* err) {
   if ((reinterpret_cast<uintptr_t>(a->kpool_dev) | reinterpret_cast<uintptr_t>(a->vpool_dev)) & 15)
     return bad("pools must be 16-byte aligned");
   const int64_t most = 0x7fffffff;
-  if (a->pages > most / kPageTokens || static_cast<int64_t>(a->batch) * a->kv_heads > most / kPageTokens / a->pages ||
+  if (a->pages > kMostPages || static_cast<int64_t>(a->batch) * a->kv_heads > most / kPageTokens / a->pages ||
       a->keep > most - kPageTokens || static_cast<int64_t>(a->batch) * a->kv_heads > most / ((a->keep + kPageTokens - 1) / kPageTokens))
     return bad("batch * kv_heads * slots is too large");
   return MTJ_OK;

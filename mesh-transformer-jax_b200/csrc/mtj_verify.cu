@@ -531,12 +531,13 @@ int32_t check_args(const mtj_verify_args* a, std::string* err) {
     *err = "dtype must be MTJ_F32 or MTJ_BF16";
     return MTJ_ERR_UNSUPPORTED;
   }
+  if (!a->temp_dev && a->temp == INFINITY) return bad("temp must be finite");
   const uintptr_t size = a->dtype == MTJ_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(a->target_dev) | reinterpret_cast<uintptr_t>(a->draft_dev)) & (size - 1))
     return bad("logits must be aligned to their type");
   if (a->ld_target < a->vocab || (a->draft_dev && a->ld_draft < a->vocab)) return bad("a row's stride is shorter than the vocabulary");
   if (a->batch_target < 0 || a->batch_draft < 0) return bad("strides must not be negative");
-  if (a->vocab > 0x7fffffff - 2 * kChunk) return bad("the vocabulary is too large");
+  if (a->vocab > 1 << 30) return bad("the vocabulary is too large");
   if (static_cast<int64_t>(a->batch) * rows_of(*a) > 0x7fffffff / chunks_of(*a)) return bad("batch * drafts * vocab is too large");
   return MTJ_OK;
 }

@@ -153,10 +153,13 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
     out = torch.empty(batch, rows, dtype=torch.int32, device=dev)
     taken = torch.empty(batch, dtype=torch.int32, device=dev)
     logprobs = torch.empty(batch, rows, dtype=torch.float32, device=dev)
-    a = _VERIFY_ARGS(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else 0, tokens.data_ptr(),
-                     accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else 0,
-                     temps.data_ptr() if temps is not None else 0, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
-                     ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
+    try:
+        a = _VERIFY_ARGS(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else 0, tokens.data_ptr(),
+                         accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else 0,
+                         temps.data_ptr() if temps is not None else 0, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
+                         ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
+    except (struct.error, OverflowError, TypeError) as e:
+        raise ValueError(f"temp must be a number or a tensor: {e}") from None
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev.index):
             _run_verify(a, dev)

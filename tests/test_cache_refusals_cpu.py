@@ -132,3 +132,13 @@ def test_packed_arguments_are_laid_out_as_the_structures(L):
         assert [getattr(back, n) for n, _ in cls._fields_] == values
     src = open(__import__("mesh_transformer.cache", fromlist=["x"]).__file__).read() + open(__import__("mesh_transformer.sampling", fromlist=["x"]).__file__).read()
     assert all(f'"{fmt}"' in src for fmt in ("@12P4q10if4x", "@11P8i", "@10P4q4if4x"))
+
+
+def test_numbers_beyond_the_kernels_own(L):
+    """Slots of a sequence, entries of a row and temperatures up to which places and scaled logits stay in 32 bits."""
+    err = lambda: L.lib.mtj_last_error().decode()
+    assert L.lib.mtj_k_cache_attn(ctypes.byref(_attn(L, pages=2 ** 24 + 1, batch=1, kv_heads=1)), BASE, 1 << 40, None) == 1 and "2^30 slots" in err()
+    assert L.lib.mtj_k_cache_evict(ctypes.byref(_evict(L, pages=2 ** 24 + 1, batch=1, kv_heads=1)), None) == 1 and "slots" in err()
+    long = dict(vocab=2 ** 30 + 1, ld_target=2 ** 31, ld_draft=2 ** 31, batch=1, drafts=0)
+    assert L.lib.mtj_verify_drafts(ctypes.byref(_verify(L, **long)), BASE, 1 << 40, None) == 1 and "vocabulary" in err()
+    assert L.lib.mtj_verify_drafts(ctypes.byref(_verify(L, temp=float("inf"))), BASE, 1 << 40, None) == 1 and "temp" in err()

@@ -378,3 +378,73 @@ def test_a_key_that_is_not_a_number(cuda_device, tokens, d_head):
         sees = (place <= p) & (p - place < 250)
         assert got[0, sees][:, 2:].isnan().all()
         assert torch.equal(got[0, :, :2], want[0, :, :2]) and torch.equal(got[0, ~sees], want[0, ~sees])
+
+
+def _dense(q, keys, values, p, j, window, sinks):
+    """64-bit attention [batch, tokens, heads, d] over slots of their own; ``p`` [batch, tokens] slots of the tokens, -1: none."""
+    batch, tokens, heads, d = q.shape
+    kv_heads, group = keys.shape[1], heads // keys.shape[1]
+    hidden = (j > p[..., None]) | ((j >= sinks) & (p[..., None] - j >= window))
+    s = torch.einsum("btghd,bgjd->bghtj", q.double().unflatten(2, (kv_heads, group)), keys.double()) * d ** -0.5
+    share = torch.nan_to_num(torch.softmax(s.masked_fill(hidden[:, None, None], float("-inf")), -1))
+    out = lambda v: torch.einsum("bghtj,bgjd->btghd", share, v).flatten(2, 3)
+    return out(values.double()), out(values.double().abs()), share.sum((2, 3))
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv_heads,weights", [(300, 1, 4, 2, True), (300, 5, 2, 2, False), (513, 2, 2, 1, True),
+                                                                 (8300, 65, 2, 2, False), (1100, 129, 1, 1, False)])
+def test_more_sequences_than_a_launch_plans(cuda_device, batch, tokens, heads, kv_heads, weights):
+    from mesh_transformer.cache import cache_attention
+    d_head, pages, window, sinks = 64, 3, 70, 3
+    g = torch.Generator("cuda").manual_seed(59)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
+    kpool, vpool = rand(batch * pages, kv_heads, PAGE, d_head), rand(batch * pages, kv_heads, PAGE, d_head)
+    table = torch.randperm(batch * pages, generator=g, device="cuda").to(torch.int32).reshape(batch, pages)
+    new = torch.randint(0, tokens + 1, (batch,), generator=g, device="cuda").to(torch.int32)
+    lengths = (new + torch.randint(0, pages * PAGE - tokens + 1, (batch,), generator=g, device="cuda")).to(torch.int32)
+    q = rand(batch, tokens, heads, d_head)
+    w = torch.zeros((batch, kv_heads, pages * PAGE), device="cuda") if weights else None
+    out = cache_attention(q, None, None, kpool, vpool, table, lengths, new=new, window=window, sinks=sinks, weights_out=w)
+    for b in range(0, batch, 512):
+        part = slice(b, b + 512)
+        keys, values = (x[table[part].long()].transpose(1, 2).flatten(2, 3) for x in (kpool, vpool))
+        t = torch.arange(tokens, device="cuda")
+        p = torch.where(t < new[part, None], lengths[part, None] - new[part, None] + t, -1)
+        want, spread, received = _dense(q[part], keys, values, p, torch.arange(pages * PAGE, device="cuda"), window, sinks)
+        assert ((out[part].double() - want).abs() <= rounding(torch.bfloat16) * want.abs() + 2.0 ** -8 * spread).all(), b
+        if weights:
+            assert ((w[part].double() - received).abs() <= 2.0 ** -13 * received).all(), b
+
+
+@pytest.mark.parametrize("tokens", [1, 130])
+def test_a_pool_of_more_than_32_bits(cuda_device, tokens):
+    """Pages behind the pool's first 2^32 bytes and 2^31 elements: attention, storing and eviction."""
+    from mesh_transformer.cache import cache_attention, cache_evict
+    d_head, kv_heads, heads, pages = 256, 4, 4, 5
+    n_pages = 2 ** 31 // (kv_heads * PAGE * d_head) + 40
+    if torch.cuda.mem_get_info()[0] < 5 * n_pages * kv_heads * PAGE * d_head:
+        pytest.skip("not enough memory")
+    g = torch.Generator("cuda").manual_seed(61)
+    kpool = torch.empty((n_pages, kv_heads, PAGE, d_head), dtype=torch.bfloat16, device="cuda")
+    vpool = torch.empty_like(kpool)
+    for pool in (kpool, vpool):
+        pool[-40:].normal_(generator=g)
+    table = (n_pages - 40 + torch.randperm(40, generator=g, device="cuda")[:2 * pages]).to(torch.int32).reshape(2, pages)
+    lengths = torch.tensor([300, 257], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn((2, tokens, heads, d_head), generator=g, device="cuda").to(torch.bfloat16) for _ in range(3))
+    out = cache_attention(q, k, v, kpool, vpool, table, lengths, window=200, sinks=4)
+    keys, values = (x[table.long()].transpose(1, 2).flatten(2, 3) for x in (kpool, vpool))
+    p = lengths[:, None] - tokens + torch.arange(tokens, device="cuda")
+    for b in range(2):
+        assert torch.equal(keys[b, :, p[b].long()].transpose(0, 1), k[b]) and torch.equal(values[b, :, p[b].long()].transpose(0, 1), v[b])
+    want, spread, _ = _dense(q, keys, values, p, torch.arange(pages * PAGE, device="cuda"), 200, 4)
+    assert ((out.double() - want).abs() <= rounding(torch.bfloat16) * want.abs() + 2.0 ** -8 * spread).all()
+    used = set(table.flatten().tolist())
+    spare = torch.tensor([x for x in range(n_pages - 40, n_pages) if x not in used][:2], dtype=torch.int32, device="cuda").reshape(2, 1)
+    weights = torch.rand((2, kv_heads, pages * PAGE), generator=g, device="cuda")
+    kept, _, _, cut = cache_evict(kpool, vpool, table, lengths, weights, spare, 64, first=4, last=16)
+    assert torch.equal(cut[:, :1], spare)
+    for b in range(2):
+        for h in range(kv_heads):
+            for pool, rows in ((kpool, keys), (vpool, values)):
+                assert torch.equal(pool[int(spare[b, 0]), h], rows[b, h, kept[b, h].long()])

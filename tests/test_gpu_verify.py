@@ -157,3 +157,97 @@ def test_captured(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         _check(got, target, draft, tokens, accept, noise, [3] * 2, [1.0] * 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("batch,drafts,vocab,temp", [
+    (1, 2, 200003, 1.0),              # a block goes over its part of a row in several steps, a lane over a row's chunks
+    (1, 3, 140001, 0.0),
+    (160, 1, 2500, 0.7),              # two blocks a sequence, and one
+    (400, 2, 300, 1.1),
+])
+def test_long_rows_and_many_sequences(cuda_device, batch, drafts, vocab, temp, known, dtype):
+    from mesh_transformer.sampling import verify_drafts
+    target, draft, tokens, accept, noise = _inputs(31 + batch, batch, drafts, vocab, dtype, apart=0.3, agree=0.5)
+    if temp == 0.0:
+        tokens = target[:, :drafts].float().argmax(-1).to(torch.int32)
+    d = draft if known else None
+    got = verify_drafts(target, d, tokens, accept, noise, temp=temp)
+    _check(got, target, d, tokens, accept, noise, [drafts] * batch, [temp] * batch)
+
+
+def test_more_sequences_than_a_launch_takes(cuda_device):
+    """The parts of the batch that are launched one after another give what each gives alone."""
+    from mesh_transformer.sampling import verify_drafts
+    target, draft, tokens, accept, noise = _inputs(37, 4500, 2, 70, torch.float32, agree=0.5)
+    count = torch.randint(0, 3, (4500,), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(torch.int32)
+    temp = torch.rand((4500,), device="cuda", generator=torch.Generator("cuda").manual_seed(2)) + 0.5
+    got = verify_drafts(target, draft, tokens, accept, noise, count=count, temp=temp)
+    for part in (slice(0, 1000), slice(3600, 4500)):
+        alone = verify_drafts(target[part], draft[part], tokens[part], accept[part], noise[part], count=count[part], temp=temp[part])
+        assert all(torch.equal(x[part], y) for x, y in zip(got, alone))
+    tail = slice(4400, 4500)
+    _check(tuple(x[tail] for x in got), target[tail], draft[tail], tokens[tail], accept[tail], noise[tail], count[tail].tolist(), temp[tail].tolist())
+
+
+def test_drafts_over_a_cache(cuda_device):
+    """Drafted tokens through an attention layer over a paged cache, checked, the refused ones taken back by the length alone; the
+    cache is cut when it is full.  Every step's attention against 64 bits over the tokens that were kept so far, every check against
+    the plain form on the step's logits."""
+    from cache_util import PAGE, host, rounding
+    from mesh_transformer.cache import cache_attention, cache_evict
+    from mesh_transformer.sampling import verify_drafts
+    g = torch.Generator("cuda").manual_seed(41)
+    vocab, heads, kv_heads, d_head, pages, drafts, keep = 500, 4, 2, 64, 3, 3, 64
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)
+    embed_q, embed_k, embed_v, head = (rand(vocab, heads, d_head), rand(vocab, kv_heads, d_head), rand(vocab, kv_heads, d_head),
+                                       rand(heads * d_head, vocab).float() * 0.3)
+    kpool, vpool = (torch.full((pages + 2, kv_heads, PAGE, d_head), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = torch.tensor([[4, 1, 3]], dtype=torch.int32, device="cuda")
+    free = [0, 2]
+    weights = torch.zeros((1, kv_heads, pages * PAGE), device="cuda")
+    lengths = torch.zeros((1,), dtype=torch.int32, device="cuda")
+    held = [np.zeros((0, 2, d_head)) for _ in range(kv_heads)]
+    last, cuts, accepted = 7, 0, 0
+    for step in range(200):
+        guess = torch.randint(0, vocab, (1, drafts), generator=g, device="cuda").to(torch.int32)
+        if step % 3 < 2:                                  # what the layer itself would say: the row is stored again by the step
+            t = torch.tensor([[last]], device="cuda")
+            y = cache_attention(embed_q[t], embed_k[t], embed_v[t], kpool, vpool, table, lengths + 1)
+            guess[0, 0] = (y.float().flatten(2) @ head)[0, 0].argmax()
+        tokens = torch.cat([torch.tensor([[last]], dtype=torch.int32, device="cuda"), guess], 1).long()
+        n = int(lengths)
+        lengths = lengths + (drafts + 1)
+        out = cache_attention(embed_q[tokens], embed_k[tokens], embed_v[tokens], kpool, vpool, table, lengths, weights=weights)
+        for h in range(kv_heads):
+            rows = np.concatenate([held[h], np.stack([host(embed_k[tokens[0], h]), host(embed_v[tokens[0], h])], 1)])
+            mine = slice(h * heads // kv_heads, (h + 1) * heads // kv_heads)
+            qh = host(embed_q[tokens[0]])[:, mine]
+            want, _ = cache_oracle.attention(qh, rows[:, :1], rows[:, 1:], len(rows), drafts + 1, 10 ** 6, 0, d_head ** -0.5)
+            room, _ = cache_oracle.attention(qh, rows[:, :1], np.abs(rows[:, 1:]), len(rows), drafts + 1, 10 ** 6, 0, d_head ** -0.5)
+            # a bf16 number has 8 significant bits: its step is 2^-7 of a power of two, half of it at most 2^-8 of the value
+            assert (np.abs(host(out[0])[:, mine] - want) <= rounding(torch.bfloat16) * np.abs(want) + 2.0 ** -13 * room).all(), step
+            held[h] = rows
+        logits = out.float().flatten(2) @ head
+        accept = torch.rand((1, drafts), generator=g, device="cuda").clamp_(min=TINY)
+        noise = torch.rand((1, vocab), generator=g, device="cuda").clamp_(min=TINY)
+        got = verify_drafts(logits, None, guess, accept, noise, temp=0.0 if step % 2 else 0.5)
+        _check(got, logits, None, guess, accept, noise, [drafts], [0.0 if step % 2 else 0.5])
+        taken = int(got[1])
+        accepted += taken
+        last = int(got[0][0, taken])
+        lengths = lengths - (drafts - taken)
+        held = [x[:n + 1 + taken] for x in held]
+        if int(lengths) + drafts + 1 > pages * PAGE:
+            spare = torch.tensor([[free[0]]], dtype=torch.int32, device="cuda")
+            old = table[0].tolist()
+            kept, lengths, weights, table = cache_evict(kpool, vpool, table, lengths, weights, spare, keep, first=2, last=20)
+            assert int(lengths) == keep
+            free = free[1:] + old
+            table[0, 1:] = torch.tensor(free[:pages - 1], dtype=torch.int32, device="cuda")
+            free = free[pages - 1:]
+            kept = kept[0].cpu().numpy()
+            held = [x[kept[h]] for h, x in enumerate(held)]
+            cuts += 1
+    assert int(lengths) == len(held[0]) and accepted >= 20 and cuts >= 1
