@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars + kPeerBars; ++i) mbar_init(bar0 + 8u * i, 1);
     for (int i = 0; i < 2; ++i) {
-      constexpr int kArrivals = kPair ? 2 * kSoftThreads / 32 : kSoftThreads / kTiles;      // a pair: both blocks' warps
+      constexpr int kArrivals = (kPair ? 2 : 1) * kSoftThreads / 32 / kTiles;      // a warp each, of a pair both blocks'
       mbar_init(p_full + 8u * i, kArrivals);
       mbar_init(p_half + 8u * i, kArrivals);
       mbar_init(o_free + 8u * i, kArrivals);
@@ -825,11 +825,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       do {
         // the same in all lanes, and known to be: what hangs on it stays in uniform registers
         const int blocks = __reduce_max_sync(0xffffffffu, w.n), units = blocks * kTiles;
+        auto keys_there = [&](int u) {
+          const int j = k0 + u / kTiles, st = j % C::kKSlots;
+          const uint32_t parity = (j / C::kKSlots) & 1;
+          return (u % kTiles != 0 || wait(k_full + 8 * st, parity)) && (!kPair || wait(k_peer + 8 * st, parity));
+        };
         auto issue_s = [&](int u) {
           const int j = k0 + u / kTiles, t = u % kTiles, st = j % C::kKSlots, buf = (u0 + u) & 1;
-          const uint32_t parity = (j / C::kKSlots) & 1;
-          if (t == 0 && !wait(k_full + 8 * st, parity)) return false;
-          if (kPair && !wait(k_peer + 8 * st, parity)) return false;
           fence_after();
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c) {
@@ -844,21 +846,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           commit(s_full + 8 * buf);
           if (t == kTiles - 1) commit(k_empty + 8 * st);
           if (u == units - 1) commit(q_empty);
-          return true;
         };
         auto issue_pv = [&](int u) {
           const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1, n = k0 + j, st = n % C::kVSlots;
           const uint32_t parity = ((u0 + u) >> 1) & 1, landed = (n / C::kVSlots) & 1;
           // the accumulator's last job has been read
           if (seg > 0 && u < kTiles && !wait(o_free + 8 * t, (seg - 1) & 1)) return false;
-          if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
+          // a wait costs 60 ns even where there is nothing to wait for: those that are likely over come before those for the weights,
+          // the next unit's keys among them
           if (t == 0 && !wait(v_full + 8 * st, landed)) return false;
           if (kPair && !wait(v_peer + 8 * st, landed)) return false;
+          const bool more = u + 2 < units;
+          if (C::kHalves == 1 && more && !keys_there(u + 2)) return false;
+          if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
           const uint64_t vd = smem_desc(sV + st * C::kVBytes, kKeysB * 128, 1024);
           const uint32_t pa = tmem + C::kColS + buf * kKeysB;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {                    // by the page: the second half of the weights comes later
-            if (C::kHalves == 2 && h == 1 && !wait(p_full + 8 * buf, parity)) return false;
+            if (C::kHalves == 2 && h == 1) {
+              if (more && !keys_there(u + 2)) return false;
+              if (!wait(p_full + 8 * buf, parity)) return false;
+            }
             fence_after();
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; ++k) {
@@ -868,14 +876,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           }
           if (t == kTiles - 1) commit(v_empty + 8 * st);
           commit(o_done + 8 * buf);
+          if (more) issue_s(u + 2);
           return true;
         };
-        ok = wait(q_full, seg & 1) && (!kPair || wait(q_peer, seg & 1)) && issue_s(0);
-        if (ok && units > 1) ok = issue_s(1);
-        for (int u = 0; ok && u < units; ++u) {
-          ok = issue_pv(u);
-          if (ok && u + 2 < units) ok = issue_s(u + 2);
+        ok = wait(q_full, seg & 1) && (!kPair || wait(q_peer, seg & 1));
+        for (int u = 0; ok && u < min(units, 2); ++u) {
+          ok = keys_there(u);
+          if (ok) issue_s(u);
         }
+        for (int u = 0; ok && u < units; ++u) ok = issue_pv(u);
         k0 += blocks;
         u0 += units;
         ++seg;
@@ -896,11 +905,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     const int job_tile = kPair ? rank : tile;
     auto announce = [&](uint32_t bar) {
       fence_before();
-      if constexpr (kPair) {
-        __syncwarp();
-        if (lane == 0) arrive_first(bar);
-      } else {
-        arrive_at(bar);
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair) arrive_first(bar);
+        else arrive_at(bar);
       }
     };
     const int r = quad * 32 + lane;                        // row of the tile = lane of tensor memory
@@ -916,9 +924,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
       float m_ref = -INFINITY, l = 0.f;
       for (int j = 0; j < w.n; ++j, ++block) {
         const int u = kTiles == 2 ? 2 * block + wg : block;
+        const int slot0 = w.k.slot_of(w.k.place(w.j + j)), key = slot0 + part * kKeysThread;      // slots of the block's and this thread's first key
+        const int warp_last = min(warp_first + 31, p_last);
+        const bool inside = key + kKeysThread - 1 <= warp_first && warp_last >= warp_first &&
+                            (key + kKeysThread - 1 < a.c.sinks || warp_last - key < a.c.window);
+        const bool unseen = slot0 < w.k.low && slot0 + kKeysB > w.k.sinks;         // some of them, by all tokens
         if (ok) ok = mbar_wait(s_full + 8 * (u & 1), (u >> 1) & 1);
         fence_after();
-        const int key = w.k.slot_of(w.k.place(w.j + j)) + part * kKeysThread;      // slot of this thread's first key
         const int note = notes[block % kBlockNotes];
         const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
         uint32_t x[kKeysThread];
@@ -929,8 +941,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
         constexpr int kFullNote = kPageTokens | kPageTokens << 8;
         // V's rows that hold nothing, or nothing that a token of the job sees: zeroed before anybody's weights are announced
-        const int slot0 = key - part * kKeysThread;
-        if (note != kFullNote || (slot0 < w.k.low && slot0 + kKeysB > w.k.sinks)) {
+        if (note != kFullNote || unseen) {
           const int st = block % C::kVSlots;
           if (ok) ok = mbar_wait(v_full + 8 * st, (block / C::kVSlots) & 1);
           if (tile == 0) {
@@ -945,10 +956,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        const int warp_last = min(warp_first + 31, p_last);
-        const bool all_seen = note == kFullNote && key + kKeysThread - 1 <= warp_first &&
-                              (key + kKeysThread - 1 < a.c.sinks || warp_last - key < a.c.window) && warp_last >= warp_first;
-        if (!all_seen) {
+        if (note != kFullNote || !inside) {
           // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
           const int hi = p - key, lo = p - a.c.window + 1 - key, sk = a.c.sinks - key;
 #pragma unroll
@@ -977,8 +985,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         // first keys are poor ones (a few first tokens, the edge of its window) does not have O rescaled for its next ones
         float m_new = m_ref;
         if (!(top <= m_ref + 8.0f)) m_new = top + 8.0f;     // a score that is NaN makes the row NaN: the reference, and with it the sum
-        const float corr = (m_new == m_ref || m_ref == -INFINITY) ? 1.0f : exp2_ftz(m_ref - m_new);
-        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+        if (__any_sync(0xffffffffu, m_new != m_ref && m_ref != -INFINITY)) {
+          const float corr = m_new == m_ref || m_ref == -INFINITY ? 1.0f : exp2_ftz(m_ref - m_new);
+          l *= corr;
           // O changes scale: the tile's products so far must have landed
           const int before = u - kTiles;
           if (ok) ok = mbar_wait(o_done + 8 * (before & 1), (before >> 1) & 1);
@@ -1022,7 +1031,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         }
         float sum0, sum1;
         unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
-        l = fmaf(l, corr, sum0 + sum1);
+        l += sum0 + sum1;
         m_ref = m_new;
       }
       // the job's result, or the piece's part of it
