@@ -448,3 +448,19 @@ def test_a_pool_of_more_than_32_bits(cuda_device, tokens):
         for h in range(kv_heads):
             for pool, rows in ((kpool, keys), (vpool, values)):
                 assert torch.equal(pool[int(spare[b, 0]), h], rows[b, h, kept[b, h].long()])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,d_head,tokens", [(10, 2, 64, 4), (24, 4, 128, 3), (40, 8, 64, 5), (8, 1, 128, 5), (12, 2, 64, 9), (5, 1, 256, 4)])
+def test_rows_that_fill_three_eighths_and_five(cuda_device, heads, kv_heads, d_head, tokens, dtype):
+    """17 to 24 rows a key head, and 25 to 54 in tiles of which the last has rows left over; weights and ragged lengths with them."""
+    lengths, fresh = [700, tokens, 65, 1300], [tokens, tokens, tokens - 1, tokens]
+    _, out, outs, received, spread, (w_in, w_out) = _run(67, 4, heads, kv_heads, d_head, tokens, lengths, fresh, 500, 9, dtype, weights=True)
+    _check(out, outs, spread, dtype, 2.0 ** -16)
+    _, out, outs, _, spread, _ = _run(67, 4, heads, kv_heads, d_head, tokens, lengths, fresh, 500, 9, dtype)
+    _check(out, outs, spread, dtype, 2.0 ** -16)
+    w_in, w_out = w_in.double().cpu().numpy(), w_out.double().cpu().numpy()
+    for b, (n, f) in enumerate(zip(lengths, fresh)):
+        before = w_in[b, :, :n].copy()
+        before[:, n - f:] = 0
+        assert (np.abs(w_out[b, :, :n] - before - received[b]) <= 2.0 ** -13 * received[b] + 2.0 ** -22 * (before + received[b])).all()
