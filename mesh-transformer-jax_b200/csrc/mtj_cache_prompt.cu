@@ -11,8 +11,13 @@
 //     P = 2^(S c - m)            a thread a row (d_head 256: two threads a row, 64 keys each), written over S as bf16
 //     O[128, d] += P V           P from tensor memory, V as MN-major operand straight from the pages
 // and units go round two score buffers: one thread issues S0 S1 | PV0 S2 | PV1 S3 | ..., so that while one warp group works out the
-// weights of a unit, the tensor cores have the other unit's products.  The bound for d_head 128 is shared by the tensor cores (1024
-// cycles a unit) and the exponentials (16 a cycle: 1024).
+// weights of a unit, the tensor cores have the other unit's products.  For d_head 128 a unit is 1024 cycles of products and, at 16
+// exponentials a cycle less the quarter that the multiply-add units take, 768 of exponentials; the chain of a tile (scores, maximum,
+// weights, products, next scores) is what is left in the open.  32 heads of 128, 8 key heads, 8191 tokens, window 4096: 0.39 ms, 1060
+// TFLOP/s of visible pairs, 0.45 ms (925) in a row of calls, where the SMs run at 1.6 GHz; tensor pipe 54 % active.  16 heads of 256, 2047
+// tokens, window 1024: 49 us, 41 %.  Built and measured at the first of these, none ahead by more than 2 %: score buffers of 64 keys, two a tile, so that
+// no tile waits for its scores (386 us from a warp of products a tile, 528 from one for both); two threads a row for 128-wide heads (407);
+// pairs of blocks for them (414); a warp of products a tile with buffers of 128 (460: the tiles' products get in each other's way).
 //
 // A job is a sequence, a head (pair) and the tokens of a block.  148 blocks, one an SM, take whole jobs, longest first, in turns that
 // go forth and back; where that would leave SMs idle for longer than a join takes, the line of all jobs' key blocks is cut into equal
@@ -25,8 +30,9 @@
 // tokens: storing in a kernel before took 16 us, row by row beside the products it was longer than they were.)
 //
 // Scores, maxima, sums and O are 32-bit; P is rounded to bf16, half a step on average as large as the rounding of the output (a second
-// term would be half as many products again).  O is rescaled when a row's scores have outgrown its reference, which waits for the products before.  The rows of V
-// behind the sequence, or of a page that does not exist, are zeroed in shared memory before they meet their zero weights.
+// term would be half as many products again).  O is rescaled when a row's scores have outgrown its reference, which waits for the
+// products before.  The rows of V behind the sequence, of a page that does not exist, or that no token of the job sees, are zeroed in
+// shared memory before they meet their zero weights.
 // Every wait is bounded.
 #include <cuda.h>
 #include <math.h>
@@ -531,7 +537,9 @@ struct Walk {
 };
 
 // Whether the 64 new tokens from t on fill a page of their own and are stored from shared memory.
-__device__ __forceinline__ bool stored_by_page(const JobKeys& k, int t) { return k.first % kPageTokens == 0 && t / kPageTokens * kPageTokens + kPageTokens <= k.fresh; }
+__device__ __forceinline__ bool stored_by_page(const JobKeys& k, int t) {
+  return k.first % kPageTokens == 0 && t / kPageTokens * kPageTokens + kPageTokens <= k.fresh;
+}
 
 // The other new rows into their slots, a warp a row, dealt out to all warps but those of TMA and products: the two that do nothing else
 // begin at once, the softmax warps when they have run out of jobs.
@@ -638,441 +646,445 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     Walk w;
     const bool work = w.begin(a, piece);
-  if (warp == 8) {
-    // ---- TMA ----
-    if (lane == 0 && work) {
-      int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
-      constexpr int kKChunk = C::kKPages * kPageTokens * 128;      // bytes of 64 columns of a slot of keys
-      const int v_chunk0 = kPair ? rank * C::kVChunks : 0;
-      uint32_t storing_k = 0, storing_v = 0;               // slots with rows to store
-      bool ok = true;
-      // a slot's new rows go to their pages when the products have read it, before it is filled again
-      auto store_k = [&](int st) {
-        const int* rows = to_store[st];
-        storing_k &= ~(1u << st);
-#pragma unroll
-        for (int h = 0; h < C::kKPages; ++h)
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
-            if (rows[h] >= 0) tma_store(&map_k, c * 64, rows[h], sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128));
-        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
-      };
-      auto store_v = [&](int st) {
-        const int* rows = to_store[C::kKSlots + st];
-        storing_v &= ~(1u << st);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < C::kVChunks; ++c)
-            if (rows[h] >= 0)
-              tma_store(&map_v, (v_chunk0 + c) * 64, rows[h], sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128));
-        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
-      };
-      do {
-        const int head0 = w.head_job * (a.by_heads ? 2 : 1), kvh = head0 / group;
-        if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1);
-        if (!ok) break;
-        mbar_expect_tx(q_full, C::kQBytes);
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
-            tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t + rank : 0)) * DH + c * 64,
-                    w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : (t + rank) * kRowsT), q_full);
-        const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
-        // a key block's pages, or its rows of new tokens: the row where each 64 begin, how many hold something, the page they are stored
-        // to; looked up before the slot is waited for, because the products wait for what comes behind that
-        struct Block {
-          int row[2], valid[2], target[2];
-          bool cached;
-        };
-        auto look_up = [&](int j) {
-          Block x;
-          const int place = w.k.place(w.j + j);
-          x.cached = place < w.k.tail;
-          // a key head's new rows are stored by the job that has these tokens and the group's first head
-          const bool mine = !x.cached && place - w.k.tail >= w.k.t_first && place - w.k.tail < w.k.t_end && head0 % group == 0;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            x.target[h] = -1;
-            if (!x.cached) {
-              const int t = place - w.k.tail + h * kPageTokens;
-              x.valid[h] = min(kPageTokens, max(0, w.k.fresh - t));
-              x.row[h] = w.b * a.c.tokens + t;
-              if (mine && x.valid[h] > 0 && stored_by_page(w.k, t)) {
-                const int page = table[(w.k.first + t) / kPageTokens];
-                if (cache_page_ok(page, a.c.n_pages)) x.target[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
-                else if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
-              }
-              continue;
-            }
-            const int at = place / kPageTokens + h;
-            const bool seen = at * kPageTokens < w.k.sinks || (at + 1) * kPageTokens > w.k.low;
-            x.valid[h] = seen ? min(kPageTokens, max(0, w.k.cached - at * kPageTokens)) : 0;
-            int page = x.valid[h] > 0 ? table[at] : 0;
-            if (!cache_page_ok(page, a.c.n_pages)) {
-              // not read: page 0 stands in, nobody sees its scores
-              x.valid[h] = page = 0;
-              if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
-            }
-            x.row[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
-          }
-          return x;
-        };
-        auto load_k = [&](const Block& x) {
-          const int st = kc % C::kKSlots;
-          const CUtensorMap* map = x.cached ? &map_k : &map_k_new;
-          const int col = x.cached ? 0 : kvh * DH;
-          if (kc >= C::kKSlots && !mbar_wait(k_empty + 8 * st, (kc / C::kKSlots - 1) & 1)) return false;
-          if (storing_k >> st & 1u) store_k(st);
-          mbar_expect_tx(k_full + 8 * st, C::kKBytes);
+    if (warp == 8) {
+      // ---- TMA ----
+      if (lane == 0 && work) {
+        int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
+        constexpr int kKChunk = C::kKPages * kPageTokens * 128;      // bytes of 64 columns of a slot of keys
+        const int v_chunk0 = kPair ? rank * C::kVChunks : 0;
+        uint32_t storing_k = 0, storing_v = 0;               // slots with rows to store
+        bool ok = true;
+        // a slot's new rows go to their pages when the products have read it, before it is filled again
+        auto store_k = [&](int st) {
+          const int* rows = to_store[st];
+          storing_k &= ~(1u << st);
 #pragma unroll
           for (int h = 0; h < C::kKPages; ++h)
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c)
-              tma_box(sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128), map, col + c * 64, kPair && rank ? x.row[1] : x.row[h],
-                      k_full + 8 * st);
-          const int t0 = kPair && rank ? x.target[1] : x.target[0], t1 = kPair ? -1 : x.target[1];
-          if (t0 >= 0 || t1 >= 0) {
-            storing_k |= 1u << st;
-            to_store[st][0] = t0;
-            to_store[st][1] = t1;
-          }
-          ++kc;
-          return true;
+              if (rows[h] >= 0) tma_store(&map_k, c * 64, rows[h], sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128));
+          asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
         };
-        auto load_v = [&](const Block& x) {
-          const CUtensorMap* map = x.cached ? &map_v : &map_v_new;
-          const int col = x.cached ? 0 : kvh * DH;
-          const int st = vc % C::kVSlots;
-          if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
-          if (storing_v >> st & 1u) store_v(st);
-          mbar_expect_tx(v_full + 8 * st, C::kVBytes);
+        auto store_v = [&](int st) {
+          const int* rows = to_store[C::kKSlots + st];
+          storing_v &= ~(1u << st);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int c = 0; c < C::kVChunks; ++c)
-              tma_box(sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), map, col + (v_chunk0 + c) * 64, x.row[h], v_full + 8 * st);
-          if (x.target[0] >= 0 || x.target[1] >= 0) {
-            storing_v |= 1u << st;
-            to_store[C::kKSlots + st][0] = x.target[0];
-            to_store[C::kKSlots + st][1] = x.target[1];
-          }
-          ++vc;
-          return true;
-        };
-        // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...; the softmax warps' note of a block is written
-        // before the arrival that its products wait for
-        Block now = look_up(0), then;
-        notes[kc % kBlockNotes] = now.valid[0] | now.valid[1] << 8;
-        ok = load_k(now);
-        for (int j = 0; ok && j < w.n; ++j) {
-          if (j + 1 < w.n) {
-            then = look_up(j + 1);
-            notes[kc % kBlockNotes] = then.valid[0] | then.valid[1] << 8;
-            ok = load_k(then);
-          }
-          if (ok) ok = load_v(now);
-          now = then;
-        }
-        ++seg;
-      } while (ok && w.next(a));
-      // what the last round of slots holds
-      for (int n = max(0, kc - C::kKSlots); ok && n < kc; ++n) {
-        ok = mbar_wait(k_empty + 8 * (n % C::kKSlots), (n / C::kKSlots) & 1);
-        if (ok && (storing_k >> (n % C::kKSlots) & 1u)) store_k(n % C::kKSlots);
-      }
-      for (int n = max(0, vc - C::kVSlots); ok && n < vc; ++n) {
-        ok = mbar_wait(v_empty + 8 * (n % C::kVSlots), (n / C::kVSlots) & 1);
-        if (ok && (storing_v >> (n % C::kVSlots) & 1u)) store_v(n % C::kVSlots);
-      }
-      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      if (!ok) atomicOr(&failed, 1u);
-    }
-  } else if (warp == 9) {
-    // ---- products ----
-    if (kPair && rank != 0) {
-      // the second block of a pair tells the first what has landed, in the order in which the products want it
-      if (lane == 0 && work) {
-        int kc = 0, vc = 0, seg = 0;
-        bool ok = true;
-        auto tell = [&](uint32_t full, uint32_t peer, int n, int slots) {
-          ok = ok && mbar_wait(full + 8 * (n % slots), (n / slots) & 1);
-          if (ok) arrive_first(peer + 8 * (n % slots));
+              if (rows[h] >= 0)
+                tma_store(&map_v, (v_chunk0 + c) * 64, rows[h], sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128));
+          asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
         };
         do {
-          tell(q_full, q_peer, seg++, 1);
-          tell(k_full, k_peer, kc++, C::kKSlots);
+          const int head0 = w.head_job * (a.by_heads ? 2 : 1), kvh = head0 / group;
+          if (seg > 0) ok = mbar_wait(q_empty, (seg - 1) & 1);
+          if (!ok) break;
+          mbar_expect_tx(q_full, C::kQBytes);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)
+              tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t + rank : 0)) * DH + c * 64,
+                      w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : (t + rank) * kRowsT), q_full);
+          const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
+          // a key block's pages, or its rows of new tokens: the row where each 64 begin, how many hold something, the page they are stored
+          // to; looked up before the slot is waited for, because the products wait for what comes behind that
+          struct Block {
+            int row[2], valid[2], target[2];
+            bool cached;
+          };
+          auto look_up = [&](int j) {
+            Block x;
+            const int place = w.k.place(w.j + j);
+            x.cached = place < w.k.tail;
+            // a key head's new rows are stored by the job that has these tokens and the group's first head
+            const bool mine = !x.cached && place - w.k.tail >= w.k.t_first && place - w.k.tail < w.k.t_end && head0 % group == 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              x.target[h] = -1;
+              if (!x.cached) {
+                const int t = place - w.k.tail + h * kPageTokens;
+                x.valid[h] = min(kPageTokens, max(0, w.k.fresh - t));
+                x.row[h] = w.b * a.c.tokens + t;
+                if (mine && x.valid[h] > 0 && stored_by_page(w.k, t)) {
+                  const int page = table[(w.k.first + t) / kPageTokens];
+                  if (cache_page_ok(page, a.c.n_pages)) x.target[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
+                  else if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+                }
+                continue;
+              }
+              const int at = place / kPageTokens + h;
+              const bool seen = at * kPageTokens < w.k.sinks || (at + 1) * kPageTokens > w.k.low;
+              x.valid[h] = seen ? min(kPageTokens, max(0, w.k.cached - at * kPageTokens)) : 0;
+              int page = x.valid[h] > 0 ? table[at] : 0;
+              if (!cache_page_ok(page, a.c.n_pages)) {
+                // not read: page 0 stands in, nobody sees its scores
+                x.valid[h] = page = 0;
+                if (a.c.status_dev) atomicOr(a.c.status_dev, kDevErrBadIndex);
+              }
+              x.row[h] = (page * a.c.kv_heads + kvh) * kPageTokens;
+            }
+            return x;
+          };
+          auto load_k = [&](const Block& x) {
+            const int st = kc % C::kKSlots;
+            const CUtensorMap* map = x.cached ? &map_k : &map_k_new;
+            const int col = x.cached ? 0 : kvh * DH;
+            if (kc >= C::kKSlots && !mbar_wait(k_empty + 8 * st, (kc / C::kKSlots - 1) & 1)) return false;
+            if (storing_k >> st & 1u) store_k(st);
+            mbar_expect_tx(k_full + 8 * st, C::kKBytes);
+#pragma unroll
+            for (int h = 0; h < C::kKPages; ++h)
+#pragma unroll
+              for (int c = 0; c < C::kChunks; ++c)
+                tma_box(sK + st * C::kKBytes + c * kKChunk + h * (kPageTokens * 128), map, col + c * 64, kPair && rank ? x.row[1] : x.row[h],
+                        k_full + 8 * st);
+            const int t0 = kPair && rank ? x.target[1] : x.target[0], t1 = kPair ? -1 : x.target[1];
+            if (t0 >= 0 || t1 >= 0) {
+              storing_k |= 1u << st;
+              to_store[st][0] = t0;
+              to_store[st][1] = t1;
+            }
+            ++kc;
+            return true;
+          };
+          auto load_v = [&](const Block& x) {
+            const CUtensorMap* map = x.cached ? &map_v : &map_v_new;
+            const int col = x.cached ? 0 : kvh * DH;
+            const int st = vc % C::kVSlots;
+            if (vc >= C::kVSlots && !mbar_wait(v_empty + 8 * st, (vc / C::kVSlots - 1) & 1)) return false;
+            if (storing_v >> st & 1u) store_v(st);
+            mbar_expect_tx(v_full + 8 * st, C::kVBytes);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int c = 0; c < C::kVChunks; ++c)
+                tma_box(sV + st * C::kVBytes + c * (kKeysB * 128) + h * (kPageTokens * 128), map, col + (v_chunk0 + c) * 64, x.row[h],
+                        v_full + 8 * st);
+            if (x.target[0] >= 0 || x.target[1] >= 0) {
+              storing_v |= 1u << st;
+              to_store[C::kKSlots + st][0] = x.target[0];
+              to_store[C::kKSlots + st][1] = x.target[1];
+            }
+            ++vc;
+            return true;
+          };
+          // in the order in which the products want them: S0 (S1) | PV0 S2 | PV1 S3 ...; the softmax warps' note of a block is written
+          // before the arrival that its products wait for
+          Block now = look_up(0), then;
+          notes[kc % kBlockNotes] = now.valid[0] | now.valid[1] << 8;
+          ok = load_k(now);
           for (int j = 0; ok && j < w.n; ++j) {
-            if (j + 1 < w.n) tell(k_full, k_peer, kc++, C::kKSlots);
-            tell(v_full, v_peer, vc++, C::kVSlots);
+            if (j + 1 < w.n) {
+              then = look_up(j + 1);
+              notes[kc % kBlockNotes] = then.valid[0] | then.valid[1] << 8;
+              ok = load_k(then);
+            }
+            if (ok) ok = load_v(now);
+            now = then;
           }
+          ++seg;
         } while (ok && w.next(a));
+        // what the last round of slots holds
+        for (int n = max(0, kc - C::kKSlots); ok && n < kc; ++n) {
+          ok = mbar_wait(k_empty + 8 * (n % C::kKSlots), (n / C::kKSlots) & 1);
+          if (ok && (storing_k >> (n % C::kKSlots) & 1u)) store_k(n % C::kKSlots);
+        }
+        for (int n = max(0, vc - C::kVSlots); ok && n < vc; ++n) {
+          ok = mbar_wait(v_empty + 8 * (n % C::kVSlots), (n / C::kVSlots) & 1);
+          if (ok && (storing_v >> (n % C::kVSlots) & 1u)) store_v(n % C::kVSlots);
+        }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (!ok) atomicOr(&failed, 1u);
       }
-    } else if (work) {
-      const uint32_t leader = elected();
-      auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
-      auto commit = [&](uint32_t bar) {
-        if constexpr (kPair) commit_pair(bar, leader);
-        else commit_to(bar, leader);
-      };
-      constexpr uint32_t kM = kPair ? 2 * kRowsT : kRowsT;
-      constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kM >> 4) << 24);
-      constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kM >> 4) << 24);
-      int k0 = 0, u0 = 0, seg = 0;                         // key blocks, units and jobs before the current job
-      bool ok = true;
-      do {
-        // the same in all lanes, and known to be: what hangs on it stays in uniform registers
-        const int blocks = __reduce_max_sync(0xffffffffu, w.n), units = blocks * kTiles;
-        auto keys_there = [&](int u) {
-          const int j = k0 + u / kTiles, st = j % C::kKSlots;
-          const uint32_t parity = (j / C::kKSlots) & 1;
-          return (u % kTiles != 0 || wait(k_full + 8 * st, parity)) && (!kPair || wait(k_peer + 8 * st, parity));
-        };
-        auto issue_s = [&](int u) {
-          const int j = k0 + u / kTiles, t = u % kTiles, st = j % C::kKSlots, buf = (u0 + u) & 1;
-          fence_after();
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c) {
-            const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
-            const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (C::kKPages * kPageTokens * 128), 16, 1024);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if constexpr (kPair) mma_ss_pair(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
-              else mma_ss(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+    } else if (warp == 9) {
+      // ---- products ----
+      if (kPair && rank != 0) {
+        // the second block of a pair tells the first what has landed, in the order in which the products want it
+        if (lane == 0 && work) {
+          int kc = 0, vc = 0, seg = 0;
+          bool ok = true;
+          auto tell = [&](uint32_t full, uint32_t peer, int n, int slots) {
+            ok = ok && mbar_wait(full + 8 * (n % slots), (n / slots) & 1);
+            if (ok) arrive_first(peer + 8 * (n % slots));
+          };
+          do {
+            tell(q_full, q_peer, seg++, 1);
+            tell(k_full, k_peer, kc++, C::kKSlots);
+            for (int j = 0; ok && j < w.n; ++j) {
+              if (j + 1 < w.n) tell(k_full, k_peer, kc++, C::kKSlots);
+              tell(v_full, v_peer, vc++, C::kVSlots);
             }
-          }
-          commit(s_full + 8 * buf);
-          if (t == kTiles - 1) commit(k_empty + 8 * st);
-          if (u == units - 1) commit(q_empty);
+          } while (ok && w.next(a));
+          if (!ok) atomicOr(&failed, 1u);
+        }
+      } else if (work) {
+        const uint32_t leader = elected();
+        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+        auto commit = [&](uint32_t bar) {
+          if constexpr (kPair) commit_pair(bar, leader);
+          else commit_to(bar, leader);
         };
-        auto issue_pv = [&](int u) {
-          const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1, n = k0 + j, st = n % C::kVSlots;
-          const uint32_t parity = ((u0 + u) >> 1) & 1, landed = (n / C::kVSlots) & 1;
-          // the accumulator's last job has been read
-          if (seg > 0 && u < kTiles && !wait(o_free + 8 * t, (seg - 1) & 1)) return false;
-          // a wait costs 60 ns even where there is nothing to wait for: those that are likely over come before those for the weights,
-          // the next unit's keys among them
-          if (t == 0 && !wait(v_full + 8 * st, landed)) return false;
-          if (kPair && !wait(v_peer + 8 * st, landed)) return false;
-          const bool more = u + 2 < units;
-          if (C::kHalves == 1 && more && !keys_there(u + 2)) return false;
-          if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
-          const uint64_t vd = smem_desc(sV + st * C::kVBytes, kKeysB * 128, 1024);
-          const uint32_t pa = tmem + C::kColS + buf * kKeysB;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {                    // by the page: the second half of the weights comes later
-            if (C::kHalves == 2 && h == 1) {
-              if (more && !keys_there(u + 2)) return false;
-              if (!wait(p_full + 8 * buf, parity)) return false;
-            }
+        constexpr uint32_t kM = kPair ? 2 * kRowsT : kRowsT;
+        constexpr uint32_t kIdS = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeysB >> 3) << 17) | ((kM >> 4) << 24);
+        constexpr uint32_t kIdO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((DH >> 3) << 17) | ((kM >> 4) << 24);
+        int k0 = 0, u0 = 0, seg = 0;                         // key blocks, units and jobs before the current job
+        bool ok = true;
+        do {
+          // the same in all lanes, and known to be: what hangs on it stays in uniform registers
+          const int blocks = __reduce_max_sync(0xffffffffu, w.n), units = blocks * kTiles;
+          auto keys_there = [&](int u) {
+            const int j = k0 + u / kTiles, st = j % C::kKSlots;
+            const uint32_t parity = (j / C::kKSlots) & 1;
+            return (u % kTiles != 0 || wait(k_full + 8 * st, parity)) && (!kPair || wait(k_peer + 8 * st, parity));
+          };
+          auto issue_s = [&](int u) {
+            const int j = k0 + u / kTiles, t = u % kTiles, st = j % C::kKSlots, buf = (u0 + u) & 1;
             fence_after();
 #pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; ++k) {
-              if constexpr (kPair) mma_ts_pair(tmem + C::kColO, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | k) ? 1u : 0u, leader);
-              else mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, vd + static_cast<uint64_t>((k * 2048) >> 4), kIdO, (j | k) ? 1u : 0u, leader);
+            for (int c = 0; c < C::kChunks; ++c) {
+              const uint64_t qd = smem_desc(sQ + (t * C::kChunks + c) * (kRowsT * 128), 16, 1024);
+              const uint64_t kd = smem_desc(sK + st * C::kKBytes + c * (C::kKPages * kPageTokens * 128), 16, 1024);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if constexpr (kPair) mma_ss_pair(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+                else mma_ss(tmem + C::kColS + buf * kKeysB, qd + 2 * k, kd + 2 * k, kIdS, (c | k) ? 1u : 0u, leader);
+              }
             }
+            commit(s_full + 8 * buf);
+            if (t == kTiles - 1) commit(k_empty + 8 * st);
+            if (u == units - 1) commit(q_empty);
+          };
+          auto issue_pv = [&](int u) {
+            const int j = u / kTiles, t = u % kTiles, buf = (u0 + u) & 1, n = k0 + j, st = n % C::kVSlots;
+            const uint32_t parity = ((u0 + u) >> 1) & 1, landed = (n / C::kVSlots) & 1;
+            // the accumulator's last job has been read
+            if (seg > 0 && u < kTiles && !wait(o_free + 8 * t, (seg - 1) & 1)) return false;
+            // a wait costs 60 ns even where there is nothing to wait for: those that are likely over come before those for the weights,
+            // the next unit's keys among them
+            if (t == 0 && !wait(v_full + 8 * st, landed)) return false;
+            if (kPair && !wait(v_peer + 8 * st, landed)) return false;
+            const bool more = u + 2 < units;
+            if (C::kHalves == 1 && more && !keys_there(u + 2)) return false;
+            if (!wait((C::kHalves == 2 ? p_half : p_full) + 8 * buf, parity)) return false;
+            const uint64_t vd = smem_desc(sV + st * C::kVBytes, kKeysB * 128, 1024);
+            const uint32_t pa = tmem + C::kColS + buf * kKeysB;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                    // by the page: the second half of the weights comes later
+              if (C::kHalves == 2 && h == 1) {
+                if (more && !keys_there(u + 2)) return false;
+                if (!wait(p_full + 8 * buf, parity)) return false;
+              }
+              fence_after();
+#pragma unroll
+              for (int k = 4 * h; k < 4 * h + 4; ++k) {
+                const uint64_t rows16 = vd + static_cast<uint64_t>((k * 2048) >> 4);
+                if constexpr (kPair) mma_ts_pair(tmem + C::kColO, pa + 8 * k, rows16, kIdO, (j | k) ? 1u : 0u, leader);
+                else mma_ts(tmem + C::kColO + t * DH, pa + 8 * k, rows16, kIdO, (j | k) ? 1u : 0u, leader);
+              }
+            }
+            if (t == kTiles - 1) commit(v_empty + 8 * st);
+            commit(o_done + 8 * buf);
+            if (more) issue_s(u + 2);
+            return true;
+          };
+          ok = wait(q_full, seg & 1) && (!kPair || wait(q_peer, seg & 1));
+          for (int u = 0; ok && u < min(units, 2); ++u) {
+            ok = keys_there(u);
+            if (ok) issue_s(u);
           }
-          if (t == kTiles - 1) commit(v_empty + 8 * st);
-          commit(o_done + 8 * buf);
-          if (more) issue_s(u + 2);
-          return true;
-        };
-        ok = wait(q_full, seg & 1) && (!kPair || wait(q_peer, seg & 1));
-        for (int u = 0; ok && u < min(units, 2); ++u) {
-          ok = keys_there(u);
-          if (ok) issue_s(u);
-        }
-        for (int u = 0; ok && u < units; ++u) ok = issue_pv(u);
-        k0 += blocks;
-        u0 += units;
-        ++seg;
-      } while (__any_sync(0xffffffffu, ok && w.next(a)));
-      if (!ok && leader) atomicOr(&failed, 1u);
+          for (int u = 0; ok && u < units; ++u) ok = issue_pv(u);
+          k0 += blocks;
+          u0 += units;
+          ++seg;
+        } while (__any_sync(0xffffffffu, ok && w.next(a)));
+        if (!ok && leader) atomicOr(&failed, 1u);
+      }
+    } else if (warp >= 10) {
+      // ---- the new rows into their slots ----
+      if (a.c.k_new_dev) store_rows<DH>(a, warp - 10);
     }
-  } else if (warp >= 10) {
-    // ---- the new rows into their slots ----
-    if (a.c.k_new_dev) store_rows<DH>(a, warp - 10);
-  }
   } else {
     // ---- weights ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     Walk w;
     if (w.begin(a, piece)) {
-    const int wg = warp >> 2, quad = warp & 3;
-    const int tile = kTiles == 2 ? wg : 0, part = kTiles == 2 ? 0 : wg;      // of this block; of the keys of a block
-    const int job_tile = kPair ? rank : tile;
-    auto announce = [&](uint32_t bar) {
-      fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair) arrive_first(bar);
-        else arrive_at(bar);
-      }
-    };
-    const int r = quad * 32 + lane;                        // row of the tile = lane of tensor memory
-    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    int block = 0;                                         // key blocks so far
-    bool ok = true;
-    do {
-      const int head = w.head_job * (a.by_heads ? 2 : 1) + (a.by_heads ? job_tile : 0);
-      const int t0 = w.k.t_first + (a.by_heads ? 0 : job_tile * kRowsT), t = t0 + r;
-      const int p = t < w.k.fresh ? w.k.first + t : -1;
-      const int p_last = w.k.first + w.k.t_end - 1;
-      const int warp_first = w.k.first + t0 + quad * 32;   // slots of the warp's rows: warp_first .. + 31
-      float m_ref = -INFINITY, l = 0.f;
-      for (int j = 0; j < w.n; ++j, ++block) {
-        const int u = kTiles == 2 ? 2 * block + wg : block;
-        const int slot0 = w.k.slot_of(w.k.place(w.j + j)), key = slot0 + part * kKeysThread;      // slots of the block's and this thread's first key
-        const int warp_last = min(warp_first + 31, p_last);
-        const bool inside = key + kKeysThread - 1 <= warp_first && warp_last >= warp_first &&
-                            (key + kKeysThread - 1 < a.c.sinks || warp_last - key < a.c.window);
-        const bool unseen = slot0 < w.k.low && slot0 + kKeysB > w.k.sinks;         // some of them, by all tokens
-        if (ok) ok = mbar_wait(s_full + 8 * (u & 1), (u >> 1) & 1);
-        fence_after();
-        const int note = notes[block % kBlockNotes];
-        const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
-        uint32_t x[kKeysThread];
-#pragma unroll
-        for (int i = 0; i < kKeysThread; i += 32) tmem_fetch32(at_s + i, x + i);
-        tmem_wait();
-#pragma unroll
-        for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
-        constexpr int kFullNote = kPageTokens | kPageTokens << 8;
-        // V's rows that hold nothing, or nothing that a token of the job sees: zeroed before anybody's weights are announced
-        if (note != kFullNote || unseen) {
-          const int st = block % C::kVSlots;
-          if (ok) ok = mbar_wait(v_full + 8 * st, (block / C::kVSlots) & 1);
-          if (tile == 0) {
-            // [64-column part][page][64 rows][128 bytes]: a thread has a row of some parts, its pieces in an order that meets all banks
-            const int h = r / kPageTokens, row = r % kPageTokens, slot = slot0 + r;
-            if (row >= ((note >> (8 * h)) & 255) || (slot >= w.k.sinks && slot < w.k.low)) {
-              unsigned char* at = prompt_smem + (sV - base) + st * C::kVBytes + r * 128;
-              for (int c = kTiles == 1 ? wg : 0; c < C::kVChunks; c += 3 - kTiles)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(at + c * (kKeysB * 128) + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      const int wg = warp >> 2, quad = warp & 3;
+      const int tile = kTiles == 2 ? wg : 0, part = kTiles == 2 ? 0 : wg;      // of this block; of the keys of a block
+      const int job_tile = kPair ? rank : tile;
+      auto announce = [&](uint32_t bar) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) arrive_first(bar);
+          else arrive_at(bar);
         }
-        if (note != kFullNote || !inside) {
-          // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
-          const int hi = p - key, lo = p - a.c.window + 1 - key, sk = a.c.sinks - key;
-#pragma unroll
-          for (int i = 0; i < kKeysThread / 32; ++i) {
-            const int within = part * kKeysThread + 32 * i;
-            const int held = (within < kPageTokens ? note & 255 : note >> 8) - within % kPageTokens;
-            const uint32_t see = low_bits(min(hi + 1, held + 32 * i) - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i));
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(see >> e & 1u)) x[32 * i + e] = 0xff800000u;
-          }
-        }
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kKeysThread; i += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-        float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * a.scale_log2;      // scale > 0
-        if constexpr (kTiles == 1) {
-          part_max[part][r] = top;
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-          top = max3(top, part_max[part ^ 1][r], top);
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        }
-        // the reference stays until a score is 2^8 above it, and is then put 2^8 above that score: weights are below 2^8, and a row whose
-        // first keys are poor ones (a few first tokens, the edge of its window) does not have O rescaled for its next ones
-        float m_new = m_ref;
-        if (!(top <= m_ref + 8.0f)) m_new = top + 8.0f;     // a score that is NaN makes the row NaN: the reference, and with it the sum
-        if (__any_sync(0xffffffffu, m_new != m_ref && m_ref != -INFINITY)) {
-          const float corr = m_new == m_ref || m_ref == -INFINITY ? 1.0f : exp2_ftz(m_ref - m_new);
-          l *= corr;
-          // O changes scale: the tile's products so far must have landed
-          const int before = u - kTiles;
-          if (ok) ok = mbar_wait(o_done + 8 * (before & 1), (before >> 1) & 1);
+      };
+      const int r = quad * 32 + lane;                        // row of the tile = lane of tensor memory
+      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+      int block = 0;                                         // key blocks so far
+      bool ok = true;
+      do {
+        const int head = w.head_job * (a.by_heads ? 2 : 1) + (a.by_heads ? job_tile : 0);
+        const int t0 = w.k.t_first + (a.by_heads ? 0 : job_tile * kRowsT), t = t0 + r;
+        const int p = t < w.k.fresh ? w.k.first + t : -1;
+        const int p_last = w.k.first + w.k.t_end - 1;
+        const int warp_first = w.k.first + t0 + quad * 32;   // slots of the warp's rows: warp_first .. + 31
+        float m_ref = -INFINITY, l = 0.f;
+        for (int j = 0; j < w.n; ++j, ++block) {
+          const int u = kTiles == 2 ? 2 * block + wg : block;
+          // slots of the block's and of this thread's first key
+          const int slot0 = w.k.slot_of(w.k.place(w.j + j)), key = slot0 + part * kKeysThread;
+          const int warp_last = min(warp_first + 31, p_last);
+          const bool inside = key + kKeysThread - 1 <= warp_first && warp_last >= warp_first &&
+                              (key + kKeysThread - 1 < a.c.sinks || warp_last - key < a.c.window);
+          const bool unseen = slot0 < w.k.low && slot0 + kKeysB > w.k.sinks;         // some of them, by all tokens
+          if (ok) ok = mbar_wait(s_full + 8 * (u & 1), (u >> 1) & 1);
           fence_after();
-#pragma unroll 1
-          for (int c0 = 0; c0 < DH / (3 - kTiles); c0 += 16) {
-            const uint32_t at = tmem + lanes + C::kColO + tile * DH + part * (DH / 2) + c0;
-            uint32_t o[16];
-            tmem_load16(at, o);
+          const int note = notes[block % kBlockNotes];
+          const uint32_t at_s = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * kKeysThread;
+          uint32_t x[kKeysThread];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_store16(at, o);
-          }
-        }
-        const float neg = m_new == -INFINITY ? 0.f : -m_new;
-        const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
-        const uint32_t at_p = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * (kKeysThread / 2);
-        uint64_t sums[2] = {0, 0};
+          for (int i = 0; i < kKeysThread; i += 32) tmem_fetch32(at_s + i, x + i);
+          tmem_wait();
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half) {
+          for (int i = 0; i < kKeysThread; i += 32) pin32(x + i);
+          constexpr int kFullNote = kPageTokens | kPageTokens << 8;
+          // V's rows that hold nothing, or nothing that a token of the job sees: zeroed before anybody's weights are announced
+          if (note != kFullNote || unseen) {
+            const int st = block % C::kVSlots;
+            if (ok) ok = mbar_wait(v_full + 8 * st, (block / C::kVSlots) & 1);
+            if (tile == 0) {
+              // [64-column part][page][64 rows][128 bytes]: a thread has a row of some parts, its pieces in an order that meets all banks
+              const int h = r / kPageTokens, row = r % kPageTokens, slot = slot0 + r;
+              if (row >= ((note >> (8 * h)) & 255) || (slot >= w.k.sinks && slot < w.k.low)) {
+                unsigned char* at = prompt_smem + (sV - base) + st * C::kVBytes + r * 128;
+                for (int c = kTiles == 1 ? wg : 0; c < C::kVChunks; c += 3 - kTiles)
 #pragma unroll
-          for (int i = half * (kKeysThread / kHalves); i < (half + 1) * (kKeysThread / kHalves); i += 2) {
-            const uint64_t e2 = fma_pair(pair_of(x[i], x[i + 1]), scale2, neg2);
-            float y0, y1;
-            if (kPolyOf > 0 && (i / 2) % kPolyOf == kPolyOf - 1) {
-              float e0, e1;
-              unpair(e2, &e0, &e1);
-              exp2_pair(pair_of(fmaxf(e0, -126.f), fmaxf(e1, -126.f)), &y0, &y1);
-            } else {
-              unpair(e2, &y0, &y1);
-              y0 = exp2_ftz(y0);
-              y1 = exp2_ftz(y1);
+                  for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(at + c * (kKeysB * 128) + ((i + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
             }
-            sums[(i / 2) & 1] = add_pair(sums[(i / 2) & 1], pair_of(y0, y1));
-            x[i / 2] = pack_bf16x2(y0, y1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
+          if (note != kFullNote || !inside) {
+            // the row's visible keys as bits: up to its own slot, in the window or among the first tokens, in a page that holds something
+            const int hi = p - key, lo = p - a.c.window + 1 - key, sk = a.c.sinks - key;
 #pragma unroll
-          for (int i = half * (kKeysThread / kHalves / 2); i < (half + 1) * (kKeysThread / kHalves / 2); i += 32) tmem_store32(at_p + i, x + i);
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          announce((half < kHalves - 1 ? p_half : p_full) + 8 * (u & 1));
-        }
-        float sum0, sum1;
-        unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
-        l += sum0 + sum1;
-        m_ref = m_new;
-      }
-      // the job's result, or the piece's part of it
-      const int u = kTiles == 2 ? 2 * (block - 1) + wg : block - 1;
-      if (ok) ok = mbar_wait(o_done + 8 * (u & 1), (u >> 1) & 1);
-      fence_after();
-      if constexpr (kTiles == 1) {
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        part_max[part][r] = l;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        l = part_max[0][r] + part_max[1][r];
-      }
-      const bool whole = w.whole();
-      const float inv = m_ref == -INFINITY ? 0.f : 1.0f / l;
-      const bool wide_out = ((reinterpret_cast<uintptr_t>(a.c.out_dev) & 31) | (a.c.ld_out & 15)) == 0;
-      const size_t part_row = (static_cast<size_t>(piece) * 2 + (w.j == 0 ? 1 : 0)) * (kJobTiles * kRowsT) + job_tile * kRowsT + r;
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) + (static_cast<size_t>(w.b) * a.c.tokens + min(t, a.c.tokens - 1)) * a.c.ld_out + head * DH;
+            for (int i = 0; i < kKeysThread / 32; ++i) {
+              const int within = part * kKeysThread + 32 * i;
+              const int held = (within < kPageTokens ? note & 255 : note >> 8) - within % kPageTokens;
+              const uint32_t see = low_bits(min(hi + 1, held + 32 * i) - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i));
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(see >> e & 1u)) x[32 * i + e] = 0xff800000u;
+            }
+          }
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kKeysThread; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
+          float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * a.scale_log2;      // scale > 0
+          if constexpr (kTiles == 1) {
+            part_max[part][r] = top;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+            top = max3(top, part_max[part ^ 1][r], top);
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+          }
+          // the reference stays until a score is 2^8 above it, and is then put 2^8 above that score: weights are below 2^8, and a row whose
+          // first keys are poor ones (a few first tokens, the edge of its window) does not have O rescaled for its next ones
+          float m_new = m_ref;
+          if (!(top <= m_ref + 8.0f)) m_new = top + 8.0f;     // a score that is NaN makes the row NaN: the reference, and with it the sum
+          if (__any_sync(0xffffffffu, m_new != m_ref && m_ref != -INFINITY)) {
+            const float corr = m_new == m_ref || m_ref == -INFINITY ? 1.0f : exp2_ftz(m_ref - m_new);
+            l *= corr;
+            // O changes scale: the tile's products so far must have landed
+            const int before = u - kTiles;
+            if (ok) ok = mbar_wait(o_done + 8 * (before & 1), (before >> 1) & 1);
+            fence_after();
 #pragma unroll 1
-      for (int c0 = part * (DH / 2); c0 < (kTiles == 2 ? DH : (part + 1) * (DH / 2)); c0 += 32) {
-        uint32_t o[32];
-        tmem_load32(tmem + lanes + C::kColO + tile * DH + c0, o);
-        if (whole && p >= 0) {
-          uint32_t y[16];
+            for (int c0 = 0; c0 < DH / (3 - kTiles); c0 += 16) {
+              const uint32_t at = tmem + lanes + C::kColO + tile * DH + part * (DH / 2) + c0;
+              uint32_t o[16];
+              tmem_load16(at, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-          if (wide_out) {
-            store32(out + c0, y);
-            store32(out + c0 + 16, y + 8);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(out + c0 + 2 * i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_store16(at, o);
+            }
           }
-        } else if (!whole) {
+          const float neg = m_new == -INFINITY ? 0.f : -m_new;
+          const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), neg2 = pair_of(neg, neg);
+          const uint32_t at_p = tmem + lanes + C::kColS + (u & 1) * kKeysB + part * (kKeysThread / 2);
+          uint64_t sums[2] = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) store32(a.part_o + part_row * DH + c0 + i, o + i);
+          for (int half = 0; half < kHalves; ++half) {
+#pragma unroll
+            for (int i = half * (kKeysThread / kHalves); i < (half + 1) * (kKeysThread / kHalves); i += 2) {
+              const uint64_t e2 = fma_pair(pair_of(x[i], x[i + 1]), scale2, neg2);
+              float y0, y1;
+              if (kPolyOf > 0 && (i / 2) % kPolyOf == kPolyOf - 1) {
+                float e0, e1;
+                unpair(e2, &e0, &e1);
+                exp2_pair(pair_of(fmaxf(e0, -126.f), fmaxf(e1, -126.f)), &y0, &y1);
+              } else {
+                unpair(e2, &y0, &y1);
+                y0 = exp2_ftz(y0);
+                y1 = exp2_ftz(y1);
+              }
+              sums[(i / 2) & 1] = add_pair(sums[(i / 2) & 1], pair_of(y0, y1));
+              x[i / 2] = pack_bf16x2(y0, y1);
+            }
+#pragma unroll
+            for (int i = half * (kKeysThread / kHalves / 2); i < (half + 1) * (kKeysThread / kHalves / 2); i += 32) tmem_store32(at_p + i, x + i);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            announce((half < kHalves - 1 ? p_half : p_full) + 8 * (u & 1));
+          }
+          float sum0, sum1;
+          unpair(add_pair(sums[0], sums[1]), &sum0, &sum1);
+          l += sum0 + sum1;
+          m_ref = m_new;
         }
-      }
-      if (!whole && part == 0) a.part_ml[part_row] = make_float2(m_ref, l);
-      announce(o_free + 8 * tile);
-    } while (w.next(a));
-    if (!ok) atomicOr(&failed, 1u);
+        // the job's result, or the piece's part of it
+        const int u = kTiles == 2 ? 2 * (block - 1) + wg : block - 1;
+        if (ok) ok = mbar_wait(o_done + 8 * (u & 1), (u >> 1) & 1);
+        fence_after();
+        if constexpr (kTiles == 1) {
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+          part_max[part][r] = l;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+          l = part_max[0][r] + part_max[1][r];
+        }
+        const bool whole = w.whole();
+        const float inv = m_ref == -INFINITY ? 0.f : 1.0f / l;
+        const bool wide_out = ((reinterpret_cast<uintptr_t>(a.c.out_dev) & 31) | (a.c.ld_out & 15)) == 0;
+        const size_t part_row = (static_cast<size_t>(piece) * 2 + (w.j == 0 ? 1 : 0)) * (kJobTiles * kRowsT) + job_tile * kRowsT + r;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.c.out_dev) +
+                             (static_cast<size_t>(w.b) * a.c.tokens + min(t, a.c.tokens - 1)) * a.c.ld_out + head * DH;
+#pragma unroll 1
+        for (int c0 = part * (DH / 2); c0 < (kTiles == 2 ? DH : (part + 1) * (DH / 2)); c0 += 32) {
+          uint32_t o[32];
+          tmem_load32(tmem + lanes + C::kColO + tile * DH + c0, o);
+          if (whole && p >= 0) {
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            if (wide_out) {
+              store32(out + c0, y);
+              store32(out + c0 + 16, y + 8);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(out + c0 + 2 * i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+            }
+          } else if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) store32(a.part_o + part_row * DH + c0 + i, o + i);
+          }
+        }
+        if (!whole && part == 0) a.part_ml[part_row] = make_float2(m_ref, l);
+        announce(o_free + 8 * tile);
+      } while (w.next(a));
+      if (!ok) atomicOr(&failed, 1u);
     }
     if (a.c.k_new_dev) store_rows<DH>(a, 2 + warp);
   }

@@ -464,3 +464,33 @@ def test_rows_that_fill_three_eighths_and_five(cuda_device, heads, kv_heads, d_h
         before = w_in[b, :, :n].copy()
         before[:, n - f:] = 0
         assert (np.abs(w_out[b, :, :n] - before - received[b]) <= 2.0 ** -13 * received[b] + 2.0 ** -22 * (before + received[b])).all()
+
+
+@pytest.mark.parametrize("d_heads", [(256, 256), (128, 64), (256, 128)])
+def test_two_prompts_at_once(cuda_device, d_heads):
+    """Two streams with prompts of their own, each storing its keys and values, replayed from graphs: what each gives alone."""
+    from mesh_transformer.cache import cache_attention
+    sets = []
+    for seed, d_head in zip((71, 73), d_heads):
+        c = Cache(seed, 3, 12, 2, d_head, [700, 333, 512])
+        sets.append((c, *(c.rows(3, 320, h, d_head, torch.bfloat16) for h in (4, 2, 2))))
+    call = lambda c, q, k, v: cache_attention(q, k, v, c.kpool, c.vpool, c.page_table, c.lengths_dev, window=300, sinks=4)
+    alone = [call(*s) for s in sets]
+    pools = [s[0].kpool.clone() for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(*s))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for want, got, s, pool in zip(alone, outs, sets, pools):
+            assert torch.equal(want, got) and torch.equal(s[0].kpool.view(torch.int16), pool.view(torch.int16))

@@ -251,3 +251,18 @@ def test_drafts_over_a_cache(cuda_device):
             held = [x[kept[h]] for h, x in enumerate(held)]
             cuts += 1
     assert int(lengths) == len(held[0]) and accepted >= 20 and cuts >= 1
+
+
+def test_two_checks_at_once(cuda_device):
+    from mesh_transformer.sampling import verify_drafts
+    sets = [_inputs(seed, 30, 4, 20000, torch.float32, agree=0.5) for seed in (43, 47)]
+    alone = [verify_drafts(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(verify_drafts(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for want, have in zip(alone, got) for x, y in zip(want, have))
