@@ -44,7 +44,7 @@ int32_t check_args(const mtj_cache_attn_args* a, std::string* err) {
   const int64_t most = 0x7fffffff, rows = static_cast<int64_t>(a->batch) * a->tokens;
   if (rows > most || rows * a->heads > most) return bad("batch * tokens * heads is too large");
   if (static_cast<int64_t>(a->batch) * a->kv_heads > most / kPageTokens / a->pages) return bad("batch * kv_heads * slots is too large");
-  if (!cache_prompt_fits(*a)) return bad("more than 2^20 new tokens a sequence");
+  if (!cache_prompt_fits(*a)) return bad("too many new tokens for one call");
   if (a->kv_heads > 65535) return bad("too many key heads");
   if (static_cast<int64_t>(a->n_pages) * a->kv_heads > most / kPageTokens) return bad("n_pages * kv_heads is too large");
   return MTJ_OK;

@@ -1199,18 +1199,25 @@ int pieces_for(const mtj_cache_attn_args& c) { return c.d_head == 256 ? kBlocks 
 constexpr int64_t kPlanBytes = ((kPlanList + kMostEntries) * 4 + 255) / 256 * 256;
 int64_t part_rows(const mtj_cache_attn_args& c) { return static_cast<int64_t>(pieces_for(c)) * 2 * kJobTiles * kRowsT; }
 
-// whether no job can lie in several pieces: jobs of few blocks are taken whole
-bool all_whole(const mtj_cache_attn_args& c) {
+// most key blocks of a job
+int64_t most_blocks(const mtj_cache_attn_args& c) {
   const int64_t slots = (static_cast<int64_t>(c.pages) * kPageTokens + kKeysB - 1) / kKeysB + 1;      // and the block between cached and new
   const int64_t seen = (static_cast<int64_t>(c.window) + job_span(c)) / kKeysB + 3 + (static_cast<int64_t>(c.sinks) + kKeysB - 1) / kKeysB + 1;
-  return std::min(slots, seen) <= kJoinCost;
+  return std::min(slots, seen);
+}
+// whether no job can lie in several pieces: jobs of few blocks are taken whole
+bool all_whole(const mtj_cache_attn_args& c) { return most_blocks(c) <= kJoinCost; }
+// sequences of a launch: as many as the plan has entries for, and as have their key blocks counted in 32 bits
+int64_t most_sequences(const mtj_cache_attn_args& c) {
+  const int64_t token_jobs = (static_cast<int64_t>(c.tokens) + job_span(c) - 1) / job_span(c);
+  return std::min(kMostEntries / token_jobs, 0x7fffffff / (token_jobs * most_blocks(c)));
 }
 
 }  // namespace
 
 int64_t cache_prompt_scratch(const mtj_cache_attn_args& c) { return kPlanBytes + part_rows(c) * (8 + c.d_head * 4); }
 
-bool cache_prompt_fits(const mtj_cache_attn_args& c) { return (c.tokens + job_span(c) - 1) / job_span(c) <= kMostEntries; }
+bool cache_prompt_fits(const mtj_cache_attn_args& c) { return most_sequences(c) > 0; }
 
 cudaError_t run_cache_prompt(const mtj_cache_attn_args& c, char* scratch, cudaStream_t s) {
   PromptArgs a = {};
@@ -1224,7 +1231,7 @@ cudaError_t run_cache_prompt(const mtj_cache_attn_args& c, char* scratch, cudaSt
   a.plan = reinterpret_cast<int*>(scratch);
   a.part_ml = reinterpret_cast<float2*>(scratch + kPlanBytes);
   a.part_o = reinterpret_cast<float*>(scratch + kPlanBytes + part_rows(c) * 8);
-  const int most = kMostEntries / a.token_jobs;        // sequences of a launch
+  const int most = static_cast<int>(most_sequences(c));
   for (int b0 = 0; b0 < c.batch; b0 += most) {
     a.c.batch = std::min(most, c.batch - b0);
     const bool join = !all_whole(c);

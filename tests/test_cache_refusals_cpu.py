@@ -142,3 +142,12 @@ def test_numbers_beyond_the_kernels_own(L):
     long = dict(vocab=2 ** 30 + 1, ld_target=2 ** 31, ld_draft=2 ** 31, batch=1, drafts=0)
     assert L.lib.mtj_verify_drafts(ctypes.byref(_verify(L, **long)), BASE, 1 << 40, None) == 1 and "vocabulary" in err()
     assert L.lib.mtj_verify_drafts(ctypes.byref(_verify(L, temp=float("inf"))), BASE, 1 << 40, None) == 1 and "temp" in err()
+
+
+def test_prompts_beyond_the_plan(L):
+    """New tokens of a sequence, and the key blocks that all of them see, are counted in 32 bits."""
+    size = lambda **kw: L.lib.mtj_k_cache_attn_scratch_bytes(ctypes.byref(_attn(L, batch=1, heads=1, kv_heads=1, **kw)))
+    assert size(tokens=2 ** 20, pages=2 ** 15, window=2 ** 30) > 0
+    assert size(tokens=2 ** 21 + 1, pages=2 ** 16) == -1
+    assert size(tokens=2 ** 20, pages=2 ** 20, window=2 ** 30) == -1 and "new tokens" in L.lib.mtj_last_error().decode()
+    assert size(tokens=2 ** 20, pages=2 ** 20, window=2 ** 12) > 0
