@@ -21,32 +21,37 @@ _DTYPES = {torch.bfloat16: MTJ_BF16, torch.float32: MTJ_F32}
 # token's call is launched in a few microseconds, of which filling a ctypes structure would be a quarter
 _ATTN_ARGS = struct.Struct("@12P4q10if4x").pack
 _EVICT_ARGS = struct.Struct("@11P8i").pack
-_stream = torch._C._cuda_getCurrentRawStream
+_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+# tensors are asked for the number of their GPU (-1: the host's memory), which costs less than for their device
 
 
-def _want(t, name, dtype, shape, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+def _want(t, name, dtype, shape, index):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on cuda:{index}")
 
 
 def _pool_shape(kpool, vpool, page_table, lengths):
-    if not (isinstance(kpool, torch.Tensor) and kpool.is_cuda and kpool.dim() == 4 and kpool.shape[2] == PAGE_TOKENS):
-        raise ValueError(f"kpool must be a CUDA tensor [n_pages, kv_heads, {PAGE_TOKENS}, d_head]")
-    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
-        raise ValueError("page_table must be a tensor [batch, pages]")
-    shape, device, table = kpool.shape, kpool.device, page_table.shape
-    _want(kpool, "kpool", torch.bfloat16, shape, device)
-    _want(vpool, "vpool", torch.bfloat16, shape, device)
-    _want(page_table, "page_table", torch.int32, table, device)
-    _want(lengths, "lengths", torch.int32, table[:1], device)
-    return shape, table, device
+    shape = kpool.shape if isinstance(kpool, torch.Tensor) else ()
+    if len(shape) != 4 or shape[2] != PAGE_TOKENS or not kpool.is_cuda or kpool.dtype != _BF16 or not kpool.is_contiguous():
+        raise ValueError(f"kpool must be a contiguous bfloat16 CUDA tensor [n_pages, kv_heads, {PAGE_TOKENS}, d_head]")
+    table = page_table.shape if isinstance(page_table, torch.Tensor) else ()
+    index = kpool.get_device()
+    if len(table) != 2 or page_table.dtype != _I32 or page_table.get_device() != index or not page_table.is_contiguous():
+        raise ValueError(f"page_table must be a contiguous int32 tensor [batch, pages] on cuda:{index}")
+    _want(vpool, "vpool", _BF16, shape, index)
+    _want(lengths, "lengths", _I32, table[:1], index)
+    return shape, table, index
 
 
-def _rows(t, name, shape, like):
+def _like(t, name, shape, dtype, index):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != index or t.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on cuda:{index}")
+
+
+def _rows(t, shape):
     """``t`` [batch, tokens, heads, d_head] with heads side by side in a row, rows at one stride and 16-byte aligned (a slice
     of a fused projection is one); anything else is copied."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
-        raise ValueError(f"{name} must be a {like.dtype} tensor {list(shape)} on {like.device}")
     at = t.data_ptr()
     if t.is_contiguous():
         if at & 15:
@@ -82,44 +87,46 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
 
     ``status`` int32 [1], if given, collects what the GPU found wrong: bit 1 a length or a page number outside the cache (that
     sequence counts as empty, that page as unseen), bit 0 a wait that ran out."""
-    pool, table, device = _pool_shape(kpool, vpool, page_table, lengths)
-    n_pages, kv_heads, _, d_head = pool
-    batch, pages = table
+    (n_pages, kv_heads, _, d_head), (batch, pages), index = _pool_shape(kpool, vpool, page_table, lengths)
     shape = q.shape if isinstance(q, torch.Tensor) else ()
-    dtype = _DTYPES.get(q.dtype) if len(shape) == 4 else None
-    if dtype is None or q.device != device or shape[0] != batch or shape[3] != d_head or shape[1] < 1 or shape[2] < 1:
-        raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on {device}")
+    of_q = q.dtype if len(shape) == 4 else None
+    dtype = _DTYPES.get(of_q)
+    if dtype is None or q.get_device() != index or shape[0] != batch or shape[3] != d_head or shape[1] < 1 or shape[2] < 1:
+        raise ValueError(f"q must be a bfloat16 or float32 tensor [{batch}, tokens, heads, {d_head}] on cuda:{index}")
     _, tokens, heads, _ = shape
-    q, at_q, ld_q = _rows(q, "q", shape, q)
+    q, at_q, ld_q = _rows(q, shape)
     at_k = at_v = ld_k = ld_v = 0
     if k is not None and v is not None:
         new_shape = (batch, tokens, kv_heads, d_head)
-        k, at_k, ld_k = _rows(k, "k", new_shape, q)
-        v, at_v, ld_v = _rows(v, "v", new_shape, q)
+        _like(k, "k", new_shape, of_q, index)
+        _like(v, "v", new_shape, of_q, index)
+        k, at_k, ld_k = _rows(k, new_shape)
+        v, at_v, ld_v = _rows(v, new_shape)
     elif k is not None or v is not None:
         raise ValueError("k and v come together")
     at_new = at_status = at_in = at_out = 0
     if new is not None:
-        _want(new, "new", torch.int32, (batch,), device)
+        _want(new, "new", _I32, (batch,), index)
         at_new = new.data_ptr()
     if status is not None:
-        _want(status, "status", torch.int32, (1,), device)
+        _want(status, "status", _I32, (1,), index)
         at_status = status.data_ptr()
     if weights is not None or weights_out is not None:
         if weights_out is None:
             weights_out = weights
         slots = (batch, kv_heads, pages * PAGE_TOKENS)
-        _want(weights_out, "weights_out", torch.float32, slots, device)
+        _want(weights_out, "weights_out", _F32, slots, index)
         at_out = weights_out.data_ptr()
         if weights is not None:
-            _want(weights, "weights", torch.float32, slots, device)
+            _want(weights, "weights", _F32, slots, index)
             at_in = weights.data_ptr()
     if out is None:
-        out = torch.empty(batch, tokens, heads, d_head, dtype=q.dtype, device=device)
+        out = torch.empty(batch, tokens, heads, d_head, dtype=of_q, device=kpool.device)
         at, ld_out = out.data_ptr(), heads * d_head
     else:
         given = out
-        out, at, ld_out = _rows(out, "out", shape, q)
+        _like(out, "out", shape, of_q, index)
+        out, at, ld_out = _rows(out, shape)
         if out is not given:
             raise ValueError("out must have its heads side by side, rows at one stride and a 16-byte alignment")
     try:
@@ -129,20 +136,19 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
                        d_head ** -0.5 if scale is None else scale)
     except (struct.error, OverflowError, TypeError) as e:
         raise ValueError(f"window and sinks must be whole numbers, scale a number: {e}") from None
-    index = device.index
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
-            _run_attention(a, device, index)
+            _run_attention(a, kpool, index)
     else:
-        _run_attention(a, device, index)
+        _run_attention(a, kpool, index)
     return out
 
 
-def _run_attention(a, device, index):
+def _run_attention(a, kpool, index):
     nbytes = lib.mtj_k_cache_attn_scratch_bytes(a)
     if nbytes < 0:
         raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=kpool.device)
     check(lib.mtj_k_cache_attn(a, scratch.data_ptr(), nbytes, _stream(index)))
 
 
@@ -155,22 +161,21 @@ def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, f
     (-1 behind the last), and the cache as it is now.  The new table of a sequence that was cut names its spare pages, with -1
     behind them where the caller puts pages for the tokens to come; its old pages are free again.  Sequences of ``keep`` slots
     or fewer keep their pages and leave their spare ones unused."""
-    (n_pages, kv_heads, _, d_head), (batch, pages), device = _pool_shape(kpool, vpool, page_table, lengths)
+    (n_pages, kv_heads, _, d_head), (batch, pages), index = _pool_shape(kpool, vpool, page_table, lengths)
     keep, first, last = int(keep), int(first), int(last)
     if keep < 1 or first < 0 or last < 0 or first + last > keep:
         raise ValueError("keep must be positive and hold the first and the last slots")
-    _want(weights, "weights", torch.float32, (batch, kv_heads, pages * PAGE_TOKENS), device)
-    _want(spare_pages, "spare_pages", torch.int32, (batch, (keep + PAGE_TOKENS - 1) // PAGE_TOKENS), device)
+    _want(weights, "weights", _F32, (batch, kv_heads, pages * PAGE_TOKENS), index)
+    _want(spare_pages, "spare_pages", _I32, (batch, (keep + PAGE_TOKENS - 1) // PAGE_TOKENS), index)
     if status is not None:
-        _want(status, "status", torch.int32, (1,), device)
-    kept = torch.empty(batch, kv_heads, keep, dtype=torch.int32, device=device)
+        _want(status, "status", _I32, (1,), index)
+    kept = torch.empty(batch, kv_heads, keep, dtype=_I32, device=kpool.device)
     lengths_out, weights_out, table_out = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(page_table)
     a = _EVICT_ARGS(
         kpool.data_ptr(), vpool.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), weights.data_ptr(), spare_pages.data_ptr(),
         kept.data_ptr(), lengths_out.data_ptr(), weights_out.data_ptr(), table_out.data_ptr(),
         status.data_ptr() if status is not None else 0, n_pages, batch, pages, kv_heads, d_head, keep, first, last)
-    index = device.index
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             check(lib.mtj_k_cache_evict(a, _stream(index)))
     else:

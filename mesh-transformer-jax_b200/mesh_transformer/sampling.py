@@ -101,10 +101,8 @@ _LOGIT_TYPES = {torch.float32: MTJ_F32, torch.bfloat16: MTJ_BF16}
 _VERIFY_ARGS = struct.Struct("@10P4q4if4x").pack           # mtj_verify_args, the fields of MtjVerifyArgs
 
 
-def _logit_rows(t, name, like, shape):
+def _logit_rows(t, shape):
     """``t`` [batch, rows, vocab] with unit stride inside a row; anything else is copied."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
-        raise ValueError(f"{name} must be a {like.dtype} tensor {list(shape)} on {like.device}")
     vocab, s = shape[2], t.stride()
     if s[2] != 1 and vocab > 1 or s[1] < vocab:
         t = t.contiguous()
@@ -112,9 +110,9 @@ def _logit_rows(t, name, like, shape):
     return t, max(s[1], vocab), s[0]
 
 
-def _plain_rows(t, name, dtype, shape, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
-        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on {device}")
+def _plain_rows(t, name, dtype, shape, index):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != index or t.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -133,23 +131,28 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
     is not, from ``p`` behind the last.  Returns device tensors, nothing is read back: tokens int32 [batch, drafts + 1] (the
     taken ones, the next one, -1 behind it), the number taken int32 [batch], and log p_k of every token that comes out float32
     [batch, drafts + 1] (0 behind the last)."""
-    if not isinstance(target_logits, torch.Tensor) or not target_logits.is_cuda or target_logits.dim() != 3 or \
-            target_logits.dtype not in _LOGIT_TYPES or min(target_logits.shape) < 1:
+    shape = target_logits.shape if isinstance(target_logits, torch.Tensor) else ()
+    kind = target_logits.dtype if len(shape) == 3 and target_logits.is_cuda and min(shape) >= 1 else None
+    dtype = _LOGIT_TYPES.get(kind)
+    if dtype is None:
         raise ValueError("target_logits must be a float32 or bfloat16 CUDA tensor [batch, drafts + 1, vocab]")
-    batch, rows, vocab = target_logits.shape
-    drafts, dev = rows - 1, target_logits.device
-    target, ld_target, batch_target = _logit_rows(target_logits, "target_logits", target_logits, (batch, rows, vocab))
+    batch, rows, vocab = shape
+    drafts, index, dev = rows - 1, target_logits.get_device(), target_logits.device
+    target, ld_target, batch_target = _logit_rows(target_logits, shape)
     draft, ld_draft, batch_draft = None, 0, 0
     if draft_logits is not None:
-        draft, ld_draft, batch_draft = _logit_rows(draft_logits, "draft_logits", target, (batch, drafts, vocab))
-    tokens = _plain_rows(draft_tokens, "draft_tokens", torch.int32, (batch, drafts), dev)
-    accept = _plain_rows(accept, "accept", torch.float32, (batch, drafts), dev)
-    noise = _plain_rows(noise, "noise", torch.float32, (batch, vocab), dev)
+        if not isinstance(draft_logits, torch.Tensor) or draft_logits.dtype != kind or draft_logits.get_device() != index or \
+                draft_logits.shape != (batch, drafts, vocab):
+            raise ValueError(f"draft_logits must be a {kind} tensor {[batch, drafts, vocab]} on cuda:{index}")
+        draft, ld_draft, batch_draft = _logit_rows(draft_logits, (batch, drafts, vocab))
+    tokens = _plain_rows(draft_tokens, "draft_tokens", torch.int32, (batch, drafts), index)
+    accept = _plain_rows(accept, "accept", torch.float32, (batch, drafts), index)
+    noise = _plain_rows(noise, "noise", torch.float32, (batch, vocab), index)
     if count is not None:
-        count = _plain_rows(count, "count", torch.int32, (batch,), dev)
+        count = _plain_rows(count, "count", torch.int32, (batch,), index)
     temps = None
     if isinstance(temp, torch.Tensor):
-        temps, temp = _plain_rows(temp, "temp", torch.float32, (batch,), dev), 1.0
+        temps, temp = _plain_rows(temp, "temp", torch.float32, (batch,), index), 1.0
     out = torch.empty(batch, rows, dtype=torch.int32, device=dev)
     taken = torch.empty(batch, dtype=torch.int32, device=dev)
     logprobs = torch.empty(batch, rows, dtype=torch.float32, device=dev)
@@ -157,20 +160,20 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
         a = _VERIFY_ARGS(target.data_ptr(), draft.data_ptr() if draft is not None and drafts else 0, tokens.data_ptr(),
                          accept.data_ptr(), noise.data_ptr(), count.data_ptr() if count is not None else 0,
                          temps.data_ptr() if temps is not None else 0, out.data_ptr(), taken.data_ptr(), logprobs.data_ptr(),
-                         ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, _LOGIT_TYPES[target.dtype], temp)
+                         ld_target, batch_target, ld_draft, batch_draft, batch, drafts, vocab, dtype, temp)
     except (struct.error, OverflowError, TypeError) as e:
         raise ValueError(f"temp must be a number or a tensor: {e}") from None
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev.index):
-            _run_verify(a, dev)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            _run_verify(a, dev, index)
     else:
-        _run_verify(a, dev)
+        _run_verify(a, dev, index)
     return out, taken, logprobs
 
 
-def _run_verify(a, dev):
+def _run_verify(a, dev, index):
     nbytes = lib.mtj_verify_scratch_bytes(a)
     if nbytes < 0:
         raise ValueError(lib.mtj_last_error().decode("utf-8", "replace"))
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    check(lib.mtj_verify_drafts(a, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev.index)))
+    check(lib.mtj_verify_drafts(a, scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(index)))

@@ -494,3 +494,40 @@ def test_two_prompts_at_once(cuda_device, d_heads):
         torch.cuda.synchronize()
         for want, got, s, pool in zip(alone, outs, sets, pools):
             assert torch.equal(want, got) and torch.equal(s[0].kpool.view(torch.int16), pool.view(torch.int16))
+
+
+def test_python_refusals_with_tensors_on_a_gpu(cuda_device):
+    from mesh_transformer.cache import cache_attention, cache_evict
+    from mesh_transformer.sampling import verify_drafts
+    c = Cache(79, 2, 3, 2, 64, [100, 90])
+    q, k = c.rows(2, 3, 4, 64, torch.bfloat16), c.rows(2, 3, 2, 64, torch.bfloat16)
+    good = dict(q=q, k=k, v=k, kpool=c.kpool, vpool=c.vpool, page_table=c.page_table, lengths=c.lengths_dev)
+    before = c.kpool.clone()
+    w = torch.zeros((2, 2, 192), device="cuda")
+    for bad in (dict(q=q.half()), dict(q=q.cpu()), dict(q=q[:1]), dict(q=q[..., :32]), dict(q=q[:, :, 0]), dict(q=None), dict(k=None), dict(v=None),
+                dict(k=k.float()), dict(k=k.cpu()), dict(v=k[:, :2]), dict(v=q), dict(kpool=c.kpool.float()), dict(kpool=c.kpool.cpu()),
+                dict(kpool=c.kpool.transpose(0, 1)), dict(kpool=c.kpool[:, :, :32]), dict(vpool=c.vpool[1:]), dict(vpool=c.vpool.cpu()),
+                dict(vpool=None), dict(page_table=c.page_table.long()), dict(page_table=c.page_table[0]), dict(page_table=c.page_table.cpu()),
+                dict(page_table=c.page_table.t().contiguous().t()), dict(lengths=c.lengths_dev[:1]), dict(lengths=c.lengths_dev.float()),
+                dict(lengths=[100, 90]), dict(new=c.lengths_dev[:1]), dict(new=c.lengths_dev.cpu()), dict(status=c.lengths_dev), dict(weights=w.double()),
+                dict(weights=w[:, :1]), dict(weights_out=w.cpu()), dict(out=q.float()), dict(out=torch.empty_like(q)[:1]),
+                dict(out=torch.empty((2, 3, 4, 128), dtype=torch.bfloat16, device="cuda")[..., ::2]), dict(window=0), dict(window=1.5), dict(sinks=-1),
+                dict(scale=0.0), dict(scale="1")):
+        with pytest.raises(ValueError):
+            cache_attention(**{**good, **bad})
+    spare = torch.zeros((2, 1), dtype=torch.int32, device="cuda")
+    for bad in (dict(weights=w.half()), dict(weights=w[:, :, :64]), dict(spare_pages=spare.long()), dict(spare_pages=spare[:1]), dict(keep=0), dict(keep=65),
+                dict(first=60, last=5), dict(first=-1), dict(status=spare), dict(lengths=c.lengths_dev.cpu())):
+        with pytest.raises(ValueError):
+            cache_evict(**{**dict(kpool=c.kpool, vpool=c.vpool, page_table=c.page_table, lengths=c.lengths_dev, weights=w, spare_pages=spare, keep=64), **bad})
+    logits, u = torch.zeros((2, 3, 50), device="cuda"), torch.full((2, 50), 0.5, device="cuda")
+    drafts = torch.zeros((2, 2), dtype=torch.int32, device="cuda")
+    good = dict(target_logits=logits, draft_logits=logits[:, :2], draft_tokens=drafts, accept=u[:, :2], noise=u)
+    for bad in (dict(target_logits=logits.half()), dict(target_logits=logits.cpu()), dict(target_logits=logits[0]), dict(target_logits=None),
+                dict(draft_logits=logits), dict(draft_logits=logits[:, :2].bfloat16()), dict(draft_tokens=drafts.long()), dict(draft_tokens=drafts[:1]),
+                dict(accept=u), dict(noise=u.double()), dict(noise=u.cpu()), dict(count=drafts), dict(temp=None), dict(temp="1"), dict(temp=float("inf")),
+                dict(temp=u), dict(temp=torch.ones(2, dtype=torch.float64, device="cuda"))):
+        with pytest.raises(ValueError):
+            verify_drafts(**{**good, **bad})
+    torch.cuda.synchronize()
+    assert torch.equal(before.view(torch.int16), c.kpool.view(torch.int16))
