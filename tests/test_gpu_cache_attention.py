@@ -531,3 +531,10 @@ def test_python_refusals_with_tensors_on_a_gpu(cuda_device):
             verify_drafts(**{**good, **bad})
     torch.cuda.synchronize()
     assert torch.equal(before.view(torch.int16), c.kpool.view(torch.int16))
+
+
+@pytest.mark.parametrize("tokens,d_head", [(1, 64), (5, 128), (200, 64), (200, 128), (200, 256)])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 40, 2 ** 40), (1, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_windows_and_first_tokens_at_the_ends_of_their_range(cuda_device, tokens, d_head, window, sinks):
+    _, out, outs, _, spread, _ = _run(83, 2, 4, 2, d_head, tokens, [tokens + 310, tokens], [tokens, tokens], window, sinks, torch.bfloat16)
+    _check(out, outs, spread, torch.bfloat16, 2.0 ** -8)
