@@ -22,7 +22,7 @@
 // window, are zeroed in the tile, since weight zero times whatever stands there must be zero.
 //
 // 8 key heads of 128 with 4 query heads each: one token of 32 sequences of 2000 to 16383 slots 197 us, 1.21 GB at 6.1 TB/s, and 31 us for
-// the join that adds up the weights; five tokens of 8 sequences, window 4096, 40 us for 107 MB: there the chain of a tile (two products
+// the join that adds up the weights; five tokens of 8 sequences, window 4096, 38 to 41 us for 107 MB: there the chain of a tile (two products
 // with a softmax between them, 20 rows) and the ragged ends of 64 units count, not the bytes.
 #include <cuda.h>
 #include <math.h>
