@@ -199,36 +199,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) verify_rows_kernel(const mtj_v
           if (entry(x, u, e) == top) where = min(where, it.i0 + (u * 32 + lane) * kVec + e);
       where = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(where)));
     } else if (top > -INFINITY) {
-      // 2^(l scale - base), and the rounding of base = top scale taken out of the sum
-      const float scale = kLog2e / it.temp, base = top * scale;
-      if (fabsf(base) < 1e30f) {
-        const uint64_t scale2 = two(scale, scale), base2 = two(-base, -base);
-        uint64_t s0 = 0, s1 = 0;
+      // 2^((l - top) scale): the largest entry is taken away first.  (l scale - top scale in one rounding has top scale's own rounding in
+      // every exponent, 2^-24 of a number that has no bound: at temperatures below 1e-3 more than the shares have bits.)
+      const float scale = kLog2e / it.temp;
+      const uint64_t scale2 = two(scale, scale), top2 = two(-top, -top);
+      uint64_t s0 = 0, s1 = 0;
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u)
+      for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-          for (int e = 0; e < kVec; e += 4) {
-            uint64_t y0, y1;
-            float f0, f1, f2, f3;
-            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y0) : "l"(two(entry(x, u, e), entry(x, u, e + 1))), "l"(scale2), "l"(base2));
-            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y1) : "l"(two(entry(x, u, e + 2), entry(x, u, e + 3))), "l"(scale2), "l"(base2));
-            untwo(y0, &f0, &f1);
-            untwo(y1, &f2, &f3);
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s0) : "l"(two(ex2(f0), ex2(f1))));
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s1) : "l"(two(ex2(f2), ex2(f3))));
-          }
-        float f0, f1, f2, f3;
-        untwo(s0, &f0, &f1);
-        untwo(s1, &f2, &f3);
-        sum = (f0 + f1) + (f2 + f3);
-        sum = fmaf(-0.6931472f * fmaf(top, scale, -base), sum, sum);
-      } else {
-        // a largest logit at the end of the type's range
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) sum += ex2(fmaxf(entry(x, u, e) - top, -1e30f) * fminf(scale, 1e8f));
-      }
+        for (int e = 0; e < kVec; e += 4) {
+          uint64_t y0, y1;
+          float f0, f1, f2, f3;
+          asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y0) : "l"(two(entry(x, u, e), entry(x, u, e + 1))), "l"(top2));
+          asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y1) : "l"(two(entry(x, u, e + 2), entry(x, u, e + 3))), "l"(top2));
+          asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y0) : "l"(scale2));
+          asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y1) : "l"(scale2));
+          untwo(y0, &f0, &f1);
+          untwo(y1, &f2, &f3);
+          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s0) : "l"(two(ex2(f0), ex2(f1))));
+          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s1) : "l"(two(ex2(f2), ex2(f3))));
+        }
+      float f0, f1, f2, f3;
+      untwo(s0, &f0, &f1);
+      untwo(s1, &f2, &f3);
+      sum = (f0 + f1) + (f2 + f3);
       sum = warp_sum(sum);
     }
     if (lane == 0) *it.out = {top, sum, where, 0};

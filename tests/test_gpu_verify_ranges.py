@@ -1,0 +1,47 @@
+"""mesh_transformer.sampling.verify_drafts at the ends of its ranges, against the plain form in 64 bits: tokens and counts are equal.
+
+Logarithms: a row's sum is of 32-bit exponentials, off by at most 2^-22 each and by their arguments' roundings (the difference, the
+scale twice, the product: 2^-24 each of an argument a, which counts with the share of its entry; the mean of a under the shares is at
+most log(entries) < 11, so 2^-18.5 at most), and by the roundings of at most 16 sums (2^-20): below 2^-18 together.  The
+result is rounded to 32 bits: 2^-24 of it."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_oracle
+
+pytestmark = pytest.mark.gpu
+TINY = float(np.finfo(np.float32).tiny)
+
+
+def _same(got, target, draft, tokens, accept, noise, temp):
+    out, taken, logs = (x.cpu().numpy() for x in got)
+    host = lambda x: None if x is None else x.float().cpu().numpy() if x.is_floating_point() else x.cpu().numpy()
+    target, draft, tokens, accept, noise = (host(x) for x in (target, draft, tokens, accept, noise))
+    for b in range(len(out)):
+        want, k, lp = cache_oracle.verify(target[b], None if draft is None else draft[b], tokens[b], accept[b], noise[b], float(np.float32(temp)))
+        assert int(taken[b]) == k, b
+        assert out[b].tolist() == want + [-1] * (out.shape[1] - len(want)), b
+        assert (np.abs(logs[b, :len(lp)] - lp) <= 2.0 ** -18 + 2.0 ** -24 * np.abs(lp)).all(), (b, logs[b], lp)
+
+
+def _uniforms(g, *shape):
+    return torch.rand(shape, generator=g, device="cuda").clamp_(min=TINY)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("offset", [0.0, 100.0, -100.0, 1e4, -1e4])
+@pytest.mark.parametrize("temp", [1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 1e-7, 1e-15, 1e-18])
+def test_low_temperatures(cuda_device, temp, offset, known, dtype):
+    """Drafts sampled at the temperature itself, logits far from zero beside their differences."""
+    from mesh_transformer.sampling import verify_drafts
+    batch, drafts, vocab = 4, 4, 1501
+    g = torch.Generator("cuda").manual_seed(int(offset) % 97 + 5)
+    target = (torch.randn((batch, drafts + 1, vocab), generator=g, device="cuda") * 2.5 + offset).to(dtype)
+    draft = (target[:, :drafts].float() + 0.7 * torch.randn((batch, drafts, vocab), generator=g, device="cuda")).to(dtype)
+    gumbel = -torch.log(-torch.log(_uniforms(g, batch, drafts, vocab).double().clamp_(max=1 - 2.0 ** -53)))
+    tokens = (draft.double() + temp * gumbel).argmax(-1).to(torch.int32)
+    accept, noise = _uniforms(g, batch, drafts), _uniforms(g, batch, vocab)
+    d = draft if known else None
+    _same(verify_drafts(target, d, tokens, accept, noise, temp=temp), target, d, tokens, accept, noise, temp)
