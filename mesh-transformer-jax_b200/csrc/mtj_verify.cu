@@ -29,6 +29,7 @@ constexpr int kPerLane = 32;
 constexpr int kChunk = 32 * kPerLane;
 constexpr int kRowBlocks = 148;            // one an SM
 constexpr int kRowBatch = 4096;            // sequences of a launch
+constexpr int kMostDrafts = 1024;          // of a sequence
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickCluster = 8;
@@ -541,7 +542,7 @@ int32_t check_args(const mtj_verify_args* a, std::string* err) {
   if (!a || !a->target_dev || !a->noise_dev || !a->tokens_out_dev || !a->accepted_out_dev) return bad("null argument");
   if (a->batch <= 0 || a->vocab <= 0 || a->drafts < 0) return bad("batch and vocab must be positive, drafts not negative");
   if (a->drafts > 0 && (!a->draft_tokens_dev || !a->accept_dev)) return bad("null argument");
-  if (a->drafts > 1024) return bad("at most 1024 drafted tokens a sequence");
+  if (a->drafts > kMostDrafts) return bad("at most 1024 drafted tokens a sequence");
   if (a->dtype != MTJ_F32 && a->dtype != MTJ_BF16) {
     *err = "dtype must be MTJ_F32 or MTJ_BF16";
     return MTJ_ERR_UNSUPPORTED;
@@ -560,6 +561,13 @@ int32_t check_args(const mtj_verify_args* a, std::string* err) {
 template <typename T>
 cudaError_t run(const mtj_verify_args& all, ChunkStat* stats, cudaStream_t s) {
   const int rows = rows_of(all), chunks = chunks_of(all);
+  // the shares of 2049 rows are 48 KB and 24 bytes, more than a kernel has without asking
+  static DeviceOnce once;
+  cudaError_t e = once.run([&] {
+    return cudaFuncSetAttribute(verify_pick_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>((2 * kMostDrafts + 1) * sizeof(RowShare)));
+  });
+  if (e != cudaSuccess) return e;
   for (int b0 = 0; b0 < all.batch; b0 += kRowBatch) {
     mtj_verify_args a = all;
     a.batch = std::min(kRowBatch, all.batch - b0);
@@ -582,7 +590,7 @@ cudaError_t run(const mtj_verify_args& all, ChunkStat* stats, cudaStream_t s) {
     int64_t row_blocks = std::min<int64_t>(kRowBlocks, (items + 5) / 6);
     if (items <= 2 * kRowBlocks * (kRowThreads / 32)) row_blocks = std::min<int64_t>(row_blocks, std::max(kRowBlocks / 2, kRowBlocks - (a.batch * cluster + 1) / 2));
     verify_rows_kernel<T><<<static_cast<unsigned>(row_blocks), kRowThreads, 0, s>>>(a, stats, rows, chunks);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.batch * cluster));

@@ -45,3 +45,24 @@ def test_low_temperatures(cuda_device, temp, offset, known, dtype):
     accept, noise = _uniforms(g, batch, drafts), _uniforms(g, batch, vocab)
     d = draft if known else None
     _same(verify_drafts(target, d, tokens, accept, noise, temp=temp), target, d, tokens, accept, noise, temp)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("drafts,known", [(1014, True), (1015, True), (1024, True), (1024, False)])
+def test_the_most_drafts(cuda_device, drafts, known, dtype):
+    """All of them taken, all but the last few, and a few: the shares of every row are in shared memory at once."""
+    from mesh_transformer.sampling import verify_drafts
+    vocab = 40
+    g = torch.Generator("cuda").manual_seed(drafts)
+    target = (torch.randn((3, drafts + 1, vocab), generator=g, device="cuda") * 2.5).to(dtype)
+    draft = target[:, :drafts].clone()
+    tokens = torch.randint(0, vocab, (3, drafts), generator=g, device="cuda").to(torch.int32)
+    accept = _uniforms(g, 3, drafts) * 1e-6 if not known else _uniforms(g, 3, drafts) * 0.9 + 0.05
+    tokens[1, drafts - 3] = -1
+    tokens[2, 5] = vocab
+    noise = _uniforms(g, 3, vocab)
+    d = draft if known else None
+    got = verify_drafts(target, d, tokens, accept.contiguous(), noise)
+    if known:                         # equal rows: whatever there is is taken (a looked-up one hangs on its own share)
+        assert got[1].tolist() == [drafts, drafts - 3, 5]
+    _same(got, target, d, tokens, accept, noise, 1.0)
