@@ -477,8 +477,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
         if (first + h * kPickThreads >= i1) break;
-        const float p = ex2(fmaxf(lp[h] - ps.top, -1e30f) * scale) * p_inv;
-        const float q = known ? ex2(fmaxf(upper[h] - qs.top, -1e30f) * scale) * q_inv : 0.f;
+        const float p = ex2((lp[h] - ps.top) * scale) * p_inv;
+        const float q = known ? ex2((upper[h] - qs.top) * scale) * q_inv : 0.f;
         const bool out = first + h * kPickThreads + tid == without;
         const float r = out ? 0.f : p - q, slack = out ? 0.f : kSlack * (p + q);
         // the wait's bounds are its own error's twice over; quotients are within 2^-21

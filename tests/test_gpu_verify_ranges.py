@@ -66,3 +66,26 @@ def test_the_most_drafts(cuda_device, drafts, known, dtype):
     if known:                         # equal rows: whatever there is is taken (a looked-up one hangs on its own share)
         assert got[1].tolist() == [drafts, drafts - 3, 5]
     _same(got, target, d, tokens, accept, noise, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("temp", [1e10, 1e28, 1e30, 1e38, 3e38])
+def test_high_temperatures(cuda_device, temp, known, dtype):
+    """All shares nearly alike, masked entries still without one: the refused token and masked entries would win the race."""
+    from mesh_transformer.sampling import verify_drafts
+    vocab = 600
+    g = torch.Generator("cuda").manual_seed(7)
+    target = (torch.randn((3, 3, vocab), generator=g, device="cuda") * 2.5).to(dtype)
+    target[..., 1::2] = float("-inf")
+    draft = target[:, :2].clone()
+    draft[..., 2::4] = float("-inf")                       # the draft has half of the target's entries
+    tokens = torch.tensor([[0, 4], [4, 8], [12, 0]], dtype=torch.int32, device="cuda")
+    accept = torch.full((3, 2), 0.75, device="cuda")
+    noise = _uniforms(g, 3, vocab)
+    noise[:, 1::2] = 1 - 2.0 ** -24
+    noise[torch.arange(3), tokens[:, 0].long()] = 1 - 2.0 ** -23
+    d = draft if known else None
+    got = verify_drafts(target, d, tokens, accept, noise, temp=temp)
+    assert got[1].tolist() == [0, 0, 0]
+    _same(got, target, d, tokens, accept, noise, temp)
