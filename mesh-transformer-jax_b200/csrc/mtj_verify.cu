@@ -455,6 +455,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     const float p_inv = static_cast<float>(1.0 / ps.sum), q_inv = known ? static_cast<float>(1.0 / qs.sum) : 0.f;
     // on a share: its argument up to 126, rounded three times, the exponential, the sum and the product are below 2^-16 of it
     constexpr float kSlack = 1.6e-5f, kLogSlack = 4.76837158e-7f;      // 2^-21
+    // two shares below 2^-126 count as zero in 32 bits: where no difference is larger, everything is run in 64 bits
+    constexpr float kLeast = 2.35098870e-38f;                          // 2^-125
     Racer win = {0.0, 0x7fffffff, 0.f};
     auto run = [&](int i, bool difference) {
       const float l = value_at(prow, i);
@@ -483,8 +485,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
         const float r = out ? 0.f : p - q, slack = out ? 0.f : kSlack * (p + q);
         // the wait's bounds are its own error's twice over; quotients are within 2^-21
         const float late = fmaf(wait_of[h], 1.f + kLogSlack, kLogSlack), soon = fmaf(wait_of[h], 1.f - kLogSlack, -kLogSlack);
-        best = fmaxf(best, (r - slack) * (1.f - 4e-6f) * reciprocal(late));
-        upper[h] = (r + slack) * (1.f + 4e-6f) * (soon > 0.f ? reciprocal(soon) : INFINITY);
+        best = fmaxf(best, (r - slack - kLeast) * (1.f - 4e-6f) * reciprocal(late));
+        upper[h] = (r + slack + kLeast) * (1.f + 4e-6f) * (soon > 0.f ? reciprocal(soon) : INFINITY);
       }
       best = warp_max(best);
       if (lane == 0) sm_best[warp] = best;

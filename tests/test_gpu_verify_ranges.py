@@ -89,3 +89,29 @@ def test_high_temperatures(cuda_device, temp, known, dtype):
     got = verify_drafts(target, d, tokens, accept, noise, temp=temp)
     assert got[1].tolist() == [0, 0, 0]
     _same(got, target, d, tokens, accept, noise, temp)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [50, 9001])
+@pytest.mark.parametrize("temp", [1.0, 0.5])
+def test_differences_below_the_32_bit_range(cuda_device, temp, vocab, dtype):
+    """Target and draft agree on one token to the last bit of 64; what is left of the difference are shares of e^-100 to e^-300."""
+    from mesh_transformer.sampling import verify_drafts
+    g = torch.Generator("cuda").manual_seed(vocab)
+    target = torch.full((3, 2, vocab), -2000.0, device="cuda")
+    draft = torch.full((3, 1, vocab), -2000.0, device="cuda")
+    target[..., 7], draft[..., 7] = 0.0, 0.0
+    target[..., 3], draft[..., 3] = -1000.0, -280.0 * temp         # the drafted token: no share in the target
+    noise = _uniforms(g, 3, vocab) * 0.5
+    target[0, 0, 11], draft[0, 0, 11] = -100.0 * temp, -130.0 * temp                       # the one that is left
+    target[1, 0, 11:20], draft[1, 0, 11:20] = -100.0 * temp, -130.0 * temp                 # several: the race decides
+    noise[1, 14] = 0.999
+    target[2, 0, vocab - 1], draft[2, 0, vocab - 1] = -300.0 * temp, -1000.0               # a late entry, and a smaller one that waits less
+    target[2, 0, 20], draft[2, 0, 20] = -304.0 * temp, -1000.0
+    noise[2, 20], noise[2, vocab - 1] = 1 - 2.0 ** -24, 0.25
+    tokens = torch.full((3, 1), 3, dtype=torch.int32, device="cuda")
+    accept = torch.full((3, 1), 0.5, device="cuda")
+    target, draft = target.to(dtype), draft.to(dtype)
+    got = verify_drafts(target, draft, tokens, accept, noise, temp=temp)
+    assert got[0].tolist() == [[11, -1], [14, -1], [20, -1]]
+    _same(got, target, draft, tokens, accept, noise, temp)
