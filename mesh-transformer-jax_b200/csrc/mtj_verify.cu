@@ -453,8 +453,11 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     const int without = refused && !known ? tokens[taken] : -1;
     const float scale = kLog2e / temp;
     const float p_inv = static_cast<float>(1.0 / ps.sum), q_inv = known ? static_cast<float>(1.0 / qs.sum) : 0.f;
-    // on a share: its argument up to 126, rounded three times, the exponential, the sum and the product are below 2^-16 of it
-    constexpr float kSlack = 1.6e-5f, kLogSlack = 4.76837158e-7f;      // 2^-21
+    // on a share: its argument, up to 126, has the roundings of the difference, of the scale's quotient and of the product and the error of the
+    // scale's constant, 126 ln 2 (3 * 2^-24 + 2^-26) = 1.67e-5 at most; the exponential's 2^-22, the reciprocal sum's, the share's and
+    // the difference's roundings make it 1.73e-5, half of what is allowed for
+    constexpr float kSlack = 3.0517578125e-5f;                         // 2^-15
+    constexpr float kLogSlack = 4.76837158e-7f;                        // 2^-21
     // two shares below 2^-126 count as zero in 32 bits: where no difference is larger, everything is run in 64 bits
     constexpr float kLeast = 2.35098870e-38f;                          // 2^-125
     Racer win = {0.0, 0x7fffffff, 0.f};
