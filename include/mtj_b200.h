@@ -550,7 +550,9 @@ int32_t mtj_k_cache_evict(const mtj_cache_evict_args* a, mtj_stream s);
  * NaN): p_k is 1 at the first largest entry of its row, a draft is taken when it is that entry, and accept, noise and the
  * draft's logits are not used.
  * target [batch][drafts + 1][vocab], draft [batch][drafts][vocab], type `dtype`, with ld_* elements from row to row and
- * batch_* from sequence to sequence; -inf and the lowest value are shares of zero.  draft_tokens [batch][drafts] (outside
+ * batch_* from sequence to sequence; -inf and the lowest value are shares of zero.  A row with NaN or +inf in it, or with
+ * nothing above -inf, has no shares: its draft is refused, the next token then comes from p_k alone, and where it is p_k's row
+ * token 0 comes out with a logarithm that is NaN (temp 0 passes over NaN).  draft_tokens [batch][drafts] (outside
  * [0, vocab): never taken); accept [batch][drafts], noise [batch][vocab] uniforms in [tiny, 1); counts [batch] drafted
  * tokens of each sequence (NULL: drafts; clamped to [0, drafts]); temp_dev [batch], or NULL: `temp` for all.
  * tokens_out [batch][drafts + 1]: the taken tokens, the next one, -1 behind it; accepted_out [batch]; logprobs_out

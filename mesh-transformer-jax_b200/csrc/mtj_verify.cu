@@ -38,7 +38,7 @@ constexpr float kLowestTemp = 8.673617e-19f;      // 2^-60
 constexpr float kLog2e = 1.442695041f;
 
 struct ChunkStat {
-  float top, sum;      // largest entry; sum of exp((l - top) / temp) over the chunk
+  float top, sum;      // largest entry; sum of exp((l - top) / temp) over the chunk, NaN where an entry is
   int32_t at, pad;     // where it first stands (greedy)
 };
 
@@ -223,8 +223,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) verify_rows_kernel(const mtj_v
       float f0, f1, f2, f3;
       untwo(s0, &f0, &f1);
       untwo(s1, &f2, &f3);
-      sum = (f0 + f1) + (f2 + f3);
-      sum = warp_sum(sum);
+      sum = warp_sum((f0 + f1) + (f2 + f3));
+    } else {
+      // nothing above -inf; the maximum has passed over NaN
+      bool nan = false;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) nan |= entry(x, u, e) != entry(x, u, e);
+      if (__any_sync(0xffffffffu, nan)) sum = NAN;
     }
     if (lane == 0) *it.out = {top, sum, where, 0};
   };
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) verify_rows_kernel(const mtj_v
 struct RowShare {
   float top;           // largest logit of the row
   int at;              // its first place
-  double sum;          // sum of exp((l - top) / temp)
+  double sum;          // sum of exp((l - top) / temp); NaN: the row has no shares
   double log_sum;
 };
 
@@ -386,6 +393,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
       auto add = [&](const ChunkStat& s) {
         if (s.top > -INFINITY)
           sum += static_cast<double>(s.sum) * (s.top == top ? 1.0 : exp((static_cast<double>(s.top) - static_cast<double>(top)) * inv_t64));
+        else
+          sum += static_cast<double>(s.sum);       // 0 or NaN
       };
 #pragma unroll
       for (int i = 0; i < kSeen; ++i) add(seen[i]);
@@ -393,6 +402,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const mtj_
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (!(sum > 0.0)) sum = NAN;                   // a row without shares: NaN or +inf in it, or nothing above -inf
     if (lane == 0) row_share[r] = {top, greedy && top > -INFINITY ? at : 0, sum, greedy ? 0.0 : log(sum)};
   }
   __syncthreads();

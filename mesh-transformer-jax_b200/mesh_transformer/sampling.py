@@ -128,7 +128,8 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, accept, noise, coun
     Logits filtered by ``nucleaus_filter`` make it nucleus sampling.
 
     Draft k is taken while ``accept * q_k(x_k) < p_k(x_k)``.  The next token is sampled from ``max(p_k - q_k, 0)`` at the first that
-    is not, from ``p`` behind the last.  Returns device tensors, nothing is read back: tokens int32 [batch, drafts + 1] (the
+    is not, from ``p`` behind the last.  A row with NaN or +inf in it, or with nothing above -inf, has no shares: its draft is refused, and
+    where the next token hangs on a target row of that kind it is 0 with a logarithm that is NaN.  Returns device tensors, nothing is read back: tokens int32 [batch, drafts + 1] (the
     taken ones, the next one, -1 behind it), the number taken int32 [batch], and log p_k of every token that comes out float32
     [batch, drafts + 1] (0 behind the last)."""
     shape = target_logits.shape if isinstance(target_logits, torch.Tensor) else ()

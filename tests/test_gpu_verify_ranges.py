@@ -115,3 +115,44 @@ def test_differences_below_the_32_bit_range(cuda_device, temp, vocab, dtype):
     got = verify_drafts(target, draft, tokens, accept, noise, temp=temp)
     assert got[0].tolist() == [[11, -1], [14, -1], [20, -1]]
     _same(got, target, draft, tokens, accept, noise, temp)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("known", [True, False])
+@pytest.mark.parametrize("vocab", [300, 5000])
+@pytest.mark.parametrize("what", ["-inf", "nan", "inf", "all nan", "a part nan"])
+def test_rows_without_shares(cuda_device, what, vocab, known, dtype):
+    """In the target's first row, in a later one, in the row behind all drafts, and in the draft's: refused, token 0 with a logarithm that is
+    NaN where there is no distribution, the target's own where only the draft has none."""
+    from mesh_transformer.sampling import verify_drafts
+    g = torch.Generator("cuda").manual_seed(vocab)
+    target = torch.randn((4, 3, vocab), generator=g, device="cuda") * 2.5
+    draft = target[:, :2].clone()
+    tokens = torch.randint(1, 60, (4, 2), generator=g, device="cuda").to(torch.int32)
+    accept, noise = _uniforms(g, 4, 2) * (0.9 if known else 1e-9), _uniforms(g, 4, vocab)
+    bad = [target[0, 0], target[1, 1], target[2, 2], draft[3, 0]]
+    for row in bad:
+        if what == "-inf":
+            row.fill_(float("-inf"))
+        elif what == "nan":
+            row[70] = float("nan")
+        elif what == "inf":
+            row[70] = float("inf")
+        elif what == "all nan":
+            row.fill_(float("nan"))
+        else:                                               # whole chunks of it
+            row[100:].fill_(float("-inf"))
+            row[vocab - 3:].fill_(float("nan"))
+    target, draft = target.to(dtype), draft.to(dtype)
+    d = draft if known else None
+    out, taken, logs = verify_drafts(target, d, tokens, accept, noise)
+    assert taken.tolist() == [0, 1, 2, 0 if known else 2]
+    assert [int(out[b, b]) for b in range(3)] == [0, 0, 0]
+    assert [bool(torch.isnan(logs[b, b])) for b in range(3)] == [True] * 3 and not torch.isnan(logs[3]).any()
+    host = lambda x: x.float().cpu().numpy()
+    with np.errstate(all="ignore"):
+        for b in range(4):
+            want, k, lp = cache_oracle.verify(host(target[b]), host(draft[b]) if known else None, tokens[b].tolist(), host(accept[b]), host(noise[b]), 1.0)
+            assert out[b].tolist() == want + [-1] * (3 - len(want))
+            near = np.abs(host(logs[b])[:len(lp)] - lp) <= 2.0 ** -18 + 2.0 ** -24 * np.abs(lp)
+            assert (near | np.isnan(lp)).all()
