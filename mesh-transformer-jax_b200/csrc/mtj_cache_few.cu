@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
     const int b = sequence_of(first_piece, a.c.batch, blockIdx.x);
     const FewSeq s = few_seq<kKeys>(a, held[b]);
     const int n = (first_piece[b + 1] - first_piece[b]) / units, rest = blockIdx.x - first_piece[b], unit = rest / n, k = rest - unit * n;
-    begin = prefix[b] + unit * s.tiles + s.tiles * k / n;
-    end = prefix[b] + unit * s.tiles + s.tiles * (k + 1) / n;
+    begin = prefix[b] + unit * s.tiles + unit_piece_begin(s.tiles, n, k);
+    end = prefix[b] + unit * s.tiles + unit_piece_begin(s.tiles, n, k + 1);
     if (s.tiles == 0) {                              // rows that see nothing
       const int kvh = unit / row_tiles, row0 = unit % row_tiles * kRows;
       const float zero[8] = {};

@@ -21,6 +21,9 @@ struct CacheFewArgs {
   float2* lse;                             // [units][tile rows] of units that one block had, with weights
   float* scores;                           // [tiles][keys][score_rows] (base 2), with weights
 };
+// Tile where piece k of the n of a unit begins, the unit's end for k = n: floor(tiles k / n).  The product itself leaves 32 bits in
+// units of more than 2^31 / 296 tiles, 2^27 slots of 256-wide heads.
+__host__ __device__ __forceinline__ int unit_piece_begin(int tiles, int n, int k) { return tiles / n * k + tiles % n * k / n; }
 struct CacheFewPlan {
   int tokens, batch, tile_rows, pieces, score_rows, aligned, whole, least, teams;
   int64_t prefix_off, units_off, ml_off, o_off, lse_off, scores_off, total;
