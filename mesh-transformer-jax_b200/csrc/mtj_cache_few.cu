@@ -778,10 +778,10 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
   const FewSeq s = few_seq<kKeys>(a, few_held(a, b, false));
   pdl_wait();
   pdl_launch_dependents();
-  // the blocks that worked on a unit: the first one and how many
+  // the blocks that worked on a unit: the first one and how many (0: a wait ran out, and which they were is not known)
   auto blocks_of = [&](int unit, int* n) {
     const int2 ends = *reinterpret_cast<const int2*>(a.unit_blocks + 2 * (b * units + unit));
-    *n = ends.y - ends.x + 1;
+    *n = unit_blocks_of(ends.x, ends.y, a.pieces);
     return ends.x;
   };
 
@@ -798,6 +798,12 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
     int n;
     const int fb = blocks_of(unit, &n);
     if (n == 1) return;                                                  // one block had it all
+    if (n == 0) {
+      const float zero[8] = {};
+      if (tid < DH / 8) store8(out + tid * 8, zero, 0.f);
+      if (tid == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
+      return;
+    }
     auto part_of = [&](int k) { return (static_cast<size_t>(fb + k) * 2 + (k == 0 ? 1 : 0)) * tile_rows + r; };
     float top = -INFINITY;
     for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[part_of(k)].x);
@@ -864,6 +870,10 @@ __global__ void __launch_bounds__(kJoinThreads, 4) cache_join_kernel(const Cache
       if (fours && at_key[i] >= 0) head[i] = *reinterpret_cast<const float4*>(scores + static_cast<size_t>(at_key[i]) * a.score_rows);
     int n;
     const int fb = blocks_of(unit, &n);
+    if (n == 0) {
+      if (tid == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
+      continue;
+    }
     __syncthreads();                                                     // the tile before has been worked off
     for (int r = warp; r < live; r += kJoinThreads / 32) {
       float top = -INFINITY, l = 0.f;
@@ -1041,6 +1051,7 @@ cudaError_t run_cache_few(const mtj_cache_attn_args& c, const CacheFewPlan& p, c
       a.whole = p.whole;
       a.least = p.least;
       a.teams = p.teams;
+      a.pieces = p.pieces;
       a.prefix = reinterpret_cast<int32_t*>(scratch + p.prefix_off);
       a.unit_blocks = reinterpret_cast<int32_t*>(scratch + p.units_off);
       a.part_ml = reinterpret_cast<float2*>(scratch + p.ml_off);

@@ -14,6 +14,7 @@ struct CacheFewArgs {
   int score_rows;                          // rows of a key's scores
   int aligned, whole;                      // pieces end where units do; every unit is one piece
   int least, teams;                        // tiles of a piece at least, and the multiple that it is of
+  int pieces;                              // blocks of the launch
   int32_t* prefix;                         // [kFewBatch + 1] tiles before each sequence
   int32_t* unit_blocks;                    // [units][2] the first and the last block that worked on a unit
   float2* part_ml;                         // [pieces][2][tile rows]: maximum (base 2), sum
@@ -24,6 +25,11 @@ struct CacheFewArgs {
 // Tile where piece k of the n of a unit begins, the unit's end for k = n: floor(tiles k / n).  The product itself leaves 32 bits in
 // units of more than 2^31 / 296 tiles, 2^27 slots of 256-wide heads.
 __host__ __device__ __forceinline__ int unit_piece_begin(int tiles, int n, int k) { return tiles / n * k + tiles % n * k / n; }
+// How many blocks worked on a unit, from what its first and its last one wrote down; 0 where they did not both: a block whose wait ran out
+// leaves out the rest of its piece, and the scratch holds anything there.
+__host__ __device__ __forceinline__ int unit_blocks_of(int first, int last, int pieces) {
+  return first >= 0 && first <= last && last < pieces ? last - first + 1 : 0;
+}
 struct CacheFewPlan {
   int tokens, batch, tile_rows, pieces, score_rows, aligned, whole, least, teams;
   int64_t prefix_off, units_off, ml_off, o_off, lse_off, scores_off, total;
