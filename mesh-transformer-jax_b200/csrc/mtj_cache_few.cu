@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
 
   if (warp == kWorkers) {
     // ---- producer ----
-    int st = 0;
+    int st = 0, issued = 0;                          // stage, tiles so far
     uint32_t phase = 1;                              // a fresh barrier counts as having passed the phase before its first
     bool ok = true;
     for (int x0 = begin; ok && x0 < end; x0 += 32) {
@@ -381,13 +381,18 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) break;
+        ++issued;
         if (++st == kStages) {
           st = 0;
           phase ^= 1;
         }
       }
     }
-    if (!ok && lane == 0 && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
+    if (lane == 0) {
+      if (!ok && a.c.status_dev) atomicOr(a.c.status_dev, kDevErrTimeout);
+      // the last round of tiles has landed before the block leaves, also where the warps that should have waited for them gave up
+      for (int i = max(0, issued - kStages); i < issued; ++i) mbar_settle(full_bar(i % kStages), (i / kStages) & 1);
+    }
     return;
   }
 
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_few_kernel(const __grid_
     for (int i = 0; i < n_tiles && arrived; ++i, ++count) {
       if (count % C::kTeams != team) continue;
       const int st = count % kStages;
-      arrived = mbar_wait(full_bar(st), (count / kStages) & 1);
+      arrived = __all_sync(0xffffffffu, mbar_wait(full_bar(st), (count / kStages) & 1)) != 0;      // the warp goes on or ends as one
       if (!arrived) break;
       const int slot0 = tile_slot[st] + key0;
       if (tile_slot[st] >= 0) {

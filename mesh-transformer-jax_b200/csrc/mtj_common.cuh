@@ -114,6 +114,10 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 }
 // Bounded wait: returns false (instead of spinning forever) if the phase does
 // not complete; the caller records kDevErrTimeout and carries on.
+#ifndef MTJ_WAIT_POLLS
+#define MTJ_WAIT_POLLS (1 << 18)           // a build whose waits run out has fewer
+#endif
+template <int POLLS = MTJ_WAIT_POLLS>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   {
     // a phase that is already complete is seen without the (possibly suspending) try_wait
@@ -127,7 +131,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     if (done) return true;
   }
-  for (int i = 0; i < (1 << 18); ++i) {
+  for (int i = 0; i < POLLS; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -140,6 +144,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   }
   return false;
 }
+// The chance that a copy in flight is given to land before its block leaves, whatever the limit of the waits that ran out.
+__device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) { mbar_wait<(1 << 18)>(bar, parity); }
 __device__ __forceinline__ uint64_t l2_evict_first_policy() {
   uint64_t pol;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
