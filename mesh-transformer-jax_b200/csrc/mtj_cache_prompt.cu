@@ -162,6 +162,15 @@ __device__ __forceinline__ void arrive_first(uint32_t bar) {
       ::"r"(bar)
       : "memory");
 }
+// 1 into a word of the other block of the pair
+__device__ __forceinline__ void set_in_other(uint32_t word, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 x;\n\t"
+      "mapa.shared::cluster.u32 x, %0, %1;\n\t"
+      "st.shared::cluster.u32 [x], 1;\n\t}"
+      ::"r"(word), "r"(rank ^ 1u)
+      : "memory");
+}
 // shared-memory matrix descriptor, 128-byte swizzle; lbo / sbo in bytes
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16 |
@@ -594,7 +603,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   using C = PromptCfg<DH>;
   constexpr int kTiles = C::kTiles, kKeysThread = C::kKeysThread, kHalves = C::kHalves;
   constexpr bool kPair = C::kPair;
-  constexpr int kBars = 2 + 2 * C::kKSlots + 2 * C::kVSlots + 10, kPeerBars = kPair ? 1 + C::kKSlots + C::kVSlots : 0;
+  constexpr int kBars = 2 + 2 * C::kKSlots + 2 * C::kVSlots + 11, kPeerBars = kPair ? 1 + C::kKSlots + C::kVSlots : 0;
   extern __shared__ __align__(1024) unsigned char prompt_smem[];
   __shared__ __align__(8) uint64_t bars[kBars + kPeerBars];
   __shared__ uint32_t tmem_slot, failed;
@@ -607,11 +616,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t q_full = bar0, q_empty = bar0 + 8, k_full = bar0 + 16, k_empty = k_full + 8 * C::kKSlots, v_full = k_empty + 8 * C::kKSlots,
                  v_empty = v_full + 8 * C::kVSlots, s_full = v_empty + 8 * C::kVSlots, p_full = s_full + 16, p_half = p_full + 16,
-                 o_done = p_half + 16, o_free = o_done + 16;
+                 o_done = p_half + 16, o_free = o_done + 16, settled = o_free + 16;
   // the first block of a pair: the other one has its part
   const uint32_t q_peer = bar0 + 8 * kBars, k_peer = q_peer + 8, v_peer = k_peer + 8 * C::kKSlots;
   const uint32_t rank = kPair ? pair_rank() : 0;
   const int piece = kPair ? blockIdx.x >> 1 : blockIdx.x;
+  auto give_up = [&]() {                               // a wait of this thread ran out: known to the block, or both of the pair
+    atomicOr(&failed, 1u);
+    if constexpr (kPair) set_in_other(smem_u32(&failed), rank);
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars + kPeerBars; ++i) mbar_init(bar0 + 8u * i, 1);
     for (int i = 0; i < 2; ++i) {
@@ -649,7 +662,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
     if (warp == 8) {
       // ---- TMA ----
       if (lane == 0 && work) {
-        int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far
+        int kc = 0, vc = 0, seg = 0;                         // key blocks, value slots and jobs so far, as they have been asked for
         constexpr int kKChunk = C::kKPages * kPageTokens * 128;      // bytes of 64 columns of a slot of keys
         const int v_chunk0 = kPair ? rank * C::kVChunks : 0;
         uint32_t storing_k = 0, storing_v = 0;               // slots with rows to store
@@ -687,6 +700,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
             for (int c = 0; c < C::kChunks; ++c)
               tma_box(sQ + (t * C::kChunks + c) * (kRowsT * 128), &map_q, (head0 + (a.by_heads ? t + rank : 0)) * DH + c * 64,
                       w.b * a.c.tokens + w.k.t_first + (a.by_heads ? 0 : (t + rank) * kRowsT), q_full);
+          ++seg;
           const int32_t* table = a.c.page_table_dev + static_cast<size_t>(w.b) * a.c.pages;
           // a key block's pages, or its rows of new tokens: the row where each 64 begin, how many hold something, the page they are stored
           // to; looked up before the slot is waited for, because the products wait for what comes behind that
@@ -784,7 +798,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
             if (ok) ok = load_v(now);
             now = then;
           }
-          ++seg;
         } while (ok && w.next(a));
         // what the last round of slots holds
         for (int n = max(0, kc - C::kKSlots); ok && n < kc; ++n) {
@@ -796,7 +809,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           if (ok && (storing_v >> (n % C::kVSlots) & 1u)) store_v(n % C::kVSlots);
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        if (!ok) atomicOr(&failed, 1u);
+        if (!ok) {
+          // what was asked for lands before the block leaves
+          for (int n = max(0, kc - C::kKSlots); n < kc; ++n) mbar_settle(k_full + 8 * (n % C::kKSlots), (n / C::kKSlots) & 1);
+          for (int n = max(0, vc - C::kVSlots); n < vc; ++n) mbar_settle(v_full + 8 * (n % C::kVSlots), (n / C::kVSlots) & 1);
+          if (seg > 0) mbar_settle(q_full, (seg - 1) & 1);
+          give_up();
+        }
       }
     } else if (warp == 9) {
       // ---- products ----
@@ -817,7 +836,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
               tell(v_full, v_peer, vc++, C::kVSlots);
             }
           } while (ok && w.next(a));
-          if (!ok) atomicOr(&failed, 1u);
+          if (!ok) give_up();
         }
       } else if (work) {
         const uint32_t leader = elected();
@@ -899,7 +918,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
           u0 += units;
           ++seg;
         } while (__any_sync(0xffffffffu, ok && w.next(a)));
-        if (!ok && leader) atomicOr(&failed, 1u);
+        if (!ok && leader) give_up();
       }
     } else if (warp >= 10) {
       // ---- the new rows into their slots ----
@@ -1084,13 +1103,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache_prompt_kernel(const _
         if (!whole && part == 0) a.part_ml[part_row] = make_float2(m_ref, l);
         announce(o_free + 8 * tile);
       } while (w.next(a));
-      if (!ok) atomicOr(&failed, 1u);
+      if (!ok) give_up();
     }
     if (a.c.k_new_dev) store_rows<DH>(a, 2 + warp);
   }
   fence_before();
   if constexpr (kPair) pair_sync();                    // neither block leaves, or frees, while the other may still signal it
   else __syncthreads();
+  if (failed) {
+    // products may still be reading shared memory and tensor memory, which nobody has waited for: they end before either is given back
+    if (warp == 9 && rank == 0) {
+      const uint32_t leader = elected();
+      if constexpr (kPair) commit_pair(settled, leader);
+      else commit_to(settled, leader);
+      mbar_settle(settled, 0);
+    }
+    if constexpr (kPair) pair_sync();
+    else __syncthreads();
+  }
   if (warp == 9) {
     fence_after();
     if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");

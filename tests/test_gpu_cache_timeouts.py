@@ -12,7 +12,7 @@ from cache_util import PAGE
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "mesh-transformer-jax_b200", "csrc")
-UNITS = ("mtj_cache_attn", "mtj_cache_few")
+UNITS = ("mtj_cache_attn", "mtj_cache_few", "mtj_cache_prompt")
 
 
 @pytest.fixture(scope="module")
@@ -83,3 +83,13 @@ def _run(monkeypatch, impatient, batch, heads, kv_heads, d_head, tokens, length,
 ])
 def test_few_tokens(cuda_device, monkeypatch, impatient, batch, heads, kv_heads, d_head, tokens, length, weighed, dtype):
     _run(monkeypatch, impatient, batch, heads, kv_heads, d_head, tokens, length, dtype, weighed)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,d_head,tokens,length", [
+    (1, 32, 8, 128, 2000, 2000),      # whole jobs
+    (2, 8, 2, 64, 333, 5003),         # pieces that are joined
+    (1, 16, 16, 256, 2047, 2047),     # pairs of blocks
+    (3, 6, 2, 256, 200, 3000),
+])
+def test_prompts(cuda_device, monkeypatch, impatient, batch, heads, kv_heads, d_head, tokens, length):
+    _run(monkeypatch, impatient, batch, heads, kv_heads, d_head, tokens, length, torch.bfloat16, False)
