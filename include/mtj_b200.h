@@ -480,7 +480,8 @@ int32_t mtj_k_decode_attn_noalloc(const float* q_dev, const void* kpool_dev, con
  * out become zeros; those of k_new and v_new are not used.  Slots behind lengths[b] are never read into a result.
  * weights_out_dev [batch][kv_heads][pages * 64] f32 (or NULL) receives for every slot j < lengths[b]
  *     (j new ? 0 : weights_in_dev[j]) + sum of a_j over the call's tokens and the heads of the group,
- * weights_in_dev NULL standing for zeros; both may be the same array.
+ * weights_in_dev NULL standing for zeros; both may be the same array.  (Of drafted tokens that are refused later the shares
+ * stay in older slots: such calls go without, and a second one with the tokens that were taken adds theirs.)
  * A sequence whose length is negative, below its new_tokens or beyond its pages is treated as empty, a page number outside
  * [0, n_pages) as a page that nobody sees; either sets bit 1 of *status_dev (may be NULL), a bounded wait that runs out
  * bit 0.  A slot that none of a sequence's new tokens sees may hold anything and its page need not exist (page_table -1);

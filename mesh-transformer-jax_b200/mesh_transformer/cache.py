@@ -81,6 +81,8 @@ def cache_attention(q, k, v, kpool, vpool, page_table, lengths, new=None, window
     ``weights`` float32 [batch, kv_heads, pages * 64]: the attention weight that each slot receives, summed over the tokens and
     over the query heads that read its head, is added to it, slots of new tokens beginning at zero.  With ``weights_out`` the
     sums go there and ``weights`` (may be None: zeros) stays as it is.
+    What drafted tokens add to older slots is not taken back with their own slots.  Weights of taken tokens alone: attend without, check the drafts,
+    and call again with the lengths as they are then, ``new`` the number taken plus one, the same ``q`` and no ``k`` and ``v``.
 
     ``out`` [batch, tokens, heads, d_head], if given, is written instead of a new tensor.  It shares no memory with the others,
     nor do ``weights`` and ``weights_out`` unless they are the same.
