@@ -514,7 +514,8 @@ int32_t mtj_k_cache_attn(const mtj_cache_attn_args* a, void* scratch_dev, int64_
 
 /* No counterpart in the reference.  Eviction from such a cache by accumulated attention weight: every key head of a
  * sequence that holds more than `keep` slots keeps its first `first` slots, its last `last` slots and of the others the
- * keep - first - last with the largest weights (the lower slot among equals), in the order of their slots.  The kept keys
+ * keep - first - last with the largest weights (the lower slot among equals; NaN is larger than any number, with its sign
+ * set smaller), in the order of their slots.  The kept keys
  * and values are copied to slots 0 .. keep - 1 of the sequence's spare pages, which its row of the new table names, with -1
  * behind them.  Other sequences keep their pages.
  *   kept_out [batch][kv_heads][keep]: the slots that were kept, -1 behind the last one;

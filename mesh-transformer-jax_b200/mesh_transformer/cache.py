@@ -156,7 +156,8 @@ def _run_attention(a, kpool, index):
 
 def cache_evict(kpool, vpool, page_table, lengths, weights, spare_pages, keep, first=0, last=0, status=None):
     """Cuts every sequence that holds more than ``keep`` slots down to ``keep``: each key head keeps the ``first`` first slots, the
-    ``last`` last ones and the heaviest by ``weights`` of the others (the lower slot among equals), in the order of their slots.
+    ``last`` last ones and the heaviest by ``weights`` of the others (the lower slot among equals; NaN counts as heavier than any number),
+    in the order of their slots.
 
     The kept keys and values are copied to ``spare_pages`` int32 [batch, ceil(keep / 64)], pages that no sequence uses, each
     named once.  Returns ``(kept, lengths, weights, page_table)``, new tensors: the slots that were kept [batch, kv_heads, keep]

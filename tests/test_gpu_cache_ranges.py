@@ -39,3 +39,26 @@ def test_a_sequence_of_very_many_slots(cuda_device, d_head, pages, tokens):
     a = torch.softmax(scores.masked_fill((slots[None, :] > p[:, None])[:, None], float("-inf")), -1)
     want, spread = a @ values, a @ values.abs()
     assert ((out[0].double() - want).abs() <= rounding(torch.bfloat16) * want.abs() + 2.0 ** -8 * spread).all()
+
+
+@pytest.mark.parametrize("length", [200, 20000])
+def test_eviction_by_weights_that_are_not_numbers(cuda_device, length):
+    """NaN is heavier than any number, infinities included, and equals itself: the lower slot first.  Exact: nothing is computed."""
+    from mesh_transformer.cache import cache_evict
+    keep, first, last, nan, inf = 60, 2, 8, float("nan"), float("inf")
+    pages = (length + PAGE - 1) // PAGE
+    g = torch.Generator("cuda").manual_seed(length)
+    pools = [torch.randn((pages + 1, 1, PAGE, 64), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    for nans in (5, 70):                                          # fewer than are kept, and more
+        weights = torch.rand((1, 1, pages * PAGE), generator=g, device="cuda")
+        at = first + torch.randperm(length - first - last, generator=g, device="cuda")[:nans + 3]
+        weights[0, 0, at] = torch.tensor([nan] * nans + [inf, inf, -inf], device="cuda")
+        ranks = torch.where(torch.isnan(weights[0, 0]), torch.full((), inf, device="cuda"), torch.where(weights[0, 0] == inf, 1e30, weights[0, 0].double()))
+        middle = ranks[first:length - last]
+        heaviest = first + torch.sort(middle, descending=True, stable=True).indices[:keep - first - last]
+        want = torch.cat([torch.arange(first, device="cuda"), heaviest, torch.arange(length - last, length, device="cuda")]).sort().values
+        kept, _, _, _ = cache_evict(*pools, table, torch.tensor([length], dtype=torch.int32, device="cuda"), weights,
+                                    torch.tensor([[pages]], dtype=torch.int32, device="cuda"), keep, first=first, last=last)
+        assert torch.equal(kept[0, 0].long(), want)
+        assert all(torch.equal(p[pages, 0, :keep], p[:pages, 0].flatten(0, 1)[want]) for p in pools)
