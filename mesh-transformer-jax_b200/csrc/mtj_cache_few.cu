@@ -11,8 +11,9 @@
 // own with its own running maximum and sum:
 //     S^T[16 keys, rows] = K Q^T     keys are the M dimension of mma.sync, so that one query row wastes 7/8 of a small N and not
 //     O^T[16 d, rows]   += V^T P^T   15/16 of M; K by ldmatrix, V by ldmatrix.trans, P transposed between the two by movmatrix
-// tcgen05 would be as empty (M is at least 64 there) and has the accumulators a trip through tensor memory away; the bound is
-// traffic.  Queries in 32 bits are the exact sum of three bf16 numbers, three products each.  The weights P go into the
+// tcgen05 takes keys as M too (64 or 128, with N from 8 rows on) and would be no emptier.  It has the scores and the weights a trip through
+// tensor and shared memory away, which one token, bound by traffic, gains nothing from; for drafted tokens, where the chain of a tile
+// counts and not the bytes, that form has not been built or measured.  Queries in 32 bits are the exact sum of three bf16 numbers, three products each.  The weights P go into the
 // product as two bf16 numbers (three for 32-bit queries), an error of 2^-16 (2^-24): one would cost as much as the rounding of
 // the output (and save 6 of 44 us with 5 drafts, 4 heads a key head and 8 sequences of up to 8191 slots).  Scores, maxima, sums and
 // outputs are 32-bit.
@@ -22,7 +23,7 @@
 // window, are zeroed in the tile, since weight zero times whatever stands there must be zero.
 //
 // 8 key heads of 128 with 4 query heads each: one token of 32 sequences of 2000 to 16383 slots 197 us, 1.21 GB at 6.1 TB/s, and 31 us for
-// the join that adds up the weights; five tokens of 8 sequences, window 4096, 38 to 41 us for 107 MB: there the chain of a tile (two products
+// the join that adds up the weights; five tokens of 8 sequences, window 4096, 39 us for 107 MB: there the chain of a tile (two products
 // with a softmax between them, 20 rows) and the ragged ends of 64 units count, not the bytes.
 #include <cuda.h>
 #include <math.h>

@@ -13,8 +13,8 @@
 // and units go round two score buffers: one thread issues S0 S1 | PV0 S2 | PV1 S3 | ..., so that while one warp group works out the
 // weights of a unit, the tensor cores have the other unit's products.  For d_head 128 a unit is 1024 cycles of products and, at 16
 // exponentials a cycle less the quarter that the multiply-add units take, 768 of exponentials; the chain of a tile (scores, maximum,
-// weights, products, next scores) is what is left in the open.  32 heads of 128, 8 key heads, 8191 tokens, window 4096: 0.39 ms, 1060
-// TFLOP/s of visible pairs, 0.45 ms (925) in a row of calls, where the SMs run at 1.6 GHz; tensor pipe 54 % active.  16 heads of 256, 2047
+// weights, products, next scores) is what is left in the open.  32 heads of 128, 8 key heads, 8191 tokens, window 4096: 0.40 ms, 1040
+// TFLOP/s of visible pairs, 0.445 ms (925) in a row of calls, where the SMs run at 1.6 GHz; tensor pipe 54 % active.  16 heads of 256, 2047
 // tokens, window 1024: 49 us, 41 %.  Built and measured at the first of these, none ahead by more than 2 %: score buffers of 64 keys, two a tile, so that
 // no tile waits for its scores (386 us from a warp of products a tile, 528 from one for both); two threads a row for 128-wide heads (407);
 // pairs of blocks for them (414); a warp of products a tile with buffers of 128 (460: the tiles' products get in each other's way).
@@ -33,7 +33,7 @@
 // term would be half as many products again).  O is rescaled when a row's scores have outgrown its reference, which waits for the
 // products before.  The rows of V behind the sequence, of a page that does not exist, or that no token of the job sees, are zeroed in
 // shared memory before they meet their zero weights.
-// Every wait is bounded.
+// Every wait is bounded; where one runs out, what is in flight has landed and ended before a block leaves.
 #include <cuda.h>
 #include <math.h>
 
@@ -210,8 +210,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x of a pair on the multiply-add units, for x in [-126, 9]: x = n + f with |f| <= 1/2 by adding and taking away 1.5 * 2^23, a
-// polynomial of degree 3 in f (fitted to the relative error, 8e-5 at most: a twentieth of the rounding to bf16 that follows),
+// 2^x of a pair on the multiply-add units, for x in [-126, 9]: x = n + f with |f| <= 1/2 by adding and taking away 1.5 * 2^23 (the
+// reduction of Cody and Waite), a polynomial of degree 3 in f (fitted here to the relative error, 8e-5 at most: a twentieth of the rounding to bf16 that follows),
 // n added to its exponent
 __device__ __forceinline__ void exp2_pair(uint64_t x, float* y0, float* y1) {
   const uint64_t magic = pair_of(12582912.f, 12582912.f);

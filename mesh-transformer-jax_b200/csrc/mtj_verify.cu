@@ -4,13 +4,16 @@
 //   first stands) and the sum of exp((l - maximum) / temp).  A lane holds its entries in registers, so the maximum is known before
 //   the first exponential, and has the next ones on their way meanwhile.  The rows that take part stand in one line that is cut into
 //   equal pieces, one a warp: rows behind a sequence's drafts cost nothing.
-// verify_pick_kernel: a cluster of blocks a sequence.  Every block joins the chunks of all rows to shares, in 64 bits, and
+// verify_pick_kernel: a cluster of blocks a sequence.  Every block adds up the chunks of all rows, in 64 bits, and
 //   decides alike how many drafts are taken; then the cluster shares out the one row that the next token comes from.
 //   The race r_i / -log(noise_i) is run in 32 bits with a bound on the error of every entry; those that can win it are run
-//   again in 64 bits, so that the token does not hang on the rounding of a near-tie or of a difference of near-equal shares.  What does
+//   again in 64 bits, so that the token does not hang on the rounding of a near-tie.  What does
 //   not hang on the rows kernel (noise, the drafts' own logits) is read and worked out while that one runs.
 //
-// Bound by the bytes of the logits: 32-bit sums of exponentials of a chunk, 64-bit sums over chunks.  64 sequences of up to 7 drafts, 50400
+// What is 32-bit is the sum of a chunk's exponentials, about 1e-7 of itself off (2^-18 at most); sums over chunks, the drafts' shares, their
+// comparison and the entries that decide the race are 64-bit.  Which side of u q < p and of p > q an entry is on thus holds for shares that
+// are further apart than that; closer ones are decided by the rounding of their rows' sums.
+// Bound by the bytes of the logits.  64 sequences of up to 7 drafts, 50400
 // entries in 32 bits: 26 us for 103 MB of rows (4.0 TB/s) and 25 us for the race alone, 41 us together, since the race reads its noise and
 // takes the logarithms while the rows are read.  (With logf and divisions instead of approximations and their bounds 29 and 45 us.)
 #include <math.h>
