@@ -115,7 +115,7 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 // Bounded wait: returns false (instead of spinning forever) if the phase does
 // not complete; the caller records kDevErrTimeout and carries on.
 #ifndef MTJ_WAIT_POLLS
-#define MTJ_WAIT_POLLS (1 << 18)           // a build whose waits run out has fewer
+#define MTJ_WAIT_POLLS (1 << 18)           // behind the first look; 0 in a build that tests what a wait that runs out leaves behind
 #endif
 template <int POLLS = MTJ_WAIT_POLLS>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {

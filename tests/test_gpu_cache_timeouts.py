@@ -1,5 +1,10 @@
-"""Attention over caller-owned caches whose waits run out: a build of its kernels whose waits give up at once.  The call reports it, nothing is
-read or written outside the call's own rows and slots, copies in flight land before their blocks leave, and the next call is as ever."""
+"""Attention over caller-owned caches whose waits run out: a build of its kernels with the shortest limit, a wait that looks once.  The call
+reports it, nothing is read or written outside the call's own rows and slots, copies in flight land before their blocks leave, and the next
+call is as ever.
+
+What a block does behind a wait that ran out stays in bounds: the few-row kernel leaves its loop as one and its second kernel checks what it
+takes for an index; in the prompt kernel the warps that load and multiply stop, and the others go on over their own rows with whatever
+tensor memory holds, their waits and the block's barriers as many as ever."""
 import ctypes
 import os
 import subprocess
